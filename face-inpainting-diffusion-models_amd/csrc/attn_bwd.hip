@@ -1,0 +1,396 @@
+// Attention backward (include/ifd_ops.h): the probabilities are recomputed from q, k and the forward's log-sum-exp.
+//   p = 2^(c s - lse2), dp = dout v^T, ds = p (dp - delta), delta = rowsum(dout out)
+//   dq = scale ds k, dk = scale ds^T q, dv = p^T dout
+// Two passes, each owning its outputs, so that nothing is added atomically and the result does not depend on timing:
+// attn_bwd_q_kernel (a wave owns 32 query rows; three products per score tile) also leaves each row's lse2 and delta for
+// attn_bwd_kv_kernel (a wave owns 32 keys; four products). Seven products against the five of one pass with atomics on dq.
+#include "attn_dev.h"
+
+namespace ifd {
+
+template <typename T, int DP, int NW, int BK>
+__global__ __launch_bounds__(NW * 64) void attn_bwd_q_kernel(AttnK p) {
+  typedef AttnTile<T, DP> TL;
+  typedef typename TL::frag frag;
+  constexpr int KT = BK / 32, TB = BK * TL::ROWB;
+  extern __shared__ __attribute__((aligned(1024))) char smem[];
+  lds_c* sm = (lds_c*)smem;
+  const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, h = lane >> 5;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int BH = p.B * p.Hq;
+  int bh, qblk;
+  if (p.causal) {
+    const int r = blockIdx.x % BH;
+    qblk = p.nblk - 1 - blockIdx.x / BH;
+    bh = (BH & 7) ? r : (r & 7) * (BH >> 3) + (r >> 3);
+  } else {
+    const int id = xcd_order(blockIdx.x, BH * p.nblk);
+    bh = id / p.nblk;
+    qblk = id - bh * p.nblk;
+  }
+  const int b = bh / p.Hq, hq = bh - b * p.Hq, hk = hq / p.G;
+  const int len = seq_len(p, b), qs = q_first(p, b);
+  const int q0 = qblk * (NW * 32) + w * 32;
+  const int i = q0 + l32;
+  const bool ok = i < p.Tq;
+  const int lim = ok ? row_limit(p, qs, len, i) : 0;
+
+  frag qf[TL::KS], gf[TL::KS];
+  float delta = 0.f;
+  {
+    const char* rq = p.q + b * p.qb + hq * p.qh + (int64_t)i * p.qt;
+    const char* rg = p.dout + b * p.gb + hq * p.gh + (int64_t)i * p.gt;
+    const char* ro = p.out + b * p.ob + hq * p.oh + (int64_t)i * p.ot;
+#pragma unroll
+    for (int ks = 0; ks < TL::KS; ++ks) {
+      qf[ks] = TL::gload(rq, ok, ks, h, p.D);
+      gf[ks] = TL::gload(rg, ok, ks, h, p.D);
+      const frag of = TL::gload(ro, ok, ks, h, p.D);
+#pragma unroll
+      for (int j = 0; j < TL::CE; ++j) delta = fmaf((float)gf[ks][j], (float)of[j], delta);
+    }
+    delta += xhalf(delta);
+  }
+  float lse2 = INFINITY;  // a row that sees no key: every p is 0
+  const int64_t srow = ((int64_t)b * p.Hq + hq) * p.Tq + i;
+  if (ok) {
+    const float l = p.lse[srow];
+    if (l != -INFINITY) lse2 = l * 1.4426950408889634f;
+    if (lim == 0) delta = 0.f;
+    if (h == 0) {
+      p.ws[srow] = lse2;
+      p.ws[(int64_t)p.B * p.Hq * p.Tq + srow] = delta;
+    }
+  }
+  f32x16 acc[TL::DT];
+#pragma unroll
+  for (int d = 0; d < TL::DT; ++d)
+#pragma unroll
+    for (int x = 0; x < 16; ++x) acc[d][x] = 0.f;
+
+  const int last = min(p.Tq, (qblk + 1) * (NW * 32)) - 1;
+  const int wg_end = row_limit(p, qs, len, last);
+  const int w_last = min(p.Tq, q0 + 32) - 1;
+  const int w_end = __builtin_amdgcn_readfirstlane(w_last < q0 ? 0 : row_limit(p, qs, len, w_last));
+  const int w_all = __builtin_amdgcn_readfirstlane(w_last < q0 ? 0 : row_limit(p, qs, len, q0));
+  const int nt = (wg_end + BK - 1) / BK;
+  AttnStage<T, DP, BK, NW> sg;
+  sg.init(w, lane, p.D);
+  const char* kp = p.k + b * p.kb + hk * p.kh;
+  const char* vp = p.v + b * p.vb + hk * p.vh;
+  auto stage = [&](int t) {
+    const int k0 = t * BK, n = min(BK, len - k0);
+    lds_c* d = sm + (t & 1) * (2 * TB);
+    sg.load(kp + (int64_t)k0 * p.kt, p.kt, n, d, w);
+    sg.load(vp + (int64_t)k0 * p.vt, p.vt, n, d + TB, w);
+  };
+  if (nt > 0) {
+    stage(0);
+    dma_wait();
+    __syncthreads();
+  }
+  for (int t = 0; t < nt; ++t) {
+    if (t + 1 < nt) stage(t + 1);
+    const lds_c* kb = sm + (t & 1) * (2 * TB);
+    const lds_c* vb = kb + TB;
+    const int k0 = t * BK;
+    if (k0 < w_end) {
+      const bool mask = k0 + BK > w_all;
+#pragma unroll
+      for (int kt = 0; kt < KT; ++kt) {
+        f32x16 s, dp;
+#pragma unroll
+        for (int x = 0; x < 16; ++x) s[x] = dp[x] = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < TL::KS; ++ks) {
+          s = TL::A::mma(TL::row(kb, kt * 32, ks, l32, h), qf[ks], s);
+          dp = TL::A::mma(TL::row(vb, kt * 32, ks, l32, h), gf[ks], dp);
+        }
+        if (mask) {
+#pragma unroll
+          for (int x = 0; x < 16; ++x)
+            if (k0 + kt * 32 + 8 * (x >> 2) + 4 * h + (x & 3) >= lim) s[x] = -INFINITY;
+        }
+#pragma unroll
+        for (int x = 0; x < 16; ++x) s[x] = __builtin_amdgcn_exp2f(fmaf(s[x], p.c, -lse2)) * (dp[x] - delta);
+#pragma unroll
+        for (int ps = 0; ps < TL::PS; ++ps) {
+          const frag f = TL::pack(s, ps);
+#pragma unroll
+          for (int d = 0; d < TL::DT; ++d) acc[d] = TL::A::mma(TL::col(kb, kt * 32, ps, d, lane), f, acc[d]);
+        }
+      }
+    }
+    dma_wait();
+    __syncthreads();
+  }
+  if (!ok) return;
+  T* op = reinterpret_cast<T*>(p.dq + b * p.dqb + hq * p.dqh + (int64_t)i * p.dqt);
+#pragma unroll
+  for (int d = 0; d < TL::DT; ++d)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int ch = d * 32 + 8 * j + 4 * h;
+      if (ch >= p.D) continue;
+      f32x4 v;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = acc[d][4 * j + e] * p.scale;
+      *reinterpret_cast<typename TL::A::quad*>(op + ch) = __builtin_convertvector(v, typename TL::A::quad);
+    }
+}
+
+// A workgroup owns NW * 32 keys of one key-value head and walks over the (query head, row tile) pairs of its share:
+// with nsplit > 1 the pairs are dealt to nsplit workgroups, whose fp32 sums attn_bwd_join_kernel adds in order.
+template <typename T, int DP, int NW, int BQ>
+__global__ __launch_bounds__(NW * 64) void attn_bwd_kv_kernel(AttnK p) {
+  typedef AttnTile<T, DP> TL;
+  typedef typename TL::frag frag;
+  constexpr int QT = BQ / 32, TB = BQ * TL::ROWB, BUF = 2 * TB + 1024;  // Q, dout, lse2[BQ], delta[BQ]
+  extern __shared__ __attribute__((aligned(1024))) char smem[];
+  lds_c* sm = (lds_c*)smem;
+  const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, h = lane >> 5;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int id = xcd_order(blockIdx.x, gridDim.x);
+  // one key block's shares are neighbours: they read the same rows
+  const int sp = id % p.nsplit;
+  const int kblk = (id / p.nsplit) % p.nblk, bh = id / p.nsplit / p.nblk;
+  const int b = bh / p.Hk, hk = bh - b * p.Hk;
+  const int len = seq_len(p, b), qs = q_first(p, b);
+  const int kb0 = kblk * (NW * 32), key = kb0 + w * 32 + l32;
+  const bool ok = key < len;
+  // rows [lo, Tq) see this lane's key, [wg_lo, Tq) some key of the workgroup
+  auto first_row = [&](int k) {
+    const int64_t n = p.causal ? (int64_t)k - qs : 0;
+    return n < 0 ? 0 : (n > p.Tq ? p.Tq : (int)n);
+  };
+  const int lo = first_row(key), wg_lo = first_row(kb0);
+  const int w_lo = __builtin_amdgcn_readfirstlane(first_row(kb0 + w * 32));
+  const int w_hi = __builtin_amdgcn_readfirstlane(first_row(kb0 + w * 32 + 31));
+
+  frag kf[TL::KS], vf[TL::KS];
+  {
+    const char* rk = p.k + b * p.kb + hk * p.kh + (int64_t)key * p.kt;
+    const char* rv = p.v + b * p.vb + hk * p.vh + (int64_t)key * p.vt;
+#pragma unroll
+    for (int ks = 0; ks < TL::KS; ++ks) {
+      kf[ks] = TL::gload(rk, ok, ks, h, p.D);
+      vf[ks] = TL::gload(rv, ok, ks, h, p.D);
+    }
+  }
+  f32x16 dk[TL::DT], dv[TL::DT];
+#pragma unroll
+  for (int d = 0; d < TL::DT; ++d)
+#pragma unroll
+    for (int x = 0; x < 16; ++x) dk[d][x] = dv[d][x] = 0.f;
+
+  const int tq0 = wg_lo / BQ, ntq = kb0 < len && wg_lo < p.Tq ? (p.Tq + BQ - 1) / BQ - tq0 : 0;
+  const int64_t all = (int64_t)ntq * p.G;
+  const int it0 = (int)(all * sp / p.nsplit), it1 = (int)(all * (sp + 1) / p.nsplit);
+  AttnStage<T, DP, BQ, NW> sg;
+  sg.init(w, lane, p.D);
+  auto stage = [&](int it, int buf) {
+    const int hq = hk * p.G + it / ntq, r0 = (tq0 + it % ntq) * BQ, n = min(BQ, p.Tq - r0);
+    lds_c* d = sm + buf * BUF;
+    sg.load(p.q + b * p.qb + hq * p.qh + (int64_t)r0 * p.qt, p.qt, n, d, w);
+    sg.load(p.dout + b * p.gb + hq * p.gh + (int64_t)r0 * p.gt, p.gt, n, d + TB, w);
+    if (w < 2) {  // lse2 by wave 0, delta by wave 1
+      const float* st = p.ws + (w ? (int64_t)p.B * p.Hq * p.Tq : 0) + ((int64_t)b * p.Hq + hq) * p.Tq + r0;
+      dma_word(st, 4 * min(lane, n - 1), d + 2 * TB + w * 512);
+    }
+  };
+  if (it0 < it1) {
+    stage(it0, 0);
+    dma_wait();
+    __syncthreads();
+  }
+  int buf = 0;
+  for (int it = it0; it < it1; ++it, buf ^= 1) {
+    if (it + 1 < it1) stage(it + 1, buf ^ 1);
+    const lds_c* qb = sm + buf * BUF;
+    const lds_c* gb = qb + TB;
+    const int r0 = (tq0 + it % ntq) * BQ;
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) {
+      const int rr = r0 + qt * 32;
+      if (rr + 32 <= w_lo || rr >= p.Tq) continue;
+      f32x16 s, dp;
+#pragma unroll
+      for (int x = 0; x < 16; ++x) s[x] = dp[x] = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < TL::KS; ++ks) {
+        s = TL::A::mma(TL::row(qb, qt * 32, ks, l32, h), kf[ks], s);
+        dp = TL::A::mma(TL::row(gb, qt * 32, ks, l32, h), vf[ks], dp);
+      }
+      const bool mask = rr < w_hi || rr + 32 > p.Tq;
+#pragma unroll
+      for (int y = 0; y < 4; ++y) {
+        const f32x4 ls = lds_quad(qb + 2 * TB + 4 * (qt * 32 + 8 * y + 4 * h));
+        const f32x4 de = lds_quad(qb + 2 * TB + 512 + 4 * (qt * 32 + 8 * y + 4 * h));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int x = 4 * y + e, r = rr + 8 * y + 4 * h + e;
+          float pv = __builtin_amdgcn_exp2f(fmaf(s[x], p.c, -ls[e]));
+          if (mask && (r < lo || r >= p.Tq)) pv = 0.f;
+          float dsv = pv * (dp[x] - de[e]);
+          if (mask && (r < lo || r >= p.Tq)) dsv = 0.f;
+          s[x] = pv;
+          dp[x] = dsv;
+        }
+      }
+#pragma unroll
+      for (int ps = 0; ps < TL::PS; ++ps) {
+        const frag fp = TL::pack(s, ps), fd = TL::pack(dp, ps);
+#pragma unroll
+        for (int d = 0; d < TL::DT; ++d) {
+          dv[d] = TL::A::mma(TL::col(gb, qt * 32, ps, d, lane), fp, dv[d]);
+          dk[d] = TL::A::mma(TL::col(qb, qt * 32, ps, d, lane), fd, dk[d]);
+        }
+      }
+    }
+    dma_wait();
+    __syncthreads();
+  }
+  if (key >= p.Tk) return;
+  if (p.nsplit > 1) {
+    if (!ok) return;
+    float* po = p.ws + 2 * (int64_t)p.B * p.Hq * p.Tq + ((((int64_t)b * p.Hk + hk) * p.nsplit + sp) * p.Tk + key) * (2 * DP);
+#pragma unroll
+    for (int d = 0; d < TL::DT; ++d)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int ch = d * 32 + 8 * j + 4 * h;
+        f32x4 a, c;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          a[e] = dk[d][4 * j + e];
+          c[e] = dv[d][4 * j + e];
+        }
+        *reinterpret_cast<f32x4*>(po + ch) = a;
+        *reinterpret_cast<f32x4*>(po + DP + ch) = c;
+      }
+    return;
+  }
+  T* ok_ = reinterpret_cast<T*>(p.dk + b * p.dkb + hk * p.dkh + (int64_t)key * p.dkt);
+  T* ov_ = reinterpret_cast<T*>(p.dv + b * p.dvb + hk * p.dvh + (int64_t)key * p.dvt);
+#pragma unroll
+  for (int d = 0; d < TL::DT; ++d)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int ch = d * 32 + 8 * j + 4 * h;
+      if (ch >= p.D) continue;
+      f32x4 a, c;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        a[e] = ok ? dk[d][4 * j + e] * p.scale : 0.f;
+        c[e] = ok ? dv[d][4 * j + e] : 0.f;
+      }
+      *reinterpret_cast<typename TL::A::quad*>(ok_ + ch) = __builtin_convertvector(a, typename TL::A::quad);
+      *reinterpret_cast<typename TL::A::quad*>(ov_ + ch) = __builtin_convertvector(c, typename TL::A::quad);
+    }
+}
+
+// dk, dv = the shares' sums in order; one thread per four channels of a (key, dk | dv) row.
+template <typename T, int DP>
+__global__ __launch_bounds__(256) void attn_bwd_join_kernel(AttnK p) {
+  typedef typename AttnT<T>::quad quad;
+  constexpr int C4 = 2 * DP / 4;
+  const int64_t g = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t row = g / C4;
+  if (row >= (int64_t)p.B * p.Hk * p.Tk) return;
+  const int c4 = (int)(g - row * C4), isv = c4 >= DP / 4, ch = 4 * (c4 - isv * (DP / 4));
+  if (ch >= p.D) return;
+  const int64_t bh = row / p.Tk;
+  const int key = (int)(row - bh * p.Tk), b = (int)(bh / p.Hk), hk = (int)(bh - (int64_t)b * p.Hk);
+  f32x4 v = {0.f, 0.f, 0.f, 0.f};
+  if (key < seq_len(p, b)) {
+    const float* w = p.ws + 2 * (int64_t)p.B * p.Hq * p.Tq + (bh * p.nsplit * p.Tk + key) * (2 * DP) + isv * DP + ch;
+    for (int s = 0; s < p.nsplit; ++s) v += *reinterpret_cast<const f32x4*>(w + (int64_t)s * p.Tk * (2 * DP));
+    if (!isv) v *= p.scale;
+  }
+  T* o = isv ? reinterpret_cast<T*>(p.dv + b * p.dvb + hk * p.dvh + (int64_t)key * p.dvt)
+             : reinterpret_cast<T*>(p.dk + b * p.dkb + hk * p.dkh + (int64_t)key * p.dkt);
+  *reinterpret_cast<quad*>(o + ch) = __builtin_convertvector(v, quad);
+}
+
+// Workgroups of the key pass: 128 keys each. The chip takes two per CU at a time and causal blocks differ in length, so
+// the walk is shared out until there are about four per CU, at least four row tiles each.
+static int kv_split(const ifd_attention_args& a) {
+  const int64_t base = (int64_t)a.B * a.Hk * cdiv(a.Tk, 128), tiles = (int64_t)(a.Hq / a.Hk) * cdiv(a.Tq, 64);
+  const int64_t n = std::min<int64_t>(cdiv(1024, std::max<int64_t>(base, 1)), std::max<int64_t>(tiles / 4, 1));
+  return (int)std::min<int64_t>(n, 16);
+}
+
+template <typename T, int DP>
+static int run_bwd(AttnK p, int nsplit, hipStream_t s) {
+  constexpr int ROWB = DP * (int)sizeof(T);
+  constexpr int BK = ROWB >= 512 ? 32 : 64;
+  {
+    constexpr int lds = 4 * BK * ROWB;
+    static bool attr[kMaxDevices] = {};
+    auto kern = attn_bwd_q_kernel<T, DP, 4, BK>;
+    if (set_lds_attr_once(attr, reinterpret_cast<const void*>(kern), lds) != hipSuccess) return IFD_LAUNCH_STATUS();
+    p.nblk = (int)cdiv(p.Tq, 128);
+    if (p.Tq) {
+      hipLaunchKernelGGL(kern, dim3(p.nblk * p.B * p.Hq), dim3(256), lds, s, p);
+      if (int e = IFD_LAUNCH_STATUS()) return e;
+    }
+  }
+  if (!p.Tk) return 0;
+  constexpr int lds = 2 * (2 * BK * ROWB + 1024);
+  static bool attr[kMaxDevices] = {};
+  auto kern = attn_bwd_kv_kernel<T, DP, 4, BK>;
+  if (set_lds_attr_once(attr, reinterpret_cast<const void*>(kern), lds) != hipSuccess) return IFD_LAUNCH_STATUS();
+  p.nblk = (int)cdiv(p.Tk, 128);
+  p.nsplit = nsplit;
+  hipLaunchKernelGGL(kern, dim3(p.nblk * p.B * p.Hk * nsplit), dim3(256), lds, s, p);
+  if (int e = IFD_LAUNCH_STATUS()) return e;
+  if (nsplit > 1) {
+    auto join = attn_bwd_join_kernel<T, DP>;
+    hipLaunchKernelGGL(join, dim3((unsigned)cdiv((int64_t)p.B * p.Hk * p.Tk * (DP / 2), 256)), dim3(256), 0, s, p);
+    return IFD_LAUNCH_STATUS();
+  }
+  return 0;
+}
+
+}  // namespace ifd
+
+using namespace ifd;
+extern "C" {
+
+int64_t ifd_op_attention_bwd_ws_bytes(const ifd_attention_args* a) {
+  if (!a || attention_check(*a) || !a->B) return 0;
+  const int dp = a->D <= 64 ? 64 : 128, n = kv_split(*a);
+  const int64_t part = n > 1 ? (int64_t)a->B * a->Hk * n * a->Tk * 2 * dp : 0;
+  return (2 * (int64_t)a->B * a->Hq * a->Tq + part) * 4;
+}
+
+int ifd_op_attention_bwd(const ifd_attention_args* a, void* ws, int64_t ws_bytes, void* stream) {
+  IFD_OP_REQUIRE(a != nullptr, "null arguments");
+  const char* why = attention_check(*a);
+  IFD_OP_REQUIRE(!why, why);
+  if (!a->B || (!a->Tq && !a->Tk)) return 0;
+  if (a->Tq && ((why = attention_tensor_check(*a, a->q, a->q_s)) || (why = attention_tensor_check(*a, a->out, a->out_s)) ||
+                (why = attention_tensor_check(*a, a->dout, a->dout_s)) ||
+                (why = attention_tensor_check(*a, a->dq, a->dq_s))))
+    IFD_OP_REQUIRE(false, why);
+  if (a->Tk && ((why = attention_tensor_check(*a, a->k, a->k_s)) || (why = attention_tensor_check(*a, a->v, a->v_s)) ||
+                (why = attention_tensor_check(*a, a->dk, a->dk_s)) ||
+                (why = attention_tensor_check(*a, a->dv, a->dv_s))))
+    IFD_OP_REQUIRE(false, why);
+  IFD_OP_REQUIRE(a->lse != nullptr || !a->Tq, "a null lse");
+  const int64_t need = ifd_op_attention_bwd_ws_bytes(a);
+  IFD_OP_REQUIRE(ws_bytes >= need && (ws || !need) && !((uintptr_t)ws & 15), "workspace too small or not aligned to 16 bytes");
+  const int n = kv_split(*a);
+  IFD_OP_REQUIRE(cdiv(a->Tk, 128) * a->B * a->Hk * n < 0x7fffffff && cdiv(a->Tq, 128) * a->B * a->Hq < 0x7fffffff &&
+                     (int64_t)a->B * a->Hk * a->Tk < (int64_t)1 << 31,
+                 "sizes beyond one launch");
+  AttnK p = attention_kernel_args(*a);
+  p.ws = (float*)ws;
+  hipStream_t s = (hipStream_t)stream;
+  const bool d64 = a->D <= 64;
+  if (a->dtype == IFD_F32) return d64 ? run_bwd<float, 64>(p, n, s) : run_bwd<float, 128>(p, n, s);
+  if (a->dtype == IFD_BF16) return d64 ? run_bwd<__bf16, 64>(p, n, s) : run_bwd<__bf16, 128>(p, n, s);
+  return d64 ? run_bwd<_Float16, 64>(p, n, s) : run_bwd<_Float16, 128>(p, n, s);
+}
+
+}  // extern "C"

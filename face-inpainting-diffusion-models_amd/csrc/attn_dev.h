@@ -1,0 +1,224 @@
+// Device pieces of the attention kernels (attn_fwd.hip, attn_bwd.hip): MFMA fragments, LDS tiles, masks.
+//
+// All matrix products are 32x32 MFMA tiles with fp32 accumulators. Lane l = (l32, h): l32 = l & 31, h = l >> 5.
+//   operands   a lane holds 16 bytes of one row (A: row l32; B: column l32): CE consecutive channels of chunk
+//              2 ks + h of k-step ks (16-bit types: one 32x32x16 MFMA per k-step; fp32: four 32x32x2).
+//   results    register i of a lane is row 8 (i / 4) + 4 h + i % 4, column l32.
+// A product's result feeds the next product as its B operand without moving between lanes: contraction slot (h, j) of
+// step t is taken to be the row that register it already is (16-bit: rows 16 t + 8 (j / 4) + 4 h + j % 4; fp32:
+// 8 t + 4 h + j), and the A operand is read from LDS in that row order, transposed (16-bit: ds_read_b64_tr_b16, which
+// hands each lane four rows of one column; fp32: four ds_read_b32).
+//
+// LDS tiles are row-major [rows][DP], filled by LDS-DMA (no registers between), 16-byte chunk c of row r at position
+// c ^ swz(r): eight consecutive rows of one chunk (row reads) and two chunks of four consecutive rows (transposed
+// reads) both fall into different banks.
+#pragma once
+#include "ops.h"
+
+namespace ifd {
+
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 hf16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 hf16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 hf16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) char lds_c;
+
+template <typename T>
+struct AttnT;
+template <>
+struct AttnT<__bf16> {
+  typedef bf16x8 frag;
+  typedef bf16x4 quad;
+  typedef bf16x2 pair;
+  static constexpr int PS = 2;  // contraction steps per 32 rows
+  static __device__ __forceinline__ f32x16 mma(frag a, frag b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+  }
+};
+template <>
+struct AttnT<_Float16> {
+  typedef hf16x8 frag;
+  typedef hf16x4 quad;
+  typedef hf16x2 pair;
+  static constexpr int PS = 2;
+  static __device__ __forceinline__ f32x16 mma(frag a, frag b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+  }
+};
+template <>
+struct AttnT<float> {
+  typedef f32x4 frag;
+  typedef f32x4 quad;
+  typedef f32x2 pair;
+  static constexpr int PS = 4;
+  static __device__ __forceinline__ f32x16 mma(frag a, frag b, f32x16 c) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[j], b[j], c, 0, 0, 0);
+    return c;
+  }
+};
+
+template <typename T, int DP>
+struct AttnTile {
+  typedef AttnT<T> A;
+  typedef typename A::frag frag;
+  static constexpr int ES = sizeof(T), CE = 16 / ES, NCH = DP / CE, ROWB = DP * ES;
+  static constexpr int KS = NCH / 2, DT = DP / 32, PS = A::PS;
+
+  static __device__ __forceinline__ int swz(int r) {
+    return NCH == 8 ? ((r & 3) << 1) | ((r >> 2) & 1) : ((r & 7) << 1) | ((r >> 3) & 1);
+  }
+
+  // rows [r0, r0 + 32) as A operands of k-step ks (row l32, chunk 2 ks + h)
+  static __device__ __forceinline__ frag row(const lds_c* tile, int r0, int ks, int l32, int h) {
+    return *(const __attribute__((address_space(3))) frag*)(tile + r0 * ROWB + l32 * ROWB +
+                                                            (((2 * ks) ^ (h ^ swz(l32))) << 4));
+  }
+  // rows [r0, r0 + 32) transposed as the A operand of contraction step t: column 32 dt + l32
+  static __device__ __forceinline__ frag col(const lds_c* tile, int r0, int t, int dt, int lane) {
+    const int h = lane >> 5, l32 = lane & 31;
+    if constexpr (ES == 2) {
+      const int i = lane & 15;
+      const int c = dt * 4 + (((lane >> 4) & 1) << 1) + ((i & 3) >> 1);
+      s16x8 f;
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int r = 16 * t + 8 * u + 4 * h + (i >> 2);
+        const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (__attribute__((address_space(3))) s16x4*)(tile + r0 * ROWB + r * ROWB + ((c ^ swz(r)) << 4) +
+                                                       ((i & 1) << 3)));
+#pragma unroll
+        for (int j = 0; j < 4; ++j) f[4 * u + j] = x[j];
+      }
+      return __builtin_bit_cast(frag, f);
+    } else {
+      frag f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int r = 8 * t + 4 * h + j;
+        f[j] = *(const __attribute__((address_space(3))) float*)(tile + r0 * ROWB + r * ROWB +
+                                                                 (((dt * 8 + (l32 >> 2)) ^ swz(r)) << 4) +
+                                                                 ((l32 & 3) << 2));
+      }
+      return f;
+    }
+  }
+  // a result tile's registers of contraction step t, rounded to T (16-bit: nearest, once)
+  static __device__ __forceinline__ frag pack(const f32x16& s, int t) {
+    frag f;
+    if constexpr (ES == 2) {
+#pragma unroll
+      for (int j = 0; j < 8; j += 2) {
+        const f32x2 v = {s[8 * t + j], s[8 * t + j + 1]};
+        const typename A::pair p = __builtin_convertvector(v, typename A::pair);
+        f[j] = p[0];
+        f[j + 1] = p[1];
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) f[j] = s[4 * t + j];
+    }
+    return f;
+  }
+  // 16 bytes of a row in global memory as an operand: zeros past D or for an absent row
+  static __device__ __forceinline__ frag gload(const char* rowp, bool ok, int ks, int h, int D) {
+    const int c = 2 * ks + h;
+    u32x4 z = {0, 0, 0, 0};
+    if (ok && c * CE < D) z = *reinterpret_cast<const u32x4*>(rowp + c * 16);
+    return __builtin_bit_cast(frag, z);
+  }
+};
+
+// LDS-DMA of 16 bytes per lane, from `off` bytes past base to dst + 16 lane. (The host pass of a template that calls the
+// builtin in its body drops the kernel's stub without a message: it stays inside these two functions.)
+__device__ __forceinline__ void dma_quad(const char* base, int off, lds_c* dst) {
+  const __amdgpu_buffer_rsrc_t rs =
+      __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), (short)0, 0x7ffffff0, 0x00020000);
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)dst, 16, off, 0, 0, 0);
+}
+// LDS-DMA of one 4-byte word per lane, from `off` bytes past base to dst + 4 lane
+__device__ __forceinline__ void dma_word(const float* base, int off, lds_c* dst) {
+  const __amdgpu_buffer_rsrc_t rs =
+      __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(base), (short)0, 0x7ffffff0, 0x00020000);
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)dst, 4, off, 0, 0, 0);
+}
+
+// LDS-DMA of ROWS rows of a [token][D] matrix into a tile by NW waves (wave w of them). Rows past `nrows` repeat the
+// last one and chunks past D repeat chunk 0: what they hold is real data of the same matrix, and the products either
+// multiply it by zeros or drop its result.
+template <typename T, int DP, int ROWS, int NW>
+struct AttnStage {
+  typedef AttnTile<T, DP> TL;
+  static constexpr int RPI = 1024 / TL::ROWB;            // rows per DMA instruction (64 lanes x 16 bytes)
+  static constexpr int NI = ROWS / RPI / NW;             // instructions per wave
+  static_assert(ROWS % (RPI * NW) == 0, "tile rows divide over the waves");
+  int row[NI], cb[NI];
+
+  __device__ __forceinline__ void init(int w, int lane, int D) {
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      row[i] = (w + NW * i) * RPI + lane / TL::NCH;
+      const int c = (lane % TL::NCH) ^ TL::swz(row[i]);
+      cb[i] = c * TL::CE < D ? c * 16 : 0;
+    }
+  }
+  // base: the tile's first row; stride in bytes (host check: 128 rows stay within 31 bits)
+  __device__ __forceinline__ void load(const char* base, int stride, int nrows, lds_c* tile, int w) const {
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      const int r = row[i] < nrows ? row[i] : nrows - 1;
+      dma_quad(base, r * stride + cb[i], tile + (w + NW * i) * 1024);
+    }
+  }
+};
+
+__device__ __forceinline__ f32x4 lds_quad(const lds_c* q) { return *(const __attribute__((address_space(3))) f32x4*)q; }
+
+__device__ __forceinline__ void dma_wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+// max / sum with the other half of a wave (lane ^ 32)
+__device__ __forceinline__ float xhalf(float v) { return __shfl_xor(v, 32); }
+
+struct AttnK {  // kernel arguments: strides in bytes
+  const char *q, *k, *v, *dout;
+  char *out, *dq, *dk, *dv;
+  float* lse;
+  const int *kv_len, *q_start;
+  int64_t qb, qh, kb, kh, vb, vh, ob, oh, gb, gh, dqb, dqh, dkb, dkh, dvb, dvh;
+  int qt, kt, vt, ot, gt, dqt, dkt, dvt;  // token strides
+  int B, Tq, Tk, Hq, Hk, D, G, causal, nblk, nsplit;
+  float c, scale;  // c = scale log2(e)
+  float* ws;
+};
+
+__device__ __forceinline__ int seq_len(const AttnK& p, int b) {
+  if (!p.kv_len) return p.Tk;
+  const int n = p.kv_len[b];
+  return n < 0 ? 0 : (n > p.Tk ? p.Tk : n);
+}
+// keys that row i of sequence b sees: [0, limit)
+__device__ __forceinline__ int row_limit(const AttnK& p, int qs, int len, int i) {
+  if (!p.causal) return len;
+  const int64_t n = (int64_t)qs + i + 1;  // q_start is any int32
+  return n < 0 ? 0 : (n > len ? len : (int)n);
+}
+__device__ __forceinline__ int q_first(const AttnK& p, int b) { return p.q_start ? p.q_start[b] : p.Tk - p.Tq; }
+
+// Workgroups are dealt to the eight XCDs in turn: give each XCD a contiguous range, so that blocks that read the same
+// keys share an L2.
+__device__ __forceinline__ int xcd_order(int bid, int n) {
+  const int full = n & ~7;
+  return bid < full ? (bid & 7) * (full >> 3) + (bid >> 3) : bid;
+}
+
+// attn_fwd.hip: what is wrong with a tensor's pointer or strides (nullptr: nothing), and the kernels' form of the arguments
+const char* attention_tensor_check(const ifd_attention_args& a, const void* p, const int64_t (&s)[3]);
+AttnK attention_kernel_args(const ifd_attention_args& a);
+
+}  // namespace ifd

@@ -1,0 +1,504 @@
+// Attention forward: out = softmax(scale q k^T) v and the rows' log-sum-exp (include/ifd_ops.h), one pass over the keys
+// with a running maximum and sum.
+#include "attn_dev.h"
+
+namespace ifd {
+
+// The running softmax of 32 query rows (column l32 of the score tile) and their output accumulators.
+// Scores are kept in units of log2: p = 2^(c s - m). The reference point m moves only when a row's maximum passes it by
+// more than 2^SLACK, so most tiles skip the rescaling of O; p <= 2^SLACK then, exact in fp32 and inside fp16's range.
+constexpr float ATTN_SLACK = 8.f;
+
+template <typename T, int DP, int KT>
+struct AttnRows {
+  typedef AttnTile<T, DP> TL;
+  typedef typename TL::frag frag;
+  f32x16 o[TL::DT];
+  float m, l;  // l: this lane's keys only; the two halves are added at the end
+
+  __device__ __forceinline__ void init() {
+#pragma unroll
+    for (int d = 0; d < TL::DT; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
+    m = -INFINITY;
+    l = 0.f;
+  }
+  // scores -> probabilities in place. lim: keys [0, lim) of this tile are seen by the row (mask != 0)
+  __device__ __forceinline__ void soft(f32x16 (&s)[KT], float c, bool mask, int lim, int h) {
+    if (mask) {
+#pragma unroll
+      for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (kt * 32 + 8 * (i >> 2) + 4 * h + (i & 3) >= lim) s[kt][i] = -INFINITY;
+    }
+    float mx = s[0][0];
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+      for (int i = kt ? 0 : 1; i < 16; ++i) mx = fmaxf(mx, s[kt][i]);
+    mx = fmaxf(mx, xhalf(mx)) * c;
+    if (__any(mx > m + ATTN_SLACK || (m == -INFINITY && mx > m))) {
+      const float mn = fmaxf(m, mx);
+      const float a = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
+      m = mn;
+      l *= a;
+#pragma unroll
+      for (int d = 0; d < TL::DT; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[d][i] *= a;
+    }
+    const float ms = m == -INFINITY ? 0.f : m;  // no key seen yet: every p is 2^-inf = 0
+    float sum = 0.f;
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        s[kt][i] = __builtin_amdgcn_exp2f(fmaf(s[kt][i], c, -ms));
+        sum += s[kt][i];
+      }
+    l += sum;
+  }
+};
+
+// Many rows. A workgroup of NW waves takes NW * NQ * 32 rows of one (sequence, head); the waves share the K and V tiles
+// (BK keys, two buffers, the next tile's DMA in flight during this one's products). Per wave and tile: S^T = K Q^T with
+// Q in registers, softmax down the registers of each lane (a lane holds one row's scores of half the keys), O^T += V^T P^T.
+template <typename T, int DP, int NQ, int NW, int BK>
+__global__ __launch_bounds__(NW * 64) void attn_fwd_kernel(AttnK p) {
+  typedef AttnTile<T, DP> TL;
+  typedef typename TL::frag frag;
+  constexpr int KT = BK / 32, TB = BK * TL::ROWB;
+  extern __shared__ __attribute__((aligned(1024))) char smem[];
+  lds_c* sm = (lds_c*)smem;
+  const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, h = lane >> 5;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  // causal: longest blocks first, a head's blocks on one XCD; else head by head on each XCD
+  const int BH = p.B * p.Hq;
+  int bh, qblk;
+  if (p.causal) {
+    const int r = blockIdx.x % BH;
+    qblk = p.nblk - 1 - blockIdx.x / BH;
+    bh = (BH & 7) ? r : (r & 7) * (BH >> 3) + (r >> 3);
+  } else {
+    const int id = xcd_order(blockIdx.x, BH * p.nblk);
+    bh = id / p.nblk;
+    qblk = id - bh * p.nblk;
+  }
+  const int b = bh / p.Hq, hq = bh - b * p.Hq, hk = hq / p.G;
+  const int len = seq_len(p, b), qs = q_first(p, b);
+  const int q0 = qblk * (NW * NQ * 32) + w * (NQ * 32);
+
+  frag qf[NQ][TL::KS];
+  int lim[NQ];
+#pragma unroll
+  for (int n = 0; n < NQ; ++n) {
+    const int i = q0 + n * 32 + l32;
+    lim[n] = i < p.Tq ? row_limit(p, qs, len, i) : 0;
+    const char* rp = p.q + b * p.qb + hq * p.qh + (int64_t)i * p.qt;
+#pragma unroll
+    for (int ks = 0; ks < TL::KS; ++ks) qf[n][ks] = TL::gload(rp, i < p.Tq, ks, h, p.D);
+  }
+  AttnRows<T, DP, KT> st[NQ];
+#pragma unroll
+  for (int n = 0; n < NQ; ++n) st[n].init();
+
+  // keys that any row of the workgroup sees, of the wave; and those that all its rows see
+  const int last = min(p.Tq, (qblk + 1) * (NW * NQ * 32)) - 1;
+  const int wg_end = row_limit(p, qs, len, last);
+  const int w_last = min(p.Tq, q0 + NQ * 32) - 1;
+  const int w_end = __builtin_amdgcn_readfirstlane(w_last < q0 ? 0 : row_limit(p, qs, len, w_last));
+  const int w_all = __builtin_amdgcn_readfirstlane(w_last < q0 ? 0 : row_limit(p, qs, len, q0));
+  const int nt = (wg_end + BK - 1) / BK;
+
+  AttnStage<T, DP, BK, NW> sg;
+  sg.init(w, lane, p.D);
+  const char* kp = p.k + b * p.kb + hk * p.kh;
+  const char* vp = p.v + b * p.vb + hk * p.vh;
+  auto stage = [&](int t) {
+    const int k0 = t * BK, n = min(BK, len - k0);
+    lds_c* d = sm + (t & 1) * (2 * TB);
+    sg.load(kp + (int64_t)k0 * p.kt, p.kt, n, d, w);
+    sg.load(vp + (int64_t)k0 * p.vt, p.vt, n, d + TB, w);
+  };
+  if (nt > 0) {
+    stage(0);
+    dma_wait();
+    __syncthreads();
+  }
+  for (int t = 0; t < nt; ++t) {
+    if (t + 1 < nt) stage(t + 1);
+    const lds_c* kb = sm + (t & 1) * (2 * TB);
+    const lds_c* vb = kb + TB;
+    const int k0 = t * BK;
+    if (k0 < w_end) {
+      f32x16 s[NQ][KT];
+#pragma unroll
+      for (int kt = 0; kt < KT; ++kt) {
+#pragma unroll
+        for (int n = 0; n < NQ; ++n)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) s[n][kt][i] = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < TL::KS; ++ks) {
+          const frag a = TL::row(kb, kt * 32, ks, l32, h);
+#pragma unroll
+          for (int n = 0; n < NQ; ++n) s[n][kt] = TL::A::mma(a, qf[n][ks], s[n][kt]);
+        }
+      }
+      const bool mask = k0 + BK > w_all;
+#pragma unroll
+      for (int n = 0; n < NQ; ++n) st[n].soft(s[n], p.c, mask, lim[n] - k0, h);
+#pragma unroll
+      for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+        for (int ps = 0; ps < TL::PS; ++ps) {
+          frag pf[NQ];
+#pragma unroll
+          for (int n = 0; n < NQ; ++n) pf[n] = TL::pack(s[n][kt], ps);
+#pragma unroll
+          for (int d = 0; d < TL::DT; ++d) {
+            const frag a = TL::col(vb, kt * 32, ps, d, lane);
+#pragma unroll
+            for (int n = 0; n < NQ; ++n) st[n].o[d] = TL::A::mma(a, pf[n], st[n].o[d]);
+          }
+        }
+    }
+    dma_wait();
+    __syncthreads();
+  }
+#pragma unroll
+  for (int n = 0; n < NQ; ++n) {
+    const int i = q0 + n * 32 + l32;
+    const float l = st[n].l + xhalf(st[n].l);
+    if (i >= p.Tq) continue;
+    const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+    if (h == 0)
+      p.lse[((int64_t)b * p.Hq + hq) * p.Tq + i] =
+          l == 0.f ? -INFINITY : (st[n].m + __builtin_amdgcn_logf(l)) * 0.69314718055994531f;
+    T* op = reinterpret_cast<T*>(p.out + b * p.ob + hq * p.oh + (int64_t)i * p.ot);
+#pragma unroll
+    for (int d = 0; d < TL::DT; ++d)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int ch = d * 32 + 8 * j + 4 * h;
+        if (ch >= p.D) continue;
+        f32x4 v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = st[n].o[d][4 * j + e] * inv;
+        *reinterpret_cast<typename TL::A::quad*>(op + ch) = __builtin_convertvector(v, typename TL::A::quad);
+      }
+  }
+}
+
+// Few rows against many keys. The rows of all query heads of one key-value head (row r = token r / G, head r % G) fill
+// one 32-row tile, every key is read once, and the keys are split over the NW waves of a workgroup (each streams its own
+// tiles through its own LDS, no barriers) and over `nsplit` workgroups. The waves' results are joined in LDS, the
+// workgroups' by attn_join_kernel: O = sum_s 2^(m_s - m) O_s, l likewise.
+template <typename T, int DP, int NW, int BK>
+__global__ __launch_bounds__(NW * 64) void attn_split_kernel(AttnK p) {
+  typedef AttnTile<T, DP> TL;
+  typedef typename TL::frag frag;
+  constexpr int KT = BK / 32, TB = BK * TL::ROWB, WB = 4 * TB;  // per wave: two buffers of K and V
+  static_assert(32 * DP * 4 + 256 <= WB, "a wave's result fits its tiles' LDS");
+  extern __shared__ __attribute__((aligned(1024))) char smem[];
+  const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, h = lane >> 5;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  lds_c* sm = (lds_c*)smem + w * WB;
+  const int id = xcd_order(blockIdx.x, gridDim.x);
+  const int sp = id % p.nsplit;
+  int r_ = id / p.nsplit;
+  const int rb = r_ % p.nblk;
+  r_ /= p.nblk;
+  const int hk = r_ % p.Hk, b = r_ / p.Hk;
+  const int len = seq_len(p, b), qs = q_first(p, b);
+  const int rows = p.Tq * p.G;
+  const int r = rb * 32 + l32;
+  const bool ok = r < rows;
+  const int i = ok ? r / p.G : 0, hq = hk * p.G + (ok ? r - i * p.G : 0);
+  const int lim = ok ? row_limit(p, qs, len, i) : 0;
+  const int r1 = min(rows, rb * 32 + 32) - 1;  // the last row sees most
+  const int end = __builtin_amdgcn_readfirstlane(row_limit(p, qs, len, r1 / p.G));
+  const int all = __builtin_amdgcn_readfirstlane(row_limit(p, qs, len, rb * 32 / p.G));
+  frag qf[TL::KS];
+  {
+    const char* rp = p.q + b * p.qb + hq * p.qh + (int64_t)i * p.qt;
+#pragma unroll
+    for (int ks = 0; ks < TL::KS; ++ks) qf[ks] = TL::gload(rp, ok, ks, h, p.D);
+  }
+  AttnRows<T, DP, KT> st;
+  st.init();
+  // this workgroup's tiles: [t0, t1), wave w takes t0 + w, t0 + w + NW, ...
+  const int nt = (end + BK - 1) / BK;
+  const int per = (nt + p.nsplit - 1) / p.nsplit;
+  const int t0 = sp * per, t1 = min(nt, t0 + per);
+  AttnStage<T, DP, BK, 1> sg;
+  sg.init(0, lane, p.D);
+  const char* kp = p.k + b * p.kb + hk * p.kh;
+  const char* vp = p.v + b * p.vb + hk * p.vh;
+  auto stage = [&](int t, int buf) {
+    const int k0 = t * BK, n = min(BK, len - k0);
+    lds_c* d = sm + buf * (2 * TB);
+    sg.load(kp + (int64_t)k0 * p.kt, p.kt, n, d, 0);
+    sg.load(vp + (int64_t)k0 * p.vt, p.vt, n, d + TB, 0);
+  };
+  int buf = 0;
+  if (t0 + w < t1) stage(t0 + w, 0);
+  for (int t = t0 + w; t < t1; t += NW) {
+    // this tile's DMA is complete once at most the next tile's is outstanding
+    if (t + NW < t1) {
+      stage(t + NW, buf ^ 1);
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * AttnStage<T, DP, BK, 1>::NI) : "memory");
+    } else {
+      dma_wait();
+    }
+    const lds_c* kb = sm + buf * (2 * TB);
+    const lds_c* vb = kb + TB;
+    const int k0 = t * BK;
+    f32x16 s[KT];
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt) {
+#pragma unroll
+      for (int i2 = 0; i2 < 16; ++i2) s[kt][i2] = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < TL::KS; ++ks) s[kt] = TL::A::mma(TL::row(kb, kt * 32, ks, l32, h), qf[ks], s[kt]);
+    }
+    st.soft(s, p.c, k0 + BK > all, lim - k0, h);
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+      for (int ps = 0; ps < TL::PS; ++ps) {
+        const frag pf = TL::pack(s[kt], ps);
+#pragma unroll
+        for (int d = 0; d < TL::DT; ++d) st.o[d] = TL::A::mma(TL::col(vb, kt * 32, ps, d, lane), pf, st.o[d]);
+      }
+    // the reads above are complete before the next round's DMA overwrites this buffer
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    buf ^= 1;
+  }
+  // the waves' results: m, l of each row, then O [DP][32 rows] in the wave's own (now idle) LDS
+  const float l = st.l + xhalf(st.l);
+  float* wf = reinterpret_cast<float*>(smem + w * WB);
+  __syncthreads();
+  if (h == 0) {
+    wf[l32] = st.m;
+    wf[32 + l32] = l;
+  }
+#pragma unroll
+  for (int d = 0; d < TL::DT; ++d)
+#pragma unroll
+    for (int j = 0; j < 16; ++j) wf[64 + (d * 32 + 8 * (j >> 2) + 4 * h + (j & 3)) * 32 + l32] = st.o[d][j];
+  __syncthreads();
+  float m = -INFINITY;
+#pragma unroll
+  for (int x = 0; x < NW; ++x) m = fmaxf(m, reinterpret_cast<const float*>(smem + x * WB)[l32]);
+  float f[NW], lt = 0.f;
+#pragma unroll
+  for (int x = 0; x < NW; ++x) {
+    const float* xf = reinterpret_cast<const float*>(smem + x * WB);
+    f[x] = xf[l32] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(xf[l32] - m);
+    lt += f[x] * xf[32 + l32];
+  }
+  // thread (row l32, group tid / 32): channels group, group + 2 NW, ...
+  const int64_t prow = (((int64_t)b * p.Hk + hk) * p.nblk + rb) * 32 + l32;
+  float* po = p.nsplit > 1 ? p.ws + (prow * p.nsplit + sp) * (DP + 2) : nullptr;
+  const float inv = lt > 0.f ? 1.f / lt : (lt == 0.f ? 0.f : lt);
+  T* op = reinterpret_cast<T*>(p.out + b * p.ob + hq * p.oh + (int64_t)i * p.ot);
+  for (int g = tid >> 5; g < DP / 4; g += 2 * NW) {
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int x = 0; x < NW; ++x) {
+      const float* xf = reinterpret_cast<const float*>(smem + x * WB) + 64 + (4 * g) * 32 + l32;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] += f[x] * xf[e * 32];
+    }
+    if (po) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) po[2 + 4 * g + e] = v[e];
+    } else if (ok && 4 * g < p.D) {
+      v *= inv;
+      *reinterpret_cast<typename TL::A::quad*>(op + 4 * g) = __builtin_convertvector(v, typename TL::A::quad);
+    }
+  }
+  if (tid < 32) {
+    if (po) {
+      po[0] = m;
+      po[1] = lt;
+    } else if (ok) {
+      p.lse[((int64_t)b * p.Hq + hq) * p.Tq + i] =
+          lt == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(lt)) * 0.69314718055994531f;
+    }
+  }
+}
+
+// One wave per row: the splits' partial results in order.
+template <typename T, int DP>
+__global__ __launch_bounds__(256) void attn_join_kernel(AttnK p) {
+  const int lane = threadIdx.x & 63;
+  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int rows = p.Tq * p.G;
+  if (row >= (int64_t)p.B * p.Hk * rows) return;
+  const int bk = (int)(row / rows), r = (int)(row - (int64_t)bk * rows);
+  const int b = bk / p.Hk, hk = bk - b * p.Hk, i = r / p.G, hq = hk * p.G + (r - i * p.G);
+  const float* w = p.ws + ((int64_t)bk * p.nblk * 32 + r) * p.nsplit * (DP + 2);
+  float m = -INFINITY;
+  for (int s = lane; s < p.nsplit; s += 64) m = fmaxf(m, w[s * (DP + 2)]);
+#pragma unroll
+  for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+  float l = 0.f, a[DP / 64] = {};
+  for (int s = 0; s < p.nsplit; ++s) {
+    const float* x = w + s * (DP + 2);
+    const float f = x[0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(x[0] - m);
+    l += f * x[1];
+#pragma unroll
+    for (int e = 0; e < DP / 64; ++e) a[e] += f * x[2 + lane + 64 * e];
+  }
+  const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+  T* op = reinterpret_cast<T*>(p.out + b * p.ob + hq * p.oh + (int64_t)i * p.ot);
+#pragma unroll
+  for (int e = 0; e < DP / 64; ++e)
+    if (lane + 64 * e < p.D) op[lane + 64 * e] = (T)(a[e] * inv);
+  if (lane == 0)
+    p.lse[((int64_t)b * p.Hq + hq) * p.Tq + i] =
+        l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * 0.69314718055994531f;
+}
+
+// ---------------------------------------------------------------------------------------------- host side
+const char* attention_check(const ifd_attention_args& a) {
+  if (!dtype_ok(a.dtype)) return "dtype";
+  if (a.B < 0 || a.Tq < 0 || a.Tk < 0 || a.Hq < 1 || a.Hk < 1 || a.D < 1) return "negative or zero sizes";
+  if (a.Hq % a.Hk) return "the query heads are not a multiple of the key-value heads";
+  const int es = (int)dtype_bytes(a.dtype), ce = 16 / es;
+  if (a.D > 128 || a.D % ce) return "head width: at most 128, a multiple of 8 (16-bit) or 4 (fp32)";
+  if (!(a.scale > 0.f) || !(a.scale < 3e38f)) return "scale must be positive and finite";
+  if (a.Tk > 0x3fffffff || (int64_t)a.Tq * (a.Hq / a.Hk) > 0x3fffffff || (int64_t)a.B * a.Hq > 0x3fffffff) 
+    return "sizes beyond 2^30 rows";
+  return nullptr;
+}
+
+const char* attention_tensor_check(const ifd_attention_args& a, const void* p, const int64_t (&s)[3]) {
+  const int es = (int)dtype_bytes(a.dtype);
+  if (!p) return "a null tensor";
+  if ((uintptr_t)p & 15) return "tensors must be aligned to 16 bytes";
+  for (int j = 0; j < 3; ++j)
+    if ((s[j] * es) & 15) return "strides must be multiples of 16 bytes";
+  if (s[1] < 0 || s[1] * es >= (int64_t)1 << 24) return "token stride negative or 16 MiB and more";
+  return nullptr;
+}
+
+struct FwdPlan {
+  bool split;
+  int nblk, nsplit;
+};
+
+// The tile of 32 rows per (sequence, key-value head) reads every key once for all the heads of a group, but its products
+// have no reuse between waves: it is taken while the rows of a group fill few tiles, or while the many-row kernel's
+// workgroups (128 rows each) would leave most of the chip idle.
+static FwdPlan fwd_plan(const ifd_attention_args& a, int dp, int es) {
+  const int G = a.Hq / a.Hk;
+  FwdPlan r;
+  const int64_t rows = (int64_t)a.Tq * G, rb = cdiv(rows, 32), base = (int64_t)a.B * a.Hk * rb;
+  const int64_t big = cdiv(a.Tq, 128) * a.B * a.Hq;
+  r.split = rows <= 32 || (big < 64 && a.Tk >= 256);
+  if (!r.split) {
+    r.nblk = (int)cdiv(a.Tq, 128);
+    r.nsplit = 1;
+    return r;
+  }
+  r.nblk = (int)rb;
+  const int bk = dp * es == 128 ? 64 : 32;
+  const int64_t tiles = cdiv(a.Tk, bk);
+  int64_t n = cdiv(512, base);
+  n = std::min<int64_t>(n, cdiv(tiles, 8));
+  r.nsplit = (int)std::max<int64_t>(1, std::min<int64_t>(n, 64));
+  return r;
+}
+
+AttnK attention_kernel_args(const ifd_attention_args& a) {
+  const int es = (int)dtype_bytes(a.dtype);
+  AttnK p = {};
+  p.q = (const char*)a.q; p.k = (const char*)a.k; p.v = (const char*)a.v;
+  p.out = (char*)a.out; p.lse = a.lse; p.kv_len = a.kv_len; p.q_start = a.q_start;
+  p.qb = a.q_s[0] * es; p.qt = (int)(a.q_s[1] * es); p.qh = a.q_s[2] * es;
+  p.kb = a.k_s[0] * es; p.kt = (int)(a.k_s[1] * es); p.kh = a.k_s[2] * es;
+  p.vb = a.v_s[0] * es; p.vt = (int)(a.v_s[1] * es); p.vh = a.v_s[2] * es;
+  p.ob = a.out_s[0] * es; p.ot = (int)(a.out_s[1] * es); p.oh = a.out_s[2] * es;
+  p.dout = (const char*)a.dout; p.dq = (char*)a.dq; p.dk = (char*)a.dk; p.dv = (char*)a.dv;
+  p.gb = a.dout_s[0] * es; p.gt = (int)(a.dout_s[1] * es); p.gh = a.dout_s[2] * es;
+  p.dqb = a.dq_s[0] * es; p.dqt = (int)(a.dq_s[1] * es); p.dqh = a.dq_s[2] * es;
+  p.dkb = a.dk_s[0] * es; p.dkt = (int)(a.dk_s[1] * es); p.dkh = a.dk_s[2] * es;
+  p.dvb = a.dv_s[0] * es; p.dvt = (int)(a.dv_s[1] * es); p.dvh = a.dv_s[2] * es;
+  p.B = a.B; p.Tq = a.Tq; p.Tk = a.Tk; p.Hq = a.Hq; p.Hk = a.Hk; p.D = a.D; p.G = a.Hq / a.Hk;
+  p.causal = a.causal != 0;
+  p.scale = a.scale;
+  p.c = a.scale * 1.4426950408889634f;
+  return p;
+}
+
+template <typename T, int DP>
+static int run_fwd(const FwdPlan& pl, AttnK p, hipStream_t s) {
+  constexpr int ROWB = DP * (int)sizeof(T);
+  p.nblk = pl.nblk;
+  p.nsplit = pl.nsplit;
+  if (!pl.split) {
+    constexpr int BK = ROWB >= 512 ? 32 : 64;
+    constexpr int lds = 4 * BK * ROWB;
+    static bool attr[kMaxDevices] = {};
+    auto kern = attn_fwd_kernel<T, DP, 1, 4, BK>;
+    if (set_lds_attr_once(attr, reinterpret_cast<const void*>(kern), lds) != hipSuccess) return IFD_LAUNCH_STATUS();
+    hipLaunchKernelGGL(kern, dim3(p.nblk * p.B * p.Hq), dim3(256), lds, s, p);
+    return IFD_LAUNCH_STATUS();
+  }
+  constexpr int BK = ROWB == 128 ? 64 : 32, NW = ROWB >= 512 ? 2 : 4;
+  constexpr int lds = NW * 4 * BK * ROWB;
+  static bool attr[kMaxDevices] = {};
+  auto kern = attn_split_kernel<T, DP, NW, BK>;
+  if (set_lds_attr_once(attr, reinterpret_cast<const void*>(kern), lds) != hipSuccess) return IFD_LAUNCH_STATUS();
+  hipLaunchKernelGGL(kern, dim3(p.nsplit * p.nblk * p.B * p.Hk), dim3(NW * 64), lds, s, p);
+  if (int e = IFD_LAUNCH_STATUS()) return e;
+  if (p.nsplit > 1) {
+    const int64_t rows = (int64_t)p.B * p.Hq * p.Tq;
+    auto join = attn_join_kernel<T, DP>;
+    hipLaunchKernelGGL(join, dim3((unsigned)cdiv(rows, 4)), dim3(256), 0, s, p);
+    return IFD_LAUNCH_STATUS();
+  }
+  return 0;
+}
+
+}  // namespace ifd
+
+using namespace ifd;
+extern "C" {
+
+int64_t ifd_op_attention_ws_bytes(const ifd_attention_args* a) {
+  if (!a || attention_check(*a) || !a->B || !a->Tq) return 0;
+  const int dp = a->D <= 64 ? 64 : 128;
+  const FwdPlan pl = fwd_plan(*a, dp, (int)dtype_bytes(a->dtype));
+  if (!pl.split || pl.nsplit == 1) return 0;
+  return (int64_t)a->B * a->Hk * pl.nblk * 32 * pl.nsplit * (dp + 2) * 4;
+}
+
+int ifd_op_attention(const ifd_attention_args* a, void* ws, int64_t ws_bytes, void* stream) {
+  IFD_OP_REQUIRE(a != nullptr, "null arguments");
+  const char* why = attention_check(*a);
+  IFD_OP_REQUIRE(!why, why);
+  if (!a->B || !a->Tq) return 0;
+  const int es = (int)dtype_bytes(a->dtype), dp = a->D <= 64 ? 64 : 128;
+  if ((why = attention_tensor_check(*a, a->q, a->q_s)) || (why = attention_tensor_check(*a, a->out, a->out_s)) ||
+      (a->Tk && ((why = attention_tensor_check(*a, a->k, a->k_s)) || (why = attention_tensor_check(*a, a->v, a->v_s)))))
+    IFD_OP_REQUIRE(false, why);
+  IFD_OP_REQUIRE(a->lse != nullptr, "a null lse");
+  IFD_OP_REQUIRE(ws_bytes >= ifd_op_attention_ws_bytes(a) && (ws || !ifd_op_attention_ws_bytes(a)),
+                 "workspace too small");
+  const FwdPlan pl = fwd_plan(*a, dp, es);
+  IFD_OP_REQUIRE((int64_t)pl.nsplit * pl.nblk * a->B * a->Hq < 0x7fffffff, "sizes beyond one launch");
+  AttnK p = attention_kernel_args(*a);
+  p.ws = (float*)ws;
+  hipStream_t s = (hipStream_t)stream;
+  if (a->dtype == IFD_F32) return dp == 64 ? run_fwd<float, 64>(pl, p, s) : run_fwd<float, 128>(pl, p, s);
+  if (a->dtype == IFD_BF16) return dp == 64 ? run_fwd<__bf16, 64>(pl, p, s) : run_fwd<__bf16, 128>(pl, p, s);
+  return dp == 64 ? run_fwd<_Float16, 64>(pl, p, s) : run_fwd<_Float16, 128>(pl, p, s);
+}
+
+}  // extern "C"

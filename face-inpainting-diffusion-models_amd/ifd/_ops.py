@@ -1,0 +1,67 @@
+"""ctypes binding of the attention-layer operators (the C ABI declared in include/ifd_ops.h)."""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import _lib
+
+_c = ctypes
+vp, i32, i64, f32 = _c.c_void_p, _c.c_int, _c.c_int64, _c.c_float
+DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+Strides = i64 * 3
+
+
+class AttentionArgs(ctypes.Structure):
+    """ifd_attention_args"""
+    _fields_ = ([(n, i32) for n in ("dtype", "B", "Tq", "Tk", "Hq", "Hk", "D", "causal")]
+                + [("scale", f32), ("pad", i32)]
+                + [(n, vp) for n in ("q", "k", "v", "out", "lse", "kv_len", "q_start")]
+                + [(n, Strides) for n in ("q_s", "k_s", "v_s", "out_s")]
+                + [(n, vp) for n in ("dout", "dq", "dk", "dv")]
+                + [(n, Strides) for n in ("dout_s", "dq_s", "dk_s", "dv_s")])
+
+
+OPS_EXPORTS = {
+    "ifd_op_attention_ws_bytes": (i64, [_c.POINTER(AttentionArgs)]),
+    "ifd_op_attention": (i32, [_c.POINTER(AttentionArgs), vp, i64, vp]),
+    "ifd_op_attention_bwd_ws_bytes": (i64, [_c.POINTER(AttentionArgs)]),
+    "ifd_op_attention_bwd": (i32, [_c.POINTER(AttentionArgs), vp, i64, vp]),
+}
+
+_bound = None
+
+
+def lib():
+    global _bound
+    L = _lib.lib()
+    if _bound is not L:
+        for name, (res, args) in OPS_EXPORTS.items():
+            f = getattr(L, name)
+            f.restype = res
+            f.argtypes = args
+        _bound = L
+    return L
+
+
+def need(cond, msg):
+    if not cond:
+        raise ValueError("ifd: " + msg)
+
+
+def same_device(*tensors):
+    """The device all the tensors live on (they must be on one GPU)."""
+    dev = None
+    for t in tensors:
+        if t is None:
+            continue
+        need(t.is_cuda, f"expected a GPU tensor, got one on {t.device}")
+        need(dev is None or t.device == dev, f"tensors on {dev} and on {t.device}")
+        dev = t.device
+    return dev
+
+
+def workspace(nbytes, dev):
+    """Scratch of one call, from torch's stream-ordered allocator (None when the call needs none)."""
+    return torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
