@@ -1,0 +1,410 @@
+// AdamW over many tensors, states in 32 or in 8 bits, with the gradients' global norm (include/ifd_ops.h).
+//   g' = c g; m = b1 m + (1 - b1) g'; v = b2 v + (1 - b2) g'^2;
+//   p = p (1 - lr wd) - lr / (1 - b1^k) m / (sqrt(v) / sqrt(1 - b2^k) + eps)
+// Bound by memory: 16 bytes a value with fp32 tensors and 8-bit states, 28 with 32-bit states, plus the norm's own pass
+// over the gradients. The tensors' addresses travel in the kernel arguments (96 tensors a launch): no table to upload,
+// nothing kept between steps. A wave owns blocks of 256 values, four per lane; an 8-bit state's scale is its block's.
+//
+// 8-bit states. One byte is a small float, with one fp32 scale per block of 256 (largest magnitude / 1.875):
+//   m: sign, 4 exponent bits, 3 fraction bits: 2^(e - 15) (1 + f / 8);  v: 5 exponent bits, 3 fraction bits: 2^(e - 31)
+//   (1 + f / 8); byte 0 is 0. A relative step of 1/8 at every magnitude: v spans 2^31 below its block's largest value.
+// The new byte is the value cut to 3 fraction bits after adding 16 random bits below them, so that it is right on average:
+// with b2 = 0.999 v moves by less than half a step per update, and rounding to nearest would never let it fall. A v > 0
+// never becomes 0 (the step would divide by eps). The random bits are a hash of the element's index and the step's key.
+// Everything that decides a byte is computed in fp64 (full rate here), so it does not depend on how the compiler orders
+// fp32 roundings; the step itself uses the moments before they are rounded, in fp32.
+#include <cmath>
+#include "ops.h"
+
+namespace ifd {
+
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 hf16x4 __attribute__((ext_vector_type(4)));
+
+constexpr int AW_T = 96;      // tensors of a launch
+constexpr int AW_CHUNK = 16;  // blocks of a workgroup
+
+struct AwTab {
+  const void* p[AW_T];
+  const void* g[AW_T];
+  int64_t n[AW_T];
+  int chunk0[AW_T];     // first workgroup of the tensor
+  int block0[AW_T];     // first state block, relative to AwArgs::block0
+  uint8_t pt[AW_T], gt[AW_T];
+  int count;
+};
+struct AwArgs {
+  void *m, *v;
+  float *ms, *vs;
+  const double* clip;  // {norm, coefficient} or null
+  int64_t block0;
+  double b1, w1, b2, w2;
+  float decay, step, eps, bc2s;
+  unsigned key;
+};
+
+// the tensor of workgroup `wg`: the last one whose first workgroup is not past it
+__device__ __forceinline__ int aw_find(const AwTab& t, int wg) {
+  const int lane = threadIdx.x & 63;
+  int n = 0;
+#pragma unroll
+  for (int o = 0; o < AW_T; o += 64) n += __popcll(__ballot(o + lane < t.count && t.chunk0[min(o + lane, AW_T - 1)] <= wg));
+  return __builtin_amdgcn_readfirstlane(n - 1);
+}
+
+__device__ __forceinline__ f32x4 aw_load(const void* base, int dt, int64_t i, int64_t n) {
+  f32x4 r = {0.f, 0.f, 0.f, 0.f};
+  if (dt == IFD_F32) {
+    const float* q = reinterpret_cast<const float*>(base) + i;
+    if (i + 4 <= n && ((uintptr_t)base & 15) == 0) return *reinterpret_cast<const f32x4*>(q);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (i + j < n) r[j] = q[j];
+  } else if (dt == IFD_BF16) {
+    const __bf16* q = reinterpret_cast<const __bf16*>(base) + i;
+    if (i + 4 <= n && ((uintptr_t)base & 7) == 0)
+      return __builtin_convertvector(*reinterpret_cast<const bf16x4*>(q), f32x4);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (i + j < n) r[j] = (float)q[j];
+  } else {
+    const _Float16* q = reinterpret_cast<const _Float16*>(base) + i;
+    if (i + 4 <= n && ((uintptr_t)base & 7) == 0)
+      return __builtin_convertvector(*reinterpret_cast<const hf16x4*>(q), f32x4);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (i + j < n) r[j] = (float)q[j];
+  }
+  return r;
+}
+__device__ __forceinline__ void aw_store(void* base, int dt, int64_t i, int64_t n, f32x4 v) {
+  if (dt == IFD_F32) {
+    float* q = reinterpret_cast<float*>(base) + i;
+    if (i + 4 <= n && ((uintptr_t)base & 15) == 0) {
+      *reinterpret_cast<f32x4*>(q) = v;
+      return;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (i + j < n) q[j] = v[j];
+  } else if (dt == IFD_BF16) {
+    __bf16* q = reinterpret_cast<__bf16*>(base) + i;
+    const bf16x4 x = __builtin_convertvector(v, bf16x4);
+    if (i + 4 <= n && ((uintptr_t)base & 7) == 0) {
+      *reinterpret_cast<bf16x4*>(q) = x;
+      return;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (i + j < n) q[j] = x[j];
+  } else {
+    _Float16* q = reinterpret_cast<_Float16*>(base) + i;
+    const hf16x4 x = __builtin_convertvector(v, hf16x4);
+    if (i + 4 <= n && ((uintptr_t)base & 7) == 0) {
+      *reinterpret_cast<hf16x4*>(q) = x;
+      return;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (i + j < n) q[j] = x[j];
+  }
+}
+
+// multiply / xor-shift mix (the multipliers: 2^32 times the fractions of the golden ratio, sqrt 2 and sqrt 3, odd)
+__host__ __device__ __forceinline__ unsigned aw_mix(unsigned x) {
+  x *= 0x9E3779B9u;
+  x ^= x >> 15;
+  x *= 0x6A09E667u;
+  x ^= x >> 13;
+  x *= 0xBB67AE85u;
+  return x ^ (x >> 16);
+}
+
+__device__ __forceinline__ float wave_max(float v) {
+#pragma unroll
+  for (int o = 32; o; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
+  return v;
+}
+__device__ __forceinline__ double hi_double(unsigned hi) { return __hiloint2double((int)hi, 0); }
+__device__ __forceinline__ double m_value(unsigned c) {  // without the scale
+  const unsigned k = c & 127u;
+  return hi_double(k ? (0x3F000000u + (k << 17)) | ((c & 128u) << 24) : 0u);
+}
+__device__ __forceinline__ double v_value(unsigned c) { return hi_double(c ? 0x3E000000u + (c << 17) : 0u); }
+
+__device__ __forceinline__ unsigned m_code(double x, double inv, unsigned r16) {
+  const double tiny = 0x1.2p-15;
+  const double y = fabs(x) * inv;
+  // (the random bits lie in the high word: the low word of y never decides)
+  const int k = (int)(((unsigned)__double2hiint(fmax(y, tiny)) + (r16 << 1)) >> 17) - ((1023 - 15) << 3);
+  if (y * 65536.0 + tiny * (double)r16 < tiny * 65536.0) return 0;
+  return (unsigned)min(max(k, 1), 127) | (x < 0.0 ? 128u : 0u);
+}
+__device__ __forceinline__ unsigned v_code(double x, double inv, unsigned r16) {
+  const double tiny = 0x1.2p-31;
+  const double y = x * inv;
+  const int k = (int)(((unsigned)__double2hiint(fmax(y, tiny)) + (r16 << 1)) >> 17) - ((1023 - 31) << 3);
+  return y > 0.0 ? (unsigned)min(max(k, 1), 255) : 0u;
+}
+
+template <int BITS>
+__global__ __launch_bounds__(256) void adamw_multi_kernel(const AwTab t, const AwArgs a) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int ti = aw_find(t, blockIdx.x);
+  const int64_t n = t.n[ti];
+  const int pt = t.pt[ti], gt = t.gt[ti];
+  void* pp = const_cast<void*>(t.p[ti]);
+  const void* gp = t.g[ti];
+  double coef = 1.0;
+  if (a.clip) {
+    const double norm = a.clip[0];
+    if (!(norm < __builtin_huge_val())) return;  // a NaN or infinite gradient: no step
+    coef = a.clip[1];
+  }
+  const int nblk = (int)((n + 255) >> 8);
+  const int b0 = (blockIdx.x - t.chunk0[ti]) * AW_CHUNK;
+  for (int bi = b0 + wave; bi < min(nblk, b0 + AW_CHUNK); bi += 4) {
+    const int64_t i = (int64_t)bi * 256 + lane * 4;
+    const int64_t blk = a.block0 + t.block0[ti] + bi, e = blk * 256 + lane * 4;
+    const f32x4 p0 = aw_load(pp, pt, i, n), g0 = aw_load(gp, gt, i, n);
+    f32x4 mf, vf;
+    if (BITS == 8) {
+      unsigned char* mc = reinterpret_cast<unsigned char*>(a.m);
+      unsigned char* vc = reinterpret_cast<unsigned char*>(a.v);
+      const unsigned cm = *reinterpret_cast<const unsigned*>(mc + e), cv = *reinterpret_cast<const unsigned*>(vc + e);
+      const double sm = a.ms[blk], sv = a.vs[blk];
+      double m[4], v[4];
+      float am = 0.f, av = 0.f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const double g = (double)g0[j] * coef;
+        m[j] = a.b1 * (m_value((cm >> (8 * j)) & 255u) * sm) + a.w1 * g;
+        v[j] = a.b2 * (v_value((cv >> (8 * j)) & 255u) * sv) + a.w2 * (g * g);
+        mf[j] = (float)m[j];
+        vf[j] = (float)v[j];
+        // the scale rounds max |x| / 1.875 to fp32: rounding keeps order, so the largest rounded value is it
+        am = fmaxf(am, (float)(fabs(m[j]) / 1.875));
+        av = fmaxf(av, (float)(v[j] / 1.875));
+      }
+      am = wave_max(am);
+      av = wave_max(av);
+      const double im = am > 0.f ? 1.0 / (double)am : 0.0, iv = av > 0.f ? 1.0 / (double)av : 0.0;
+      unsigned nm = 0, nv = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const unsigned r = aw_mix((unsigned)(e + j) + a.key);
+        if (i + j < n) {  // what lies behind the tensor's end stays 0
+          nm |= m_code(m[j], im, r & 0xFFFFu) << (8 * j);
+          nv |= v_code(v[j], iv, r >> 16) << (8 * j);
+        }
+      }
+      *reinterpret_cast<unsigned*>(mc + e) = nm;
+      *reinterpret_cast<unsigned*>(vc + e) = nv;
+      if (lane == 0) {
+        a.ms[blk] = am;
+        a.vs[blk] = av;
+      }
+    } else {
+      float* mm = reinterpret_cast<float*>(a.m) + e;
+      float* vv = reinterpret_cast<float*>(a.v) + e;
+      const float w1 = (float)a.w1, b2 = (float)a.b2, w2 = (float)a.w2, c = (float)coef;
+      mf = *reinterpret_cast<const f32x4*>(mm);
+      vf = *reinterpret_cast<const f32x4*>(vv);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float g = g0[j] * c;
+        mf[j] = mf[j] + (g - mf[j]) * w1;
+        vf[j] = vf[j] * b2 + w2 * g * g;
+      }
+      *reinterpret_cast<f32x4*>(mm) = mf;
+      *reinterpret_cast<f32x4*>(vv) = vf;
+    }
+    f32x4 q;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) q[j] = p0[j] * a.decay - a.step * (mf[j] / (sqrtf(vf[j]) / a.bc2s + a.eps));
+    aw_store(pp, pt, i, n, q);
+  }
+}
+
+// sums of squares in fp64, one per workgroup
+__global__ __launch_bounds__(256) void grad_sq_kernel(const AwTab t, double* __restrict__ part) {
+  __shared__ double r[4];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int ti = aw_find(t, blockIdx.x);
+  const int64_t n = t.n[ti];
+  const int nblk = (int)((n + 255) >> 8);
+  const int b0 = (blockIdx.x - t.chunk0[ti]) * AW_CHUNK;
+  double s = 0.0;
+  for (int bi = b0 + wave; bi < min(nblk, b0 + AW_CHUNK); bi += 4) {
+    const f32x4 g = aw_load(t.g[ti], t.gt[ti], (int64_t)bi * 256 + lane * 4, n);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) s += (double)g[j] * (double)g[j];
+  }
+#pragma unroll
+  for (int o = 32; o; o >>= 1) s += __shfl_xor(s, o);
+  if (lane == 0) r[wave] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) part[blockIdx.x] = (r[0] + r[1]) + (r[2] + r[3]);
+}
+__global__ __launch_bounds__(1024) void grad_norm_kernel(const double* __restrict__ part, int64_t n, double max_norm,
+                                                         double* __restrict__ out) {
+  __shared__ double r[1024];
+  double s = 0.0;
+  for (int64_t i = threadIdx.x; i < n; i += 1024) s += part[i];
+  r[threadIdx.x] = s;
+  __syncthreads();
+  for (int k = 512; k; k >>= 1) {
+    if ((int)threadIdx.x < k) r[threadIdx.x] += r[threadIdx.x + k];
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) {
+    const double norm = sqrt(r[0]), c = max_norm / (norm + 1e-6);
+    out[0] = norm;
+    out[1] = c < 1.0 ? c : 1.0;
+  }
+}
+
+// the values that 8-bit states stand for
+__global__ __launch_bounds__(256) void state_values_kernel(const unsigned* __restrict__ m, const float* __restrict__ ms,
+                                                           const unsigned* __restrict__ v, const float* __restrict__ vs,
+                                                           int64_t nquad, f32x4* __restrict__ mo, f32x4* __restrict__ vo) {
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < nquad; i += (int64_t)gridDim.x * 256) {
+    const unsigned cm = m[i], cv = v[i];
+    const double sm = ms[i >> 6], sv = vs[i >> 6];
+    f32x4 a, b;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      a[j] = (float)(m_value((cm >> (8 * j)) & 255u) * sm);
+      b[j] = (float)(v_value((cv >> (8 * j)) & 255u) * sv);
+    }
+    mo[i] = a;
+    vo[i] = b;
+  }
+}
+
+// ---------------------------------------------------------------------------------------------- host side
+// Calls fn(table, workgroups, first workgroup over all launches) for every AW_T tensors that have a gradient and values.
+template <typename F>
+static int for_tables(int nt, const void* const* p, const void* const* g, const int64_t* n, const uint8_t* pt,
+                      const uint8_t* gt, F fn) {
+  AwTab t;
+  t.count = 0;
+  int64_t blocks = 0, chunks = 0, before = 0;
+  for (int i = 0; i < nt; ++i) {
+    const int64_t nb = cdiv(n[i], 256);
+    if (g[i] && n[i]) {
+      t.p[t.count] = p ? p[i] : nullptr;
+      t.g[t.count] = g[i];
+      t.n[t.count] = n[i];
+      t.pt[t.count] = pt ? pt[i] : 0;
+      t.gt[t.count] = gt[i];
+      t.chunk0[t.count] = (int)chunks;
+      t.block0[t.count] = (int)blocks;
+      chunks += cdiv(nb, AW_CHUNK);
+      ++t.count;
+    }
+    blocks += nb;
+    if (t.count == AW_T || (i == nt - 1 && t.count)) {
+      if (int e = fn(t, (unsigned)chunks, before)) return e;
+      before += chunks;
+      chunks = 0;
+      t.count = 0;
+    }
+  }
+  return 0;
+}
+
+static const char* tensors_check(int nt, const void* const* g, const int64_t* n, const uint8_t* gt) {
+  if (nt < 0 || (nt && (!g || !n || !gt))) return "tensor list";
+  int64_t blocks = 0;
+  for (int i = 0; i < nt; ++i) {
+    if (n[i] < 0 || n[i] >= (int64_t)1 << 38) return "tensor size";
+    if (g[i] && gt[i] > IFD_F16) return "gradient type";
+    if ((uintptr_t)g[i] % (gt[i] == IFD_F32 ? 4 : 2)) return "a gradient's address is not a multiple of its element";
+    blocks += cdiv(n[i], 256);
+  }
+  if (blocks >= 0x7fffffff) return "more than 2^31 blocks of 256 values";
+  return nullptr;
+}
+
+}  // namespace ifd
+
+using namespace ifd;
+extern "C" {
+
+int64_t ifd_op_grad_norm_ws_bytes(int nt, const int64_t* n) {
+  int64_t c = 0;
+  for (int i = 0; i < nt && n; ++i) c += n[i] > 0 ? cdiv(cdiv(n[i], 256), AW_CHUNK) : 0;
+  return 8 * c;
+}
+
+int ifd_op_grad_norm(int nt, const void* const* g, const int64_t* n, const uint8_t* gtype, double max_norm,
+                     double* norm_coef, void* ws, int64_t ws_bytes, void* stream) {
+  const char* why = tensors_check(nt, g, n, gtype);
+  IFD_OP_REQUIRE(!why, why);
+  IFD_OP_REQUIRE(norm_coef != nullptr, "null norm_coef");
+  IFD_OP_REQUIRE(max_norm >= 0.0, "max_norm must not be negative");
+  const int64_t need = ifd_op_grad_norm_ws_bytes(nt, n);
+  IFD_OP_REQUIRE(ws_bytes >= need && (ws || !need), "workspace too small");
+  hipStream_t s = (hipStream_t)stream;
+  double* part = (double*)ws;
+  int64_t total = 0;
+  const int rc = for_tables(nt, nullptr, g, n, nullptr, gtype, [&](const AwTab& t, unsigned wgs, int64_t before) {
+    hipLaunchKernelGGL(grad_sq_kernel, dim3(wgs), dim3(256), 0, s, t, part + before);
+    total = before + wgs;
+    return launch_status("ifd_op_grad_norm");
+  });
+  if (rc) return rc;
+  hipLaunchKernelGGL(grad_norm_kernel, dim3(1), dim3(1024), 0, s, part, total, max_norm, norm_coef);
+  return IFD_LAUNCH_STATUS();
+}
+
+int ifd_op_adamw(const ifd_adamw_args* a, void* stream) {
+  IFD_OP_REQUIRE(a != nullptr, "null arguments");
+  const char* why = tensors_check(a->nt, a->g, a->n, a->gtype);
+  IFD_OP_REQUIRE(!why, why);
+  IFD_OP_REQUIRE(a->bits == 8 || a->bits == 32, "states have 8 or 32 bits");
+  IFD_OP_REQUIRE(a->step >= 1, "step counts from 1");
+  IFD_OP_REQUIRE(a->b1 >= 0.0 && a->b1 < 1.0 && a->b2 >= 0.0 && a->b2 < 1.0 && a->eps > 0.0, "b1, b2 or eps");
+  IFD_OP_REQUIRE(a->block0 >= 0, "block0");
+  if (!a->nt) return 0;
+  IFD_OP_REQUIRE(a->p && a->ptype && a->m && a->v && (a->bits == 32 || (a->m_scale && a->v_scale)), "a null tensor");
+  IFD_OP_REQUIRE(!((uintptr_t)a->m & 15) && !((uintptr_t)a->v & 15), "states must be aligned to 16 bytes");
+  for (int i = 0; i < a->nt; ++i) {
+    IFD_OP_REQUIRE(a->ptype[i] <= IFD_F16, "parameter type");
+    IFD_OP_REQUIRE(a->p[i] || !a->g[i] || !a->n[i], "a gradient without its parameter");
+    IFD_OP_REQUIRE((uintptr_t)a->p[i] % (a->ptype[i] == IFD_F32 ? 4 : 2) == 0,
+                   "a parameter's address is not a multiple of its element");
+  }
+  AwArgs k = {};
+  k.m = a->m; k.v = a->v; k.ms = a->m_scale; k.vs = a->v_scale; k.clip = a->norm_coef; k.block0 = a->block0;
+  k.b1 = a->b1; k.w1 = 1.0 - a->b1; k.b2 = a->b2; k.w2 = 1.0 - a->b2;
+  k.decay = (float)(1.0 - a->lr * a->wd);
+  k.step = (float)(a->lr / (1.0 - std::pow(a->b1, a->step)));
+  k.eps = (float)a->eps;
+  k.bc2s = (float)std::sqrt(1.0 - std::pow(a->b2, a->step));
+  k.key = aw_mix(aw_mix(a->seed) + (unsigned)a->step);
+  hipStream_t s = (hipStream_t)stream;
+  return for_tables(a->nt, a->p, a->g, a->n, a->ptype, a->gtype, [&](const AwTab& t, unsigned wgs, int64_t) {
+    if (a->bits == 8)
+      hipLaunchKernelGGL(adamw_multi_kernel<8>, dim3(wgs), dim3(256), 0, s, t, k);
+    else
+      hipLaunchKernelGGL(adamw_multi_kernel<32>, dim3(wgs), dim3(256), 0, s, t, k);
+    return launch_status("ifd_op_adamw");
+  });
+}
+
+int ifd_op_state_values(const void* m, const float* m_scale, const void* v, const float* v_scale, int64_t nblocks,
+                        float* m_out, float* v_out, void* stream) {
+  IFD_OP_REQUIRE(nblocks >= 0 && nblocks < 0x7fffffff, "nblocks");
+  if (!nblocks) return 0;
+  IFD_OP_REQUIRE(m && v && m_scale && v_scale && m_out && v_out, "a null tensor");
+  IFD_OP_REQUIRE(!(((uintptr_t)m | (uintptr_t)v) & 3) && !(((uintptr_t)m_out | (uintptr_t)v_out) & 15),
+                 "states must be aligned to 4 bytes, outputs to 16");
+  hipLaunchKernelGGL(state_values_kernel, dim3((unsigned)std::min<int64_t>(cdiv(nblocks, 4), 16384)), dim3(256), 0,
+                     (hipStream_t)stream, (const unsigned*)m, m_scale, (const unsigned*)v, v_scale, nblocks * 64,
+                     (f32x4*)m_out, (f32x4*)v_out);
+  return IFD_LAUNCH_STATUS();
+}
+
+}  // extern "C"

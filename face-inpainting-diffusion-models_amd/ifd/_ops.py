@@ -23,11 +23,35 @@ class AttentionArgs(ctypes.Structure):
                 + [(n, Strides) for n in ("dout_s", "dq_s", "dk_s", "dv_s")])
 
 
+class QkArgs(ctypes.Structure):
+    """ifd_qk_args"""
+    _fields_ = ([(n, i32) for n in ("dtype", "B", "T", "Hq", "Hk", "D", "rot", "interleaved", "norm")]
+                + [("eps", f32), ("mscale", f32), ("pad", i32)]
+                + [(n, vp) for n in ("q", "k", "q_out", "k_out", "wq", "wk", "pos", "turns")]
+                + [(n, Strides) for n in ("q_s", "k_s", "q_out_s", "k_out_s")] + [("pos_s", i64 * 2)]
+                + [(n, vp) for n in ("gq", "gk", "dq", "dk", "dwq", "dwk")]
+                + [(n, Strides) for n in ("gq_s", "gk_s", "dq_s", "dk_s")])
+
+
+class AdamwArgs(ctypes.Structure):
+    """ifd_adamw_args"""
+    _fields_ = ([(n, i32) for n in ("nt", "bits", "step")] + [("seed", _c.c_uint32)]
+                + [(n, vp) for n in ("p", "g", "n", "ptype", "gtype", "m", "v", "m_scale", "v_scale")]
+                + [("block0", i64)] + [(n, _c.c_double) for n in ("lr", "b1", "b2", "eps", "wd")] + [("norm_coef", vp)])
+
+
 OPS_EXPORTS = {
     "ifd_op_attention_ws_bytes": (i64, [_c.POINTER(AttentionArgs)]),
     "ifd_op_attention": (i32, [_c.POINTER(AttentionArgs), vp, i64, vp]),
     "ifd_op_attention_bwd_ws_bytes": (i64, [_c.POINTER(AttentionArgs)]),
     "ifd_op_attention_bwd": (i32, [_c.POINTER(AttentionArgs), vp, i64, vp]),
+    "ifd_op_qk_norm_rope": (i32, [_c.POINTER(QkArgs), vp]),
+    "ifd_op_qk_norm_rope_bwd_ws_bytes": (i64, [_c.POINTER(QkArgs)]),
+    "ifd_op_qk_norm_rope_bwd": (i32, [_c.POINTER(QkArgs), vp, i64, vp]),
+    "ifd_op_grad_norm_ws_bytes": (i64, [i32, vp]),
+    "ifd_op_grad_norm": (i32, [i32, vp, vp, vp, _c.c_double, vp, vp, i64, vp]),
+    "ifd_op_adamw": (i32, [_c.POINTER(AdamwArgs), vp]),
+    "ifd_op_state_values": (i32, [vp, vp, vp, vp, i64, vp, vp, vp]),
 }
 
 _bound = None

@@ -51,6 +51,67 @@ int ifd_op_attention(const ifd_attention_args* a, void* ws, int64_t ws_bytes, vo
 int64_t ifd_op_attention_bwd_ws_bytes(const ifd_attention_args* a);
 int ifd_op_attention_bwd(const ifd_attention_args* a, void* ws, int64_t ws_bytes, void* stream);
 
+/* Per-head RMS norm of queries and keys and the rotation by their positions, in one pass.
+ *   n = x / sqrt(mean x^2 + eps) * w (norm != 0; w NULL: 1), else n = x
+ *   the first `rot` channels in pairs (i, i + rot / 2), or (2i, 2i + 1) with interleaved != 0, turned by the angle
+ *   2 pi pos turns[i] and scaled by mscale; the other channels are n.
+ * q, k, their outputs and gradients: [B][T][Hq | Hk][D] of one type, strides {batch, token, head} in elements, channels
+ * adjacent (any alignment; 16 bytes is fastest). Hq or Hk may be 0. An output may be its input (in place). pos int64 with
+ * strides {batch, token} (0: shared); turns fp64 [rot / 2]: frequency / 2 pi. D <= 128, even. */
+typedef struct ifd_qk_args {
+  int dtype, B, T, Hq, Hk, D, rot, interleaved, norm;
+  float eps, mscale;
+  int pad;
+  const void *q, *k;
+  void *q_out, *k_out;
+  const float *wq, *wk;
+  const int64_t* pos;
+  const double* turns;
+  int64_t q_s[3], k_s[3], q_out_s[3], k_out_s[3], pos_s[2];
+  /* backward only: gq, gk the gradients of the outputs; dq, dk, and dwq, dwk [D] fp32 (NULL: not wanted) are written */
+  const void *gq, *gk;
+  void *dq, *dk;
+  float *dwq, *dwk;
+  int64_t gq_s[3], gk_s[3], dq_s[3], dk_s[3];
+} ifd_qk_args;
+int ifd_op_qk_norm_rope(const ifd_qk_args* a, void* stream);
+int64_t ifd_op_qk_norm_rope_bwd_ws_bytes(const ifd_qk_args* a);
+int ifd_op_qk_norm_rope_bwd(const ifd_qk_args* a, void* ws, int64_t ws_bytes, void* stream);
+
+/* The global norm of many gradients and its clip coefficient: norm_coef (device) = {norm, min(1, max_norm / (norm +
+ * 1e-6))}, summed in fp64. g, n, gtype: HOST arrays of nt entries (addresses on the device, element counts, IFD_F32 ...);
+ * a NULL gradient is skipped. */
+int64_t ifd_op_grad_norm_ws_bytes(int nt, const int64_t* n);
+int ifd_op_grad_norm(int nt, const void* const* g, const int64_t* n, const uint8_t* gtype, double max_norm,
+                     double* norm_coef, void* ws, int64_t ws_bytes, void* stream);
+
+/* One AdamW step over nt tensors (p, g, n, ptype, gtype: HOST arrays; a tensor with a NULL gradient is left alone).
+ * Tensor i's states are blocks of 256 values, ceil(n[i] / 256) of them, after those of the tensors before it, from block
+ * block0 on; what lies behind a tensor's end in its last block is 0.
+ *   bits 32: m, v fp32 [blocks][256];  bits 8: m, v bytes [blocks][256] and m_scale, v_scale fp32 [blocks]
+ *   (m: sign, 4 exponent, 3 fraction bits; v: 5 exponent, 3 fraction bits; largest value 1.875 scale; rounded up or down
+ *   at random, from seed and step).
+ * norm_coef (device, from ifd_op_grad_norm) or NULL: the gradients are scaled by norm_coef[1]; a norm that is not finite
+ * leaves everything as it was. Without it a gradient that is not finite spoils its parameter and state, with 8-bit states
+ * the 256 values that share its scale. */
+typedef struct ifd_adamw_args {
+  int nt, bits, step;
+  uint32_t seed;
+  void* const* p;
+  const void* const* g;
+  const int64_t* n;
+  const uint8_t *ptype, *gtype;
+  void *m, *v;
+  float *m_scale, *v_scale;
+  int64_t block0;
+  double lr, b1, b2, eps, wd;
+  const double* norm_coef;
+} ifd_adamw_args;
+int ifd_op_adamw(const ifd_adamw_args* a, void* stream);
+/* The fp32 values that 8-bit states stand for. */
+int ifd_op_state_values(const void* m, const float* m_scale, const void* v, const float* v_scale, int64_t nblocks,
+                        float* m_out, float* v_out, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

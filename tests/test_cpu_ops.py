@@ -93,3 +93,119 @@ def test_attention_python_refusals():
             attention(a, b, c, **kw)
         with pytest.raises(ValueError, match=msg):
             attention_bwd(a, a, b, c, a, None, **kw)
+
+
+def test_qk_refusals():
+    from ifd import _lib, _ops
+    from ifd.rotary import Rotary, qk_norm_rope, qk_norm_rope_bwd
+    L = _ops.lib()
+    S = _ops.Strides
+    good = dict(dtype=1, B=1, T=2, Hq=2, Hk=1, D=64, rot=64, norm=1, eps=1e-6, mscale=1.0)
+    for kw, msg in ((dict(dtype=3), "dtype"), (dict(D=130), "head width"), (dict(D=63), "head width"), (dict(rot=66), "rotated"),
+                    (dict(rot=3), "rotated"), (dict(eps=-1.0), "eps"), (dict(eps=float("nan")), "eps"), (dict(B=-1), "sizes"),
+                    ({}, "null tensor")):
+        a = _ops.QkArgs(**{**good, **kw})
+        for name, args in (("ifd_op_qk_norm_rope", ()), ("ifd_op_qk_norm_rope_bwd", (None, 1 << 30))):
+            with pytest.raises(RuntimeError, match=name + ": .*" + msg):
+                _lib.check(getattr(L, name)(ctypes.byref(a), *args, None))
+    a = _ops.QkArgs(**good)
+    for n in ("q", "k", "q_out", "k_out", "gq", "gk", "dq", "dk"):
+        setattr(a, n, 0x10000)
+    with pytest.raises(RuntimeError, match="positions"):
+        _lib.check(L.ifd_op_qk_norm_rope(ctypes.byref(a), None))
+    a.pos = a.turns = 0x10000
+    need = L.ifd_op_qk_norm_rope_bwd_ws_bytes(ctypes.byref(a))
+    with pytest.raises(RuntimeError, match="workspace"):
+        _lib.check(L.ifd_op_qk_norm_rope_bwd(ctypes.byref(a), 0x10000, need - 1, None))
+    assert L.ifd_op_qk_norm_rope(ctypes.byref(_ops.QkArgs(**{**good, "T": 0})), None) == 0
+    for args, kw in (((0,), {}), ((7,), {}), ((64,), dict(base=1.0)), ((64,), dict(scaling=("cubic", 2.0))),
+                     ((64,), dict(scaling=("linear", 0.5))), ((64,), dict(scaling=("bands", 2.0))),
+                     ((64,), dict(scaling=("bands", 2.0, 0)))):
+        with pytest.raises(ValueError):
+            Rotary(*args, device="cpu", **kw)
+    rope, q, k = Rotary(64, device="cpu"), torch.zeros(1, 2, 2, 64), torch.zeros(1, 2, 1, 64)
+    pos = torch.arange(2)
+    for a, kw, msg in (((q[0], k), {}, "tokens, heads"), ((q, k.half()), {}, "one type"), ((q, k[:, :1]), {}, "k must be"),
+                       ((q[..., :32], k[..., :32], None, None, pos, rope), {}, "rotated channels"),
+                       ((q, k, None, None, None, rope), {}, "positions"), ((q, k, torch.ones(64)), dict(norm=False), "weights"),
+                       ((q, k), dict(eps=-1.0), "eps"), ((q, k), {}, "GPU tensor")):
+        with pytest.raises(ValueError, match=msg):
+            qk_norm_rope(*a, **kw)
+        with pytest.raises(ValueError, match=msg):
+            qk_norm_rope_bwd(a[0], a[1], *a, **kw)
+    del S
+
+
+def test_rotary_frequencies():
+    """The scalings' defining properties, in fp64."""
+    import math
+    from ifd.rotary import Rotary
+    plain = Rotary(64, device="cpu").inv_freq
+    assert plain[0] == 1.0 and abs(plain[16].item() - 10000.0 ** -0.5) < 1e-15
+    assert torch.allclose(Rotary(64, scaling=("linear", 4.0), device="cpu").inv_freq, plain / 4, rtol=1e-15)
+    wide = Rotary(64, scaling=("base", 4.0), device="cpu").inv_freq
+    assert wide[0] == 1.0 and abs(wide[-1] / plain[-1] - 0.25) < 1e-12
+    r = Rotary(64, scaling=("bands", 4.0, 4096), device="cpu")
+    turns = 4096 * plain / (2 * math.pi)
+    assert torch.equal(r.inv_freq[turns >= 32], plain[turns >= 32])
+    assert torch.allclose(r.inv_freq[turns <= 1], plain[turns <= 1] / 4, rtol=1e-15)
+    assert ((r.inv_freq <= plain) & (r.inv_freq >= plain / 4 * (1 - 1e-12))).all() and abs(r.mscale - 1.1386294) < 1e-6
+
+
+def _adamw_args(keep, **kw):
+    from ifd._ops import AdamwArgs
+    c = ctypes
+    n = kw.pop("n", [300, 5])
+    p, g = kw.pop("p", [0x10000] * len(n)), kw.pop("g", [0x20000] * len(n))
+    d = dict(nt=len(n), bits=8, step=1, block0=0, lr=1e-3, b1=0.9, b2=0.999, eps=1e-8, wd=0.0)
+    arr = dict(p=(c.c_void_p * len(n))(*p), g=(c.c_void_p * len(n))(*g), n=(c.c_int64 * len(n))(*n),
+               ptype=(c.c_uint8 * len(n))(*kw.pop("ptype", [0] * len(n))),
+               gtype=(c.c_uint8 * len(n))(*kw.pop("gtype", [0] * len(n))))
+    st = {s: kw.pop(s, 0x30000) for s in ("m", "v", "m_scale", "v_scale")}
+    a = AdamwArgs(**{**d, **kw})
+    keep.append(arr)
+    for k, v in arr.items():
+        setattr(a, k, c.cast(v, c.c_void_p))
+    for k, v in st.items():
+        setattr(a, k, v)
+    return a
+
+
+def test_adamw_refusals():
+    from ifd import _lib, _ops
+    L, keep = _ops.lib(), []
+    for kw, msg in ((dict(bits=16), "8 or 32"), (dict(step=0), "step"), (dict(b1=1.0), "b1"), (dict(b2=-0.1), "b2"),
+                    (dict(eps=0.0), "eps"), (dict(nt=-1), "tensor list"), (dict(n=[-1, 2]), "size"),
+                    (dict(gtype=[9, 0]), "gradient type"), (dict(ptype=[3, 0]), "parameter type"),
+                    (dict(p=[None, 0x10000]), "without its parameter"), (dict(p=[0x10002, 0x10000]), "element"),
+                    (dict(g=[0x20001, 0x20000]), "element"), (dict(m=None), "null"), (dict(v_scale=None), "null"),
+                    (dict(m=0x30008), "aligned"), (dict(n=[1 << 39, 1]), "size"), (dict(n=[1 << 37] * 5, p=[0x10000] * 5), "blocks"),
+                    (dict(block0=-1), "block0")):
+        if "n" in kw and len(kw["n"]) == 5:
+            kw["g"] = [0x20000] * 5
+        with pytest.raises(RuntimeError, match="ifd_op_adamw: .*" + msg):
+            _lib.check(L.ifd_op_adamw(ctypes.byref(_adamw_args(keep, **kw)), None))
+    assert L.ifd_op_adamw(ctypes.byref(_adamw_args(keep, g=[None, None])), None) == 0  # no gradients: nothing to do
+    n, g, t = (ctypes.c_int64 * 1)(5000), (ctypes.c_void_p * 1)(0x20000), (ctypes.c_uint8 * 1)(0)
+    need = L.ifd_op_grad_norm_ws_bytes(1, n)
+    assert need > 0
+    for args, msg in (((1, g, n, t, 1.0, None, 0x30000, need), "norm_coef"), ((1, g, n, t, -1.0, 0x30000, 0x30000, need), "max_norm"),
+                      ((1, g, n, t, 1.0, 0x30000, 0x30000, need - 1), "workspace"), ((1, None, n, t, 1.0, 0x30000, 0x30000, need), "list")):
+        with pytest.raises(RuntimeError, match="ifd_op_grad_norm: .*" + msg):
+            _lib.check(L.ifd_op_grad_norm(*args, None))
+    for args, msg in (((None, None, None, None, 4, None, None), "null"), ((0x1, 0x4, 0x4, 0x4, 4, 0x10, 0x10), "aligned"),
+                      ((None, None, None, None, -1, None, None), "nblocks")):
+        with pytest.raises(RuntimeError, match="ifd_op_state_values: .*" + msg):
+            _lib.check(L.ifd_op_state_values(*args, None))
+    assert L.ifd_op_state_values(None, None, None, None, 0, None, None, None) == 0
+
+
+def test_adamw_python_refusals():
+    from ifd.optim import AdamW
+    p = torch.zeros(8)
+    for args, kw, msg in ((([p],), dict(state_bits=16), "state_bits"), (([p],), dict(betas=(1.0, 0.9)), "betas"),
+                          (([p],), dict(eps=0.0), "eps"), (([p],), dict(max_norm=0.0), "max_norm"), (([],), {}, "no parameters"),
+                          (([p.double()],), {}, "contiguous fp32"), (([torch.zeros(4, 4).t()[:, :2]],), {}, "contiguous"),
+                          (([p, p],), {}, "twice"), (([p],), {}, "GPU tensor"), (([{"params": [p]}, p],), {}, "groups")):
+        with pytest.raises(ValueError, match=msg):
+            AdamW(*args, **kw)
