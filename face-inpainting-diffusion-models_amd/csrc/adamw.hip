@@ -39,7 +39,7 @@ struct AwArgs {
   const double* clip;  // {norm, coefficient} or null
   int64_t block0;
   double b1, w1, b2, w2;
-  float decay, step, eps, bc2s;
+  float decay, step, eps, rbc2s;
   unsigned key;
 };
 
@@ -174,7 +174,7 @@ __global__ __launch_bounds__(256) void adamw_multi_kernel(const AwTab t, const A
       const unsigned cm = *reinterpret_cast<const unsigned*>(mc + e), cv = *reinterpret_cast<const unsigned*>(vc + e);
       const double sm = a.ms[blk], sv = a.vs[blk];
       double m[4], v[4];
-      float am = 0.f, av = 0.f;
+      double xm = 0.0, xv = 0.0;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const double g = (double)g0[j] * coef;
@@ -182,12 +182,11 @@ __global__ __launch_bounds__(256) void adamw_multi_kernel(const AwTab t, const A
         v[j] = a.b2 * (v_value((cv >> (8 * j)) & 255u) * sv) + a.w2 * (g * g);
         mf[j] = (float)m[j];
         vf[j] = (float)v[j];
-        // the scale rounds max |x| / 1.875 to fp32: rounding keeps order, so the largest rounded value is it
-        am = fmaxf(am, (float)(fabs(m[j]) / 1.875));
-        av = fmaxf(av, (float)(v[j] / 1.875));
+        xm = fmax(xm, fabs(m[j]));
+        xv = fmax(xv, v[j]);
       }
-      am = wave_max(am);
-      av = wave_max(av);
+      // the scale rounds max |x| / 1.875 to fp32: rounding keeps order, so the largest rounded value of the lanes is it
+      const float am = wave_max((float)(xm * (1.0 / 1.875))), av = wave_max((float)(xv * (1.0 / 1.875)));
       const double im = am > 0.f ? 1.0 / (double)am : 0.0, iv = av > 0.f ? 1.0 / (double)av : 0.0;
       unsigned nm = 0, nv = 0;
 #pragma unroll
@@ -221,7 +220,9 @@ __global__ __launch_bounds__(256) void adamw_multi_kernel(const AwTab t, const A
     }
     f32x4 q;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) q[j] = p0[j] * a.decay - a.step * (mf[j] / (sqrtf(vf[j]) / a.bc2s + a.eps));
+    for (int j = 0; j < 4; ++j)  // hardware square root and reciprocal: 1 ulp each, of the step
+      q[j] = p0[j] * a.decay -
+             a.step * (mf[j] * __builtin_amdgcn_rcpf(fmaf(__builtin_amdgcn_sqrtf(vf[j]), a.rbc2s, a.eps)));
     aw_store(pp, pt, i, n, q);
   }
 }
@@ -382,7 +383,7 @@ int ifd_op_adamw(const ifd_adamw_args* a, void* stream) {
   k.decay = (float)(1.0 - a->lr * a->wd);
   k.step = (float)(a->lr / (1.0 - std::pow(a->b1, a->step)));
   k.eps = (float)a->eps;
-  k.bc2s = (float)std::sqrt(1.0 - std::pow(a->b2, a->step));
+  k.rbc2s = (float)(1.0 / std::sqrt(1.0 - std::pow(a->b2, a->step)));
   k.key = aw_mix(aw_mix(a->seed) + (unsigned)a->step);
   hipStream_t s = (hipStream_t)stream;
   return for_tables(a->nt, a->p, a->g, a->n, a->ptype, a->gtype, [&](const AwTab& t, unsigned wgs, int64_t) {

@@ -41,16 +41,16 @@ class AdamwArgs(ctypes.Structure):
 
 
 OPS_EXPORTS = {
-    "ifd_op_attention_ws_bytes": (i64, [_c.POINTER(AttentionArgs)]),
-    "ifd_op_attention": (i32, [_c.POINTER(AttentionArgs), vp, i64, vp]),
-    "ifd_op_attention_bwd_ws_bytes": (i64, [_c.POINTER(AttentionArgs)]),
-    "ifd_op_attention_bwd": (i32, [_c.POINTER(AttentionArgs), vp, i64, vp]),
-    "ifd_op_qk_norm_rope": (i32, [_c.POINTER(QkArgs), vp]),
-    "ifd_op_qk_norm_rope_bwd_ws_bytes": (i64, [_c.POINTER(QkArgs)]),
-    "ifd_op_qk_norm_rope_bwd": (i32, [_c.POINTER(QkArgs), vp, i64, vp]),
+    "ifd_op_attention_ws_bytes": (i64, [vp]),
+    "ifd_op_attention": (i32, [vp, vp, i64, vp]),
+    "ifd_op_attention_bwd_ws_bytes": (i64, [vp]),
+    "ifd_op_attention_bwd": (i32, [vp, vp, i64, vp]),
+    "ifd_op_qk_norm_rope": (i32, [vp, vp]),
+    "ifd_op_qk_norm_rope_bwd_ws_bytes": (i64, [vp]),
+    "ifd_op_qk_norm_rope_bwd": (i32, [vp, vp, i64, vp]),
     "ifd_op_grad_norm_ws_bytes": (i64, [i32, vp]),
     "ifd_op_grad_norm": (i32, [i32, vp, vp, vp, _c.c_double, vp, vp, i64, vp]),
-    "ifd_op_adamw": (i32, [_c.POINTER(AdamwArgs), vp]),
+    "ifd_op_adamw": (i32, [vp, vp]),
     "ifd_op_state_values": (i32, [vp, vp, vp, vp, i64, vp, vp, vp]),
 }
 
@@ -69,9 +69,8 @@ def lib():
     return L
 
 
-def need(cond, msg):
-    if not cond:
-        raise ValueError("ifd: " + msg)
+def refuse(msg):
+    raise ValueError("ifd: " + msg)
 
 
 def same_device(*tensors):
@@ -80,12 +79,27 @@ def same_device(*tensors):
     for t in tensors:
         if t is None:
             continue
-        need(t.is_cuda, f"expected a GPU tensor, got one on {t.device}")
-        need(dev is None or t.device == dev, f"tensors on {dev} and on {t.device}")
-        dev = t.device
+        d = t.device
+        if d != dev:
+            if d.type != "cuda":
+                refuse(f"expected a GPU tensor, got one on {d}")
+            if dev is not None:
+                refuse(f"tensors on {dev} and on {d}")
+            dev = d
     return dev
 
 
 def workspace(nbytes, dev):
     """Scratch of one call, from torch's stream-ordered allocator (None when the call needs none)."""
     return torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+
+
+def call(fn, dev, *args):
+    """fn(*args, stream) on the current stream of `dev`, with that device current; raises on a non-zero status."""
+    if torch.cuda.current_device() == dev.index:
+        rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+    if rc:
+        _lib.check(rc)

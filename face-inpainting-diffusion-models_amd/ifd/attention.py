@@ -18,101 +18,110 @@ Calls run on the current stream of the tensors' device and can be captured into 
 """
 from __future__ import annotations
 
-import ctypes
 import math
+import struct
 
 import torch
 
-from . import _lib
-from ._ops import DTYPES, AttentionArgs, Strides, lib, need, same_device, workspace
+from ._ops import DTYPES, call, lib, refuse, same_device, workspace
+
+# ifd_attention_args (include/ifd_ops.h): packed here because filling a ctypes structure field by field costs more than
+# the smallest kernels run (_ops.AttentionArgs has the same layout)
+_FWD, _BWD = struct.Struct("8if i 7P 12q"), struct.Struct("4P 12q")
+_NO_BWD = bytes(_BWD.size)
 
 
 def _lay(t):
     """t itself when the kernels can read it, else a contiguous copy."""
+    s0, s1, s2, s3 = t.stride()
     e = t.element_size()
-    ok = t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all((s * e) % 16 == 0 for s in t.stride()[:3])
-    if ok and 0 <= t.stride(1) * e < 1 << 24:
+    if s3 == 1 and 0 <= s1 * e < 1 << 24 and not ((s0 | s1 | s2) * e | t.data_ptr()) & 15:
         return t
     return t.clone(memory_format=torch.contiguous_format)
 
 
-def _st(t):
-    return Strides(*t.stride()[:3])
-
-
 def _int_arg(t, B, name, dev):
-    if t is None:
-        return None
-    need(isinstance(t, torch.Tensor) and t.dtype == torch.int32 and t.dim() == 1 and t.shape[0] == B,
-         f"{name} must be an int32 tensor of shape [{B}]")
-    need(t.device == dev, f"{name} must be on {dev}")
+    if not (isinstance(t, torch.Tensor) and t.dtype == torch.int32 and t.shape == (B,)):
+        refuse(f"{name} must be an int32 tensor of shape [{B}]")
+    if t.device != dev:
+        refuse(f"{name} must be on {dev}")
     return t.contiguous()
 
 
-def _args(q, k, v, scale, causal, kv_len, q_start):
-    for n, t in (("q", q), ("k", k), ("v", v)):
-        need(t.dim() == 4, f"{n} must be [batch, tokens, heads, channels]")
-    B, Tq, Hq, D = q.shape
-    Tk, Hk = k.shape[1], k.shape[2]
-    need(q.dtype in DTYPES and k.dtype == q.dtype and v.dtype == q.dtype, "q, k, v must have one type: fp32, bf16 or fp16")
-    need(k.shape == (B, Tk, Hk, D) and v.shape == k.shape, f"k, v must be [{B}, tokens, heads, {D}] and alike")
-    need(Hk > 0 and Hq > 0 and Hq % Hk == 0, f"{Hq} query heads are not a multiple of {Hk} key-value heads")
-    ce = 16 // q.element_size()
-    need(0 < D <= 128 and D % ce == 0, f"head width {D}: at most 128 and a multiple of {ce}")
+def _inputs(q, k, v, scale, kv_len, q_start):
+    """Checked inputs: (q, k, v as the kernels read them, scale, kv_len, q_start, device)."""
+    if not q.dim() == k.dim() == v.dim() == 4:
+        refuse("q, k, v must be [batch, tokens, heads, channels]")
+    B, _, Hq, D = q.shape
+    kB, Tk, Hk, kD = k.shape
+    if not (q.dtype in DTYPES and k.dtype == q.dtype and v.dtype == q.dtype):
+        refuse(f"q, k, v must have one type, fp32, bf16 or fp16, got {q.dtype}, {k.dtype}, {v.dtype}")
+    if kB != B or kD != D or v.shape != k.shape:
+        refuse(f"k, v must be [{B}, tokens, heads, {D}] and alike, got {tuple(k.shape)} and {tuple(v.shape)}")
+    if not (Hk > 0 and Hq > 0 and Hq % Hk == 0):
+        refuse(f"{Hq} query heads are not a multiple of {Hk} key-value heads")
+    if not 0 < D <= 128 or D * q.element_size() & 15:
+        refuse(f"head width {D}: at most 128 and a multiple of {16 // q.element_size()}")
     scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
-    need(0.0 < scale < 3e38, f"scale must be positive and finite, got {scale}")
+    if not 0.0 < scale < 3e38:
+        refuse(f"scale must be positive and finite, got {scale}")
     dev = same_device(q, k, v)
-    kv_len, q_start = _int_arg(kv_len, B, "kv_len", dev), _int_arg(q_start, B, "q_start", dev)
-    q, k, v = _lay(q), _lay(k), _lay(v)
-    a = AttentionArgs(dtype=DTYPES[q.dtype], B=B, Tq=Tq, Tk=Tk, Hq=Hq, Hk=Hk, D=D, causal=int(bool(causal)), scale=scale)
-    a.q, a.k, a.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
-    a.q_s, a.k_s, a.v_s = _st(q), _st(k), _st(v)
-    a.kv_len = None if kv_len is None else kv_len.data_ptr()
-    a.q_start = None if q_start is None else q_start.data_ptr()
-    return a, (q, k, v, kv_len, q_start), dev
+    if kv_len is not None:
+        kv_len = _int_arg(kv_len, B, "kv_len", dev)
+    if q_start is not None:
+        q_start = _int_arg(q_start, B, "q_start", dev)
+    return _lay(q), _lay(k), _lay(v), scale, kv_len, q_start, dev
+
+
+def _pack(q, k, v, scale, causal, kv_len, q_start, out, lse):
+    B, Tq, Hq, D = q.shape
+    return _FWD.pack(DTYPES[q.dtype], B, Tq, k.shape[1], Hq, k.shape[2], D, 1 if causal else 0, scale, 0, q.data_ptr(),
+                     k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), 0 if kv_len is None else kv_len.data_ptr(),
+                     0 if q_start is None else q_start.data_ptr(), *q.stride()[:3], *k.stride()[:3], *v.stride()[:3],
+                     *out.stride()[:3])
 
 
 def _into(t, like, name):
     """A caller's output tensor (checked) or a new contiguous one."""
     if t is None:
         return torch.empty(like.shape, dtype=like.dtype, device=like.device)
-    need(t.shape == like.shape and t.dtype == like.dtype and t.device == like.device, f"{name} must be like its input")
-    need(_lay(t) is t, f"{name}: adjacent channels, 16-byte aligned, strides in multiples of 16 bytes")
+    if not (t.shape == like.shape and t.dtype == like.dtype and t.device == like.device):
+        refuse(f"{name} must be like its input")
+    if _lay(t) is not t:
+        refuse(f"{name}: adjacent channels, 16-byte aligned, strides in multiples of 16 bytes")
     return t
 
 
 def attention(q, k, v, scale=None, causal=False, kv_len=None, q_start=None, out=None):
     """(out, lse): attention of every query row, and its log-sum-exp fp32 [B, Hq, Tq]."""
-    a, keep, dev = _args(q, k, v, scale, causal, kv_len, q_start)
+    q, k, v, scale, kv_len, q_start, dev = _inputs(q, k, v, scale, kv_len, q_start)
     out = _into(out, q, "out")
-    lse = torch.empty(a.B, a.Hq, a.Tq, dtype=torch.float32, device=dev)
-    a.out, a.out_s, a.lse = out.data_ptr(), _st(out), lse.data_ptr()
+    lse = torch.empty((q.shape[0], q.shape[2], q.shape[1]), dtype=torch.float32, device=dev)
+    a = _pack(q, k, v, scale, causal, kv_len, q_start, out, lse) + _NO_BWD
     L = lib()
-    with torch.cuda.device(dev):
-        n = L.ifd_op_attention_ws_bytes(ctypes.byref(a))
-        ws = workspace(n, dev)
-        _lib.check(L.ifd_op_attention(ctypes.byref(a), _lib.ptr(ws), n, _lib.stream_ptr(dev)))
+    n = L.ifd_op_attention_ws_bytes(a)
+    ws = workspace(n, dev)
+    call(L.ifd_op_attention, dev, a, None if ws is None else ws.data_ptr(), n)
     return out, lse
 
 
 def attention_bwd(dout, q, k, v, out, lse, scale=None, causal=False, kv_len=None, q_start=None, dq=None, dk=None, dv=None):
     """(dq, dk, dv) from the gradient of `out`; out, lse and the other arguments as the forward call had them.
     Keys at and past kv_len get zero gradients."""
-    a, keep, dev = _args(q, k, v, scale, causal, kv_len, q_start)
+    q, k, v, scale, kv_len, q_start, dev = _inputs(q, k, v, scale, kv_len, q_start)
     for n, t in (("dout", dout), ("out", out)):
-        need(t.shape == q.shape and t.dtype == q.dtype, f"{n} must be like q")
-    need(lse.shape == (a.B, a.Hq, a.Tq) and lse.dtype == torch.float32, f"lse must be fp32 [{a.B}, {a.Hq}, {a.Tq}]")
+        if not (t.shape == q.shape and t.dtype == q.dtype):
+            refuse(f"{n} must be like q")
+    if lse.shape != (q.shape[0], q.shape[2], q.shape[1]) or lse.dtype != torch.float32:
+        refuse("lse must be the forward's, fp32 [B, Hq, Tq]")
     same_device(q, dout, out, lse)
     dout, out, lse = _lay(dout), _lay(out), lse.contiguous()
     dq, dk, dv = _into(dq, q, "dq"), _into(dk, k, "dk"), _into(dv, v, "dv")
-    for n in ("dout", "out", "dq", "dk", "dv"):
-        t = locals()[n]
-        setattr(a, n, t.data_ptr())
-        setattr(a, n + "_s", _st(t))
-    a.lse = lse.data_ptr()
+    a = _pack(q, k, v, scale, causal, kv_len, q_start, out, lse) + _BWD.pack(
+        dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), *dout.stride()[:3], *dq.stride()[:3],
+        *dk.stride()[:3], *dv.stride()[:3])
     L = lib()
-    with torch.cuda.device(dev):
-        n = L.ifd_op_attention_bwd_ws_bytes(ctypes.byref(a))
-        ws = workspace(n, dev)
-        _lib.check(L.ifd_op_attention_bwd(ctypes.byref(a), _lib.ptr(ws), n, _lib.stream_ptr(dev)))
+    n = L.ifd_op_attention_bwd_ws_bytes(a)
+    ws = workspace(n, dev)
+    call(L.ifd_op_attention_bwd, dev, a, None if ws is None else ws.data_ptr(), n)
     return dq, dk, dv

@@ -20,10 +20,14 @@ import ctypes
 
 import torch
 
-from . import _lib
-from ._ops import DTYPES, AdamwArgs, lib, need, same_device, workspace
+from ._ops import DTYPES, AdamwArgs, call, lib, refuse, same_device, workspace
 
 BLOCK = 256  # values per scale
+
+
+def need(cond, msg):
+    if not cond:
+        refuse(msg)
 
 
 class AdamW:
@@ -49,6 +53,7 @@ class AdamW:
         at = 0
         for g in self.groups:
             g["block0"] = at
+            g["sizes"] = [p.numel() for p in g["params"]]
             at += sum(-(-p.numel() // BLOCK) for p in g["params"])
         self.nblocks = at
         z = lambda n, dt: torch.zeros(n, dtype=dt, device=self.device)  # noqa: E731
@@ -57,66 +62,62 @@ class AdamW:
         self.m_scale, self.v_scale = (z(at, torch.float32), z(at, torch.float32)) if state_bits == 8 else (None, None)
         self.norm_coef = torch.ones(2, dtype=torch.float64, device=self.device)
 
-    def _arrays(self, params, grads):
+    def _arrays(self, params, sizes, grads):
         """Host arrays of one group: addresses, counts, types (read afresh at every step: tensors may have moved)."""
-        n = len(params)
-        p, g, cnt = (ctypes.c_void_p * n)(), (ctypes.c_void_p * n)(), (ctypes.c_int64 * n)()
-        pt, gt = (ctypes.c_uint8 * n)(), (ctypes.c_uint8 * n)()
-        dev = self.device
+        n, dev, types = len(params), self.device, DTYPES
+        gp, gt = [0] * n, bytearray(n)
         for i, (x, d) in enumerate(zip(params, grads)):
-            p[i], cnt[i], pt[i] = x.data_ptr(), x.numel(), DTYPES[x.dtype]
             if d is None:
                 continue
-            if not (d.dtype in DTYPES and d.shape == x.shape and d.device == dev and d.is_contiguous() and x.is_contiguous()
-                    and x.device == dev):
-                raise ValueError(f"ifd: gradient {i}: contiguous fp32, bf16 or fp16 of shape {tuple(x.shape)} on {dev} "
-                                 f"expected, got {d.dtype} {tuple(d.shape)} on {d.device}")
-            g[i], gt[i] = d.data_ptr(), DTYPES[d.dtype]
-        return p, g, cnt, pt, gt
+            if not (d.dtype in types and d.shape == x.shape and d.is_contiguous() and d.device == dev):
+                refuse(f"gradient {i}: contiguous fp32, bf16 or fp16 of shape {tuple(x.shape)} on {dev} expected, got "
+                       f"{d.dtype} {tuple(d.shape)} on {d.device}")
+            if not (x.is_contiguous() and x.device == dev):
+                refuse(f"parameter {i} is no longer a contiguous tensor on {dev}")
+            gp[i], gt[i] = d.data_ptr(), types[d.dtype]
+        if [x.numel() for x in params] != sizes:
+            refuse("a parameter has changed its size")
+        return ((ctypes.c_void_p * n)(*[x.data_ptr() for x in params]), (ctypes.c_void_p * n)(*gp),
+                (ctypes.c_int64 * n)(*sizes), bytes(types[x.dtype] for x in params), bytes(gt))
 
     def step(self, grads=None):
         """One step; grads in the order of the parameters (None entries: that tensor is left alone)."""
-        if grads is None:
-            grads = [p.grad for p in self.params]
-        grads = list(grads)
+        grads = [p.grad for p in self.params] if grads is None else list(grads)
         need(len(grads) == len(self.params), f"{len(grads)} gradients for {len(self.params)} parameters")
         need(not torch.cuda.is_current_stream_capturing(), "an optimizer step cannot be captured: its step number would stay")
-        L = lib()
+        L, dev = lib(), self.device
         at, arrays = 0, []
         for grp in self.groups:
             k = len(grp["params"])
-            arrays.append(self._arrays(grp["params"], grads[at:at + k]))
+            arrays.append(self._arrays(grp["params"], grp["sizes"], grads[at:at + k]))
             at += k
-        with torch.cuda.device(self.device):
-            s = _lib.stream_ptr(self.device)
-            if self.max_norm is not None:
-                self._norm(L, arrays, s)
-            self.step_count += 1
-            for grp, (p, g, cnt, pt, gt) in zip(self.groups, arrays):
-                vp = ctypes.c_void_p
-                a = AdamwArgs(nt=len(cnt), bits=self.state_bits, step=self.step_count, seed=self.seed, block0=grp["block0"],
-                              lr=grp["lr"], b1=self.betas[0], b2=self.betas[1], eps=self.eps, wd=grp["weight_decay"])
-                a.p, a.g, a.n, a.ptype, a.gtype = (ctypes.cast(x, vp) for x in (p, g, cnt, pt, gt))
-                a.m, a.v = self.m.data_ptr(), self.v.data_ptr()
-                if self.state_bits == 8:
-                    a.m_scale, a.v_scale = self.m_scale.data_ptr(), self.v_scale.data_ptr()
-                a.norm_coef = self.norm_coef.data_ptr() if self.max_norm is not None else None
-                _lib.check(L.ifd_op_adamw(ctypes.byref(a), s))
+        if self.max_norm is not None:
+            self._norm(L, arrays)
+        self.step_count += 1
+        for grp, (p, g, cnt, pt, gt) in zip(self.groups, arrays):
+            a = AdamwArgs(len(cnt), self.state_bits, self.step_count, self.seed)
+            keep = ctypes.create_string_buffer(pt, len(pt)), ctypes.create_string_buffer(gt, len(gt))
+            a.p, a.g, a.n, a.ptype, a.gtype = (ctypes.addressof(x) for x in (p, g, cnt, *keep))
+            a.m, a.v = self.m.data_ptr(), self.v.data_ptr()
+            if self.state_bits == 8:
+                a.m_scale, a.v_scale = self.m_scale.data_ptr(), self.v_scale.data_ptr()
+            a.block0, a.lr, a.b1, a.b2 = grp["block0"], grp["lr"], self.betas[0], self.betas[1]
+            a.eps, a.wd = self.eps, grp["weight_decay"]
+            a.norm_coef = None if self.max_norm is None else self.norm_coef.data_ptr()
+            call(L.ifd_op_adamw, dev, ctypes.byref(a))
 
-    def _norm(self, L, arrays, s):
-        n = sum(len(a[2]) for a in arrays)
+    def _norm(self, L, arrays):
         if len(arrays) == 1:
             _, g, cnt, _, gt = arrays[0]
         else:
-            g, cnt, gt = (ctypes.c_void_p * n)(), (ctypes.c_int64 * n)(), (ctypes.c_uint8 * n)()
-            i = 0
-            for _, ga, ca, _, ta in arrays:
-                for j in range(len(ca)):
-                    g[i], cnt[i], gt[i] = ga[j], ca[j], ta[j]
-                    i += 1
-        nb = L.ifd_op_grad_norm_ws_bytes(n, cnt)
+            n = len(self.params)
+            g = (ctypes.c_void_p * n)(*[x for a in arrays for x in a[1]])
+            cnt = (ctypes.c_int64 * n)(*[x for a in arrays for x in a[2]])
+            gt = b"".join(a[4] for a in arrays)
+        nb = L.ifd_op_grad_norm_ws_bytes(len(cnt), cnt)
         ws = workspace(nb, self.device)
-        _lib.check(L.ifd_op_grad_norm(n, g, cnt, gt, float(self.max_norm), _lib.ptr(self.norm_coef), _lib.ptr(ws), nb, s))
+        call(L.ifd_op_grad_norm, self.device, len(cnt), g, cnt, gt, float(self.max_norm), self.norm_coef.data_ptr(),
+             None if ws is None else ws.data_ptr(), nb)
 
     def moments(self):
         """(m, v): both moments as fp32 [blocks * 256], each tensor from a multiple of 256 on (the states themselves with
@@ -125,10 +126,8 @@ class AdamW:
             return self.m, self.v
         m = torch.empty(self.nblocks * BLOCK, dtype=torch.float32, device=self.device)
         v = torch.empty_like(m)
-        with torch.cuda.device(self.device):
-            _lib.check(lib().ifd_op_state_values(_lib.ptr(self.m), _lib.ptr(self.m_scale), _lib.ptr(self.v),
-                                                 _lib.ptr(self.v_scale), self.nblocks, _lib.ptr(m), _lib.ptr(v),
-                                                 _lib.stream_ptr(self.device)))
+        call(lib().ifd_op_state_values, self.device, self.m.data_ptr(), self.m_scale.data_ptr(), self.v.data_ptr(),
+             self.v_scale.data_ptr(), self.nblocks, m.data_ptr(), v.data_ptr())
         return m, v
 
     def load_moments(self, m, v, m_scale=None, v_scale=None):

@@ -12,13 +12,17 @@ pos: int64 [B, T] or [T]. Statistics and products are fp32, each output is round
 """
 from __future__ import annotations
 
-import ctypes
 import math
+import struct
 
 import torch
 
-from . import _lib
-from ._ops import DTYPES, QkArgs, Strides, lib, need, same_device, workspace
+from ._ops import DTYPES, call, lib, refuse, same_device, workspace
+
+# ifd_qk_args (include/ifd_ops.h; _ops.QkArgs has the same layout)
+_HEAD, _MORE = struct.Struct("9i2fi 8P 14q"), struct.Struct("6P 12q")
+_NO_BWD = bytes(_MORE.size)
+_NO_ST = (0, 0, 0)
 
 
 class Rotary:
@@ -33,12 +37,15 @@ class Rotary:
     """
 
     def __init__(self, rot, base=10000.0, interleaved=False, scaling=None, device="cuda"):
-        need(isinstance(rot, int) and rot > 0 and rot % 2 == 0, f"rotated channels must be even and positive, got {rot}")
-        need(base > 1.0, f"base must be larger than 1, got {base}")
+        if not (isinstance(rot, int) and rot > 0 and rot % 2 == 0):
+            refuse(f"rotated channels must be even and positive, got {rot}")
+        if not base > 1.0:
+            refuse(f"base must be larger than 1, got {base}")
         kind = scaling[0] if scaling else None
-        need(kind in (None, "linear", "base", "bands"), f"unknown scaling {scaling!r}")
-        need(kind is None or (len(scaling) == (3 if kind == "bands" else 2) and scaling[1] >= 1.0),
-             f"scaling {scaling!r}: a factor of at least 1" + (" and a length" if kind == "bands" else ""))
+        if kind not in (None, "linear", "base", "bands"):
+            refuse(f"unknown scaling {scaling!r}")
+        if kind and not (len(scaling) == (3 if kind == "bands" else 2) and scaling[1] >= 1.0):
+            refuse(f"scaling {scaling!r}: a factor of at least 1" + (" and a length" if kind == "bands" else ""))
         self.rot, self.base, self.interleaved, self.scaling, self.mscale = rot, float(base), bool(interleaved), scaling, 1.0
         if kind == "base":
             base = base * scaling[1] ** (rot / max(rot - 2, 1))
@@ -46,7 +53,8 @@ class Rotary:
         if kind == "linear":
             f = f / scaling[1]
         elif kind == "bands":
-            need(scaling[2] > 0, f"scaling {scaling!r}: the length must be positive")
+            if not scaling[2] > 0:
+                refuse(f"scaling {scaling!r}: the length must be positive")
             keep = ((scaling[2] * f / (2 * math.pi) - 1.0) / 31.0).clamp(0, 1)
             f = f * keep + f / scaling[1] * (1 - keep)
             self.mscale = 0.1 * math.log(scaling[1]) + 1.0
@@ -54,48 +62,61 @@ class Rotary:
         self.turns = (f / (2 * math.pi)).to(device)
 
 
-def _st(t):
-    return Strides(*t.stride()[:3])
-
-
 def _rows(t):
-    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+    return t if t.stride(3) == 1 or t.shape[3] == 1 else t.contiguous()
 
 
 def _weight(w, D, name, dev):
-    if w is None:
-        return None
-    need(w.shape == (D,) and w.is_floating_point() and w.device == dev, f"{name} must be a float [{D}] on {dev}")
-    return w.detach().float().contiguous()
+    if not (w.shape == (D,) and w.is_floating_point() and w.device == dev):
+        refuse(f"{name} must be a float [{D}] on {dev}")
+    return w if w.dtype == torch.float32 and w.is_contiguous() else w.detach().float().contiguous()
 
 
-def _args(q, k, wq, wk, pos, rope, eps, norm):
-    need(q.dim() == 4 and (k is None or k.dim() == 4), "q, k must be [batch, tokens, heads, channels]")
-    B, T, Hq, D = q.shape
-    need(q.dtype in DTYPES and (k is None or k.dtype == q.dtype), "q, k must have one type: fp32, bf16 or fp16")
-    need(k is None or (k.shape[0], k.shape[1], k.shape[3]) == (B, T, D), f"k must be [{B}, {T}, heads, {D}]")
-    need(0 < D <= 128 and D % 2 == 0, f"head width {D}: at most 128 and even")
-    need(eps >= 0.0, f"eps must not be negative, got {eps}")
-    need(rope is None or rope.rot <= D, f"{rope and rope.rot} rotated channels of {D}")
-    need(rope is None or pos is not None, "a rotation needs positions")
-    need(norm or (wq is None and wk is None), "weights without the norm")
+def _ptr_st(t):
+    return (0, _NO_ST) if t is None else (t.data_ptr(), t.stride()[:3])
+
+
+def _inputs(q, k, wq, wk, pos, rope, eps, norm):
+    if q.dim() != 4 or (k is not None and k.dim() != 4):
+        refuse("q, k must be [batch, tokens, heads, channels]")
+    B, T, _, D = q.shape
+    if q.dtype not in DTYPES or (k is not None and k.dtype != q.dtype):
+        refuse("q, k must have one type: fp32, bf16 or fp16")
+    if k is not None and (k.shape[0] != B or k.shape[1] != T or k.shape[3] != D):
+        refuse(f"k must be [{B}, {T}, heads, {D}], got {tuple(k.shape)}")
+    if not 0 < D <= 128 or D & 1:
+        refuse(f"head width {D}: at most 128 and even")
+    if not eps >= 0.0:
+        refuse(f"eps must not be negative, got {eps}")
+    if rope is not None and (rope.rot > D or pos is None):
+        refuse("a rotation needs positions" if pos is None else f"{rope.rot} rotated channels of {D}")
+    if not norm and not (wq is None and wk is None):
+        refuse("weights without the norm")
     dev = same_device(q, k)
-    a = QkArgs(dtype=DTYPES[q.dtype], B=B, T=T, Hq=Hq, Hk=0 if k is None else k.shape[2], D=D, norm=int(bool(norm)), eps=eps,
-               mscale=1.0)
-    keep = [_rows(q), None if k is None else _rows(k), _weight(wq, D, "wq", dev), _weight(wk, D, "wk", dev)]
-    for n, t in zip(("q", "k"), keep):
-        if t is not None:
-            setattr(a, n, t.data_ptr())
-            setattr(a, n + "_s", _st(t))
-    a.wq, a.wk = (None if t is None else t.data_ptr() for t in keep[2:4])
+    if wq is not None:
+        wq = _weight(wq, D, "wq", dev)
+    if wk is not None:
+        wk = _weight(wk, D, "wk", dev)
     if rope is not None:
-        need(pos.dtype == torch.int64 and pos.shape in ((B, T), (T,)), f"pos must be int64 [{B}, {T}] or [{T}]")
-        need(pos.device == dev and rope.turns.device == dev, f"pos and the rotation's frequencies must be on {dev}")
-        a.rot, a.interleaved, a.mscale = rope.rot, int(rope.interleaved), rope.mscale
-        a.pos, a.turns = pos.data_ptr(), rope.turns.data_ptr()
-        a.pos_s = (ctypes.c_int64 * 2)(*((0,) + pos.stride() if pos.dim() == 1 else pos.stride()))
-        keep += [pos, rope.turns]
-    return a, keep, dev
+        if pos.dtype != torch.int64 or pos.shape not in ((B, T), (T,)):
+            refuse(f"pos must be int64 [{B}, {T}] or [{T}]")
+        if pos.device != dev or rope.turns.device != dev:
+            refuse(f"pos and the rotation's frequencies must be on {dev}")
+    return _rows(q), None if k is None else _rows(k), wq, wk, dev
+
+
+def _pack(q, k, wq, wk, pos, rope, eps, norm, q_out, k_out):
+    B, T, Hq, D = q.shape
+    kp, ks = _ptr_st(k)
+    qo, qos = _ptr_st(q_out)
+    ko, kos = _ptr_st(k_out)
+    rot, il, ms, pp, tp, ps = 0, 0, 1.0, 0, 0, (0, 0)
+    if rope is not None:
+        rot, il, ms, pp, tp = rope.rot, rope.interleaved, rope.mscale, pos.data_ptr(), rope.turns.data_ptr()
+        ps = pos.stride() if pos.dim() == 2 else (0, pos.stride(0))
+    return _HEAD.pack(DTYPES[q.dtype], B, T, Hq, 0 if k is None else k.shape[2], D, rot, il, 1 if norm else 0, eps, ms, 0,
+                      q.data_ptr(), kp, qo, ko, 0 if wq is None else wq.data_ptr(), 0 if wk is None else wk.data_ptr(), pp, tp,
+                      *q.stride()[:3], *ks, *qos, *kos, *ps)
 
 
 def _into(t, like, name):
@@ -103,45 +124,40 @@ def _into(t, like, name):
         return None
     if t is None:
         return torch.empty(like.shape, dtype=like.dtype, device=like.device)
-    need(t.shape == like.shape and t.dtype == like.dtype and t.device == like.device and (t.stride(-1) == 1 or
-         t.shape[-1] == 1), f"{name} must be like its input, with adjacent channels")
+    if not (t.shape == like.shape and t.dtype == like.dtype and t.device == like.device
+            and (t.stride(3) == 1 or t.shape[3] == 1)):
+        refuse(f"{name} must be like its input, with adjacent channels")
     return t
 
 
 def qk_norm_rope(q, k, wq=None, wk=None, pos=None, rope=None, eps=1e-6, norm=True, q_out=None, k_out=None):
     """(q_out, k_out); q_out=q and k_out=k work in place. k=None: (q_out, None)."""
-    a, keep, dev = _args(q, k, wq, wk, pos, rope, eps, norm)
+    q, k, wq, wk, dev = _inputs(q, k, wq, wk, pos, rope, eps, norm)
     q_out, k_out = _into(q_out, q, "q_out"), _into(k_out, k, "k_out")
-    for n, t in (("q_out", q_out), ("k_out", k_out)):
-        if t is not None:
-            setattr(a, n, t.data_ptr())
-            setattr(a, n + "_s", _st(t))
-    with torch.cuda.device(dev):
-        _lib.check(lib().ifd_op_qk_norm_rope(ctypes.byref(a), _lib.stream_ptr(dev)))
+    call(lib().ifd_op_qk_norm_rope, dev, _pack(q, k, wq, wk, pos, rope, eps, norm, q_out, k_out) + _NO_BWD)
     return q_out, k_out
 
 
 def qk_norm_rope_bwd(gq, gk, q, k, wq=None, wk=None, pos=None, rope=None, eps=1e-6, norm=True, dq=None, dk=None):
     """(dq, dk, dwq, dwk) from the gradients of the outputs; q, k are the forward's inputs. dwq, dwk are fp32 sums over
     tokens and heads (None without weights); dq=gq and dk=gk work in place."""
-    a, keep, dev = _args(q, k, wq, wk, pos, rope, eps, norm)
-    need((gk is None) == (k is None), "gk without k")
-    for n, t, like in (("gq", gq, q), ("gk", gk, k)):
-        if t is not None:
-            need(t.shape == like.shape and t.dtype == like.dtype, f"{n} must be like {n[1]}")
+    q, k, wq, wk, dev = _inputs(q, k, wq, wk, pos, rope, eps, norm)
+    if (gk is None) != (k is None):
+        refuse("gk without k")
+    if gq.shape != q.shape or gq.dtype != q.dtype or (k is not None and (gk.shape != k.shape or gk.dtype != k.dtype)):
+        refuse("gq, gk must be like q, k")
     same_device(q, gq, gk)
     gq, gk = _rows(gq), None if gk is None else _rows(gk)
     dq, dk = _into(dq, q, "dq"), _into(dk, k, "dk")
     dwq = None if wq is None else torch.empty(q.shape[3], dtype=torch.float32, device=dev)
     dwk = None if wk is None else torch.empty(q.shape[3], dtype=torch.float32, device=dev)
-    for n, t in (("gq", gq), ("gk", gk), ("dq", dq), ("dk", dk)):
-        if t is not None:
-            setattr(a, n, t.data_ptr())
-            setattr(a, n + "_s", _st(t))
-    a.dwq, a.dwk = (None if t is None else t.data_ptr() for t in (dwq, dwk))
+    gkp, gks = _ptr_st(gk)
+    dkp, dks = _ptr_st(dk)
+    a = _pack(q, k, wq, wk, pos, rope, eps, norm, None, None) + _MORE.pack(
+        gq.data_ptr(), gkp, dq.data_ptr(), dkp, 0 if dwq is None else dwq.data_ptr(), 0 if dwk is None else dwk.data_ptr(),
+        *gq.stride()[:3], *gks, *dq.stride()[:3], *dks)
     L = lib()
-    with torch.cuda.device(dev):
-        n = L.ifd_op_qk_norm_rope_bwd_ws_bytes(ctypes.byref(a))
-        ws = workspace(n, dev)
-        _lib.check(L.ifd_op_qk_norm_rope_bwd(ctypes.byref(a), _lib.ptr(ws), n, _lib.stream_ptr(dev)))
+    n = L.ifd_op_qk_norm_rope_bwd_ws_bytes(a)
+    ws = workspace(n, dev)
+    call(L.ifd_op_qk_norm_rope_bwd, dev, a, None if ws is None else ws.data_ptr(), n)
     return dq, dk, dwq, dwk

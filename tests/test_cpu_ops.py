@@ -20,6 +20,14 @@ def test_library_exports_ops_header_symbols():
     assert set(syms) == set(_ops.OPS_EXPORTS)
 
 
+def test_packed_arguments_have_the_structures_layout():
+    from ifd import _ops, attention, rotary
+    assert ctypes.sizeof(_ops.AttentionArgs) == attention._FWD.size + attention._BWD.size
+    assert _ops.AttentionArgs.dout.offset == attention._FWD.size
+    assert ctypes.sizeof(_ops.QkArgs) == rotary._HEAD.size + rotary._MORE.size
+    assert _ops.QkArgs.gq.offset == rotary._HEAD.size
+
+
 def _attention_args(**kw):
     """Valid arguments with made-up addresses: only the checks run."""
     from ifd._ops import AttentionArgs, Strides
