@@ -47,9 +47,10 @@ __global__ __launch_bounds__(256) void qk_rope_kernel(QkK p) {
   for (int x = 0; x < 2; ++x) {
     const float* wp = x ? p.wk : p.wq;
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      w[x][j] = wp ? wp[ia + j] : 1.f;
-      w[x][V + j] = wp ? wp[ib + j] : 1.f;
+    for (int j = 0; j < 2 * V; ++j) w[x][j] = 1.f;
+    if (wp) {  // (4-byte aligned: vector loads all the same)
+      __builtin_memcpy(&w[x][0], wp + ia, 4 * V);
+      __builtin_memcpy(&w[x][V], wp + ib, 4 * V);
     }
   }
 #pragma unroll
@@ -230,8 +231,8 @@ static const char* qk_check(const ifd_qk_args& a) {
   return nullptr;
 }
 
-constexpr int QK_FWD_WGS = 2048;  // eight per CU
-constexpr int QK_WGS = 1024;  // workgroups of the backward pass (each leaves one partial row of weight gradients)
+constexpr int QK_FWD_WGS = 1024;
+constexpr int QK_WGS = 512;  // workgroups of the backward pass (each leaves one partial row of weight gradients)
 
 static bool vec_ok(int V, int es, const ifd_qk_args& a, bool bwd) {
   if ((a.rot / 2) % V || ((a.D - a.rot) / 2) % V) return false;
