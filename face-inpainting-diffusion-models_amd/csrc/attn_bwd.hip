@@ -8,8 +8,8 @@
 
 namespace ifd {
 
-template <typename T, int DP, int NW, int BK>
-__global__ __launch_bounds__(NW * 64) void attn_bwd_q_kernel(AttnK p) {
+template <typename T, int DP, int NW, int BK, int AHEAD, int OCC>
+__global__ __launch_bounds__(NW * 64, OCC) void attn_bwd_q_kernel(AttnK p) {
   typedef AttnTile<T, DP> TL;
   typedef typename TL::frag frag;
   constexpr int KT = BK / 32, TB = BK * TL::ROWB;
@@ -102,9 +102,19 @@ __global__ __launch_bounds__(NW * 64) void attn_bwd_q_kernel(AttnK p) {
 #pragma unroll
         for (int x = 0; x < 16; ++x) s[x] = dp[x] = 0.f;
 #pragma unroll
-        for (int ks = 0; ks < TL::KS; ++ks) {
-          s = TL::A::mma(TL::row(kb, kt * 32, ks, l32, h), qf[ks], s);
-          dp = TL::A::mma(TL::row(vb, kt * 32, ks, l32, h), gf[ks], dp);
+        for (int k1 = 0; k1 < TL::KS; k1 += AHEAD) {  // operands are read ahead of the products that take them
+          frag ka[AHEAD], va[AHEAD];
+#pragma unroll
+          for (int x = 0; x < AHEAD; ++x) {
+            ka[x] = TL::row(kb, kt * 32, k1 + x, l32, h);
+            va[x] = TL::row(vb, kt * 32, k1 + x, l32, h);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int x = 0; x < AHEAD; ++x) {
+            s = TL::A::mma(ka[x], qf[k1 + x], s);
+            dp = TL::A::mma(va[x], gf[k1 + x], dp);
+          }
         }
         if (mask) {
 #pragma unroll
@@ -141,8 +151,8 @@ __global__ __launch_bounds__(NW * 64) void attn_bwd_q_kernel(AttnK p) {
 
 // A workgroup owns NW * 32 keys of one key-value head and walks over the (query head, row tile) pairs of its share:
 // with nsplit > 1 the pairs are dealt to nsplit workgroups, whose fp32 sums attn_bwd_join_kernel adds in order.
-template <typename T, int DP, int NW, int BQ>
-__global__ __launch_bounds__(NW * 64) void attn_bwd_kv_kernel(AttnK p) {
+template <typename T, int DP, int NW, int BQ, bool VL, int OCC>
+__global__ __launch_bounds__(NW * 64, OCC) void attn_bwd_kv_kernel(AttnK p) {
   typedef AttnTile<T, DP> TL;
   typedef typename TL::frag frag;
   constexpr int QT = BQ / 32, TB = BQ * TL::ROWB, BUF = 2 * TB + 1024;  // Q, dout, lse2[BQ], delta[BQ]
@@ -167,14 +177,15 @@ __global__ __launch_bounds__(NW * 64) void attn_bwd_kv_kernel(AttnK p) {
   const int w_lo = __builtin_amdgcn_readfirstlane(first_row(kb0 + w * 32));
   const int w_hi = __builtin_amdgcn_readfirstlane(first_row(kb0 + w * 32 + 31));
 
-  frag kf[TL::KS], vf[TL::KS];
+  frag kf[TL::KS], vf[VL ? 1 : TL::KS];
+  const lds_c* vt = sm + 2 * BUF;  // VL: the workgroup's V rows stay in LDS, for want of registers
   {
     const char* rk = p.k + b * p.kb + hk * p.kh + (int64_t)key * p.kt;
     const char* rv = p.v + b * p.vb + hk * p.vh + (int64_t)key * p.vt;
 #pragma unroll
     for (int ks = 0; ks < TL::KS; ++ks) {
       kf[ks] = TL::gload(rk, ok, ks, h, p.D);
-      vf[ks] = TL::gload(rv, ok, ks, h, p.D);
+      if (!VL) vf[VL ? 0 : ks] = TL::gload(rv, ok, ks, h, p.D);
     }
   }
   f32x16 dk[TL::DT], dv[TL::DT];
@@ -199,8 +210,22 @@ __global__ __launch_bounds__(NW * 64) void attn_bwd_kv_kernel(AttnK p) {
     }
   };
   if (it0 < it1) {
+    if (VL) {
+      AttnStage<T, DP, NW * 32, NW> sv;
+      sv.init(w, lane, p.D);
+      sv.load(p.v + b * p.vb + hk * p.vh + (int64_t)kb0 * p.vt, p.vt, min(NW * 32, len - kb0), sm + 2 * BUF, w);
+    }
     stage(it0, 0);
     dma_wait();
+    if (VL && p.D < DP) {
+      // both factors of dp come from LDS here: V's channels past D must be zeros
+      __syncthreads();
+      const int c0 = p.D / TL::CE, nz = TL::NCH - c0;
+      for (int x = tid; x < NW * 32 * nz; x += NW * 64) {
+        const int r = x / nz, c = c0 + x - r * nz;
+        lds_zero(sm + 2 * BUF + r * TL::ROWB + ((c ^ TL::swz(r)) << 4));
+      }
+    }
     __syncthreads();
   }
   int buf = 0;
@@ -219,7 +244,7 @@ __global__ __launch_bounds__(NW * 64) void attn_bwd_kv_kernel(AttnK p) {
 #pragma unroll
       for (int ks = 0; ks < TL::KS; ++ks) {
         s = TL::A::mma(TL::row(qb, qt * 32, ks, l32, h), kf[ks], s);
-        dp = TL::A::mma(TL::row(gb, qt * 32, ks, l32, h), vf[ks], dp);
+        dp = TL::A::mma(TL::row(gb, qt * 32, ks, l32, h), VL ? TL::row(vt, w * 32, ks, l32, h) : vf[VL ? 0 : ks], dp);
       }
       const bool mask = rr < w_hi || rr + 32 > p.Tq;
 #pragma unroll
@@ -323,11 +348,13 @@ static int kv_split(const ifd_attention_args& a) {
 template <typename T, int DP>
 static int run_bwd(AttnK p, int nsplit, hipStream_t s) {
   constexpr int ROWB = DP * (int)sizeof(T);
-  constexpr int BK = ROWB >= 512 ? 32 : 64;
+  constexpr int BK = ROWB >= 512 ? 32 : 64, OCC = ROWB >= 512 ? 1 : 2, AHQ = 4, OCCK = OCC;
+  constexpr bool VL = sizeof(T) == 2 && DP == 128;
+  constexpr int NWK = 4, BQ = VL ? 32 : BK;
   {
     constexpr int lds = 4 * BK * ROWB;
     static bool attr[kMaxDevices] = {};
-    auto kern = attn_bwd_q_kernel<T, DP, 4, BK>;
+    auto kern = attn_bwd_q_kernel<T, DP, 4, BK, AHQ, OCC>;
     if (set_lds_attr_once(attr, reinterpret_cast<const void*>(kern), lds) != hipSuccess) return IFD_LAUNCH_STATUS();
     p.nblk = (int)cdiv(p.Tq, 128);
     if (p.Tq) {
@@ -336,13 +363,13 @@ static int run_bwd(AttnK p, int nsplit, hipStream_t s) {
     }
   }
   if (!p.Tk) return 0;
-  constexpr int lds = 2 * (2 * BK * ROWB + 1024);
+  constexpr int lds = 2 * (2 * BQ * ROWB + 1024) + (VL ? NWK * 32 * ROWB : 0);
   static bool attr[kMaxDevices] = {};
-  auto kern = attn_bwd_kv_kernel<T, DP, 4, BK>;
+  auto kern = attn_bwd_kv_kernel<T, DP, NWK, BQ, VL, OCCK>;
   if (set_lds_attr_once(attr, reinterpret_cast<const void*>(kern), lds) != hipSuccess) return IFD_LAUNCH_STATUS();
-  p.nblk = (int)cdiv(p.Tk, 128);
+  p.nblk = (int)cdiv(p.Tk, 32 * NWK);
   p.nsplit = nsplit;
-  hipLaunchKernelGGL(kern, dim3(p.nblk * p.B * p.Hk * nsplit), dim3(256), lds, s, p);
+  hipLaunchKernelGGL(kern, dim3(p.nblk * p.B * p.Hk * nsplit), dim3(64 * NWK), lds, s, p);
   if (int e = IFD_LAUNCH_STATUS()) return e;
   if (nsplit > 1) {
     auto join = attn_bwd_join_kernel<T, DP>;

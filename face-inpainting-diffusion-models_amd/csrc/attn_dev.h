@@ -10,8 +10,12 @@
 // hands each lane four rows of one column; fp32: four ds_read_b32).
 //
 // LDS tiles are row-major [rows][DP], filled by LDS-DMA (no registers between), 16-byte chunk c of row r at position
-// c ^ swz(r): eight consecutive rows of one chunk (row reads) and two chunks of four consecutive rows (transposed
-// reads) both fall into different banks.
+// c ^ swz(r). LDS serves 256 bytes a cycle: 16 rows of one chunk (row reads), four chunks of four consecutive rows
+// (transposed reads) and, in fp32, eight chunks of two rows four apart must cover the 64 banks once. Measured: 4.0 cycles
+// a row read and 2.3 a transposed read of a wave, twice that where two rows meet in a bank. The 128-byte rows (16-bit,
+// DP = 64) take an order that repeats every 8 rows although its row reads meet in pairs (8 cycles): the transposed reads
+// then differ by constants alone, which saves the registers that decide how many waves fit (forward, 4096 tokens x 32
+// heads, causal: 95 us against 102 with the order that never meets).
 #pragma once
 #include "ops.h"
 
@@ -72,7 +76,8 @@ struct AttnTile {
   static constexpr int KS = NCH / 2, DT = DP / 32, PS = A::PS;
 
   static __device__ __forceinline__ int swz(int r) {
-    return NCH == 8 ? ((r & 3) << 1) | ((r >> 2) & 1) : ((r & 7) << 1) | ((r >> 3) & 1);
+    if (ES == 4) return ((r & 7) << 1) | ((r >> 3) & 1);
+    return NCH == 8 ? ((r & 3) << 1) | ((r >> 2) & 1) : ((r & 3) << 2) | ((r >> 2) & 3);
   }
 
   // rows [r0, r0 + 32) as A operands of k-step ks (row l32, chunk 2 ks + h)
@@ -158,13 +163,14 @@ struct AttnStage {
   static constexpr int RPI = 1024 / TL::ROWB;            // rows per DMA instruction (64 lanes x 16 bytes)
   static constexpr int NI = ROWS / RPI / NW;             // instructions per wave
   static_assert(ROWS % (RPI * NW) == 0, "tile rows divide over the waves");
-  int row[NI], cb[NI];
+  static constexpr int ROWS_STEP = RPI * NW, NCB = ROWS_STEP >= 16 ? 1 : 16 / ROWS_STEP;  // swz repeats every 16 rows
+  int row, cb[NCB];  // of instruction 0; of instruction i: row + i ROWS_STEP, cb[i % NCB]
 
   __device__ __forceinline__ void init(int w, int lane, int D) {
+    row = w * RPI + lane / TL::NCH;
 #pragma unroll
-    for (int i = 0; i < NI; ++i) {
-      row[i] = (w + NW * i) * RPI + lane / TL::NCH;
-      const int c = (lane % TL::NCH) ^ TL::swz(row[i]);
+    for (int i = 0; i < NCB; ++i) {
+      const int c = (lane % TL::NCH) ^ TL::swz(row + i * ROWS_STEP);
       cb[i] = c * TL::CE < D ? c * 16 : 0;
     }
   }
@@ -172,12 +178,13 @@ struct AttnStage {
   __device__ __forceinline__ void load(const char* base, int stride, int nrows, lds_c* tile, int w) const {
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
-      const int r = row[i] < nrows ? row[i] : nrows - 1;
-      dma_quad(base, r * stride + cb[i], tile + (w + NW * i) * 1024);
+      const int r = min(row + i * ROWS_STEP, nrows - 1);
+      dma_quad(base, r * stride + cb[i % NCB], tile + (w + NW * i) * 1024);
     }
   }
 };
 
+__device__ __forceinline__ void lds_zero(lds_c* q) { *(__attribute__((address_space(3))) u32x4*)q = u32x4{0, 0, 0, 0}; }
 __device__ __forceinline__ f32x4 lds_quad(const lds_c* q) { return *(const __attribute__((address_space(3))) f32x4*)q; }
 
 __device__ __forceinline__ void dma_wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }

@@ -5,9 +5,11 @@
 namespace ifd {
 
 // The running softmax of 32 query rows (column l32 of the score tile) and their output accumulators.
-// Scores are kept in units of log2: p = 2^(c s - m). The reference point m moves only when a row's maximum passes it by
-// more than 2^SLACK, so most tiles skip the rescaling of O; p <= 2^SLACK then, exact in fp32 and inside fp16's range.
-constexpr float ATTN_SLACK = 8.f;
+// Scores are kept in units of log2: p = 2^(c s - m). The reference point m need not be the maximum: a tile's p are first
+// taken with the m there is, and only when a lane's sum of them passes LIMIT (or is not a number: the first tile, whose m
+// is -inf) are the tile's maxima found, m moved there and O rescaled. The usual tile so needs no maximum, no exchange
+// between lanes and no rescaling; p <= LIMIT is exact in fp32 and inside fp16's range.
+constexpr float ATTN_LIMIT = 4096.f;
 
 template <typename T, int DP, int KT>
 struct AttnRows {
@@ -24,8 +26,23 @@ struct AttnRows {
     m = -INFINITY;
     l = 0.f;
   }
-  // scores -> probabilities in place. lim: keys [0, lim) of this tile are seen by the row (mask != 0)
-  __device__ __forceinline__ void soft(f32x16 (&s)[KT], float c, bool mask, int lim, int h) {
+  static __device__ __forceinline__ float probs(const f32x16 (&s)[KT], float c, float ms, frag (&pf)[KT][TL::PS]) {
+    float sum[2] = {0.f, 0.f};
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt) {
+      f32x16 e;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        e[i] = __builtin_amdgcn_exp2f(fmaf(s[kt][i], c, -ms));
+        sum[i & 1] += e[i];
+      }
+#pragma unroll
+      for (int ps = 0; ps < TL::PS; ++ps) pf[kt][ps] = TL::pack(e, ps);
+    }
+    return sum[0] + sum[1];
+  }
+  // scores -> probabilities as operands. lim: keys [0, lim) of this tile are seen by the row (mask != 0)
+  __device__ __forceinline__ void soft(f32x16 (&s)[KT], float c, bool mask, int lim, int h, frag (&pf)[KT][TL::PS]) {
     if (mask) {
 #pragma unroll
       for (int kt = 0; kt < KT; ++kt)
@@ -33,13 +50,14 @@ struct AttnRows {
         for (int i = 0; i < 16; ++i)
           if (kt * 32 + 8 * (i >> 2) + 4 * h + (i & 3) >= lim) s[kt][i] = -INFINITY;
     }
-    float mx = s[0][0];
+    float sum = probs(s, c, m, pf);
+    if (__any(!(sum < ATTN_LIMIT))) {
+      float mx = s[0][0];
 #pragma unroll
-    for (int kt = 0; kt < KT; ++kt)
+      for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
-      for (int i = kt ? 0 : 1; i < 16; ++i) mx = fmaxf(mx, s[kt][i]);
-    mx = fmaxf(mx, xhalf(mx)) * c;
-    if (__any(mx > m + ATTN_SLACK || (m == -INFINITY && mx > m))) {
+        for (int i = kt ? 0 : 1; i < 16; ++i) mx = fmaxf(mx, s[kt][i]);
+      mx = fmaxf(mx, xhalf(mx)) * c;
       const float mn = fmaxf(m, mx);
       const float a = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
       m = mn;
@@ -48,16 +66,8 @@ struct AttnRows {
       for (int d = 0; d < TL::DT; ++d)
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[d][i] *= a;
+      sum = probs(s, c, m == -INFINITY ? 0.f : m, pf);  // no key seen yet: every p is 2^-inf = 0
     }
-    const float ms = m == -INFINITY ? 0.f : m;  // no key seen yet: every p is 2^-inf = 0
-    float sum = 0.f;
-#pragma unroll
-    for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        s[kt][i] = __builtin_amdgcn_exp2f(fmaf(s[kt][i], c, -ms));
-        sum += s[kt][i];
-      }
     l += sum;
   }
 };
@@ -65,11 +75,11 @@ struct AttnRows {
 // Many rows. A workgroup of NW waves takes NW * NQ * 32 rows of one (sequence, head); the waves share the K and V tiles
 // (BK keys, two buffers, the next tile's DMA in flight during this one's products). Per wave and tile: S^T = K Q^T with
 // Q in registers, softmax down the registers of each lane (a lane holds one row's scores of half the keys), O^T += V^T P^T.
-template <typename T, int DP, int NQ, int NW, int BK>
-__global__ __launch_bounds__(NW * 64) void attn_fwd_kernel(AttnK p) {
+template <typename T, int DP, int NQ, int NW, int BK, int SUB, int OCC>
+__global__ __launch_bounds__(NW * 64, OCC) void attn_fwd_kernel(AttnK p) {
   typedef AttnTile<T, DP> TL;
   typedef typename TL::frag frag;
-  constexpr int KT = BK / 32, TB = BK * TL::ROWB;
+  constexpr int KT = SUB / 32, TB = BK * TL::ROWB;
   extern __shared__ __attribute__((aligned(1024))) char smem[];
   lds_c* sm = (lds_c*)smem;
   const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, h = lane >> 5;
@@ -129,41 +139,47 @@ __global__ __launch_bounds__(NW * 64) void attn_fwd_kernel(AttnK p) {
   }
   for (int t = 0; t < nt; ++t) {
     if (t + 1 < nt) stage(t + 1);
-    const lds_c* kb = sm + (t & 1) * (2 * TB);
-    const lds_c* vb = kb + TB;
-    const int k0 = t * BK;
-    if (k0 < w_end) {
+#pragma unroll 1
+    for (int sub = 0; sub < BK / SUB; ++sub) {
+      const int k0 = t * BK + sub * SUB;
+      if (k0 >= w_end) break;
+      const lds_c* kb = sm + (t & 1) * (2 * TB) + sub * (SUB * TL::ROWB);
+      const lds_c* vb = kb + TB;
       f32x16 s[NQ][KT];
+      // KB operands are read ahead of the products that take them
+      constexpr int KB = TL::ROWB == 128 ? 4 : 8;
 #pragma unroll
-      for (int kt = 0; kt < KT; ++kt) {
+      for (int n = 0; n < NQ; ++n)
 #pragma unroll
-        for (int n = 0; n < NQ; ++n)
+        for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
           for (int i = 0; i < 16; ++i) s[n][kt][i] = 0.f;
 #pragma unroll
-        for (int ks = 0; ks < TL::KS; ++ks) {
-          const frag a = TL::row(kb, kt * 32, ks, l32, h);
+      for (int x0 = 0; x0 < KT * TL::KS; x0 += KB) {
+        frag a[KB];
 #pragma unroll
-          for (int n = 0; n < NQ; ++n) s[n][kt] = TL::A::mma(a, qf[n][ks], s[n][kt]);
-        }
+        for (int x = 0; x < KB; ++x) a[x] = TL::row(kb, (x0 + x) / TL::KS * 32, (x0 + x) % TL::KS, l32, h);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int x = 0; x < KB; ++x)
+#pragma unroll
+          for (int n = 0; n < NQ; ++n)
+            s[n][(x0 + x) / TL::KS] = TL::A::mma(a[x], qf[n][(x0 + x) % TL::KS], s[n][(x0 + x) / TL::KS]);
       }
-      const bool mask = k0 + BK > w_all;
+      const bool mask = k0 + SUB > w_all;
+      frag pf[NQ][KT][TL::PS];
 #pragma unroll
-      for (int n = 0; n < NQ; ++n) st[n].soft(s[n], p.c, mask, lim[n] - k0, h);
+      for (int n = 0; n < NQ; ++n) st[n].soft(s[n], p.c, mask, lim[n] - k0, h, pf[n]);
 #pragma unroll
       for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
-        for (int ps = 0; ps < TL::PS; ++ps) {
-          frag pf[NQ];
-#pragma unroll
-          for (int n = 0; n < NQ; ++n) pf[n] = TL::pack(s[n][kt], ps);
+        for (int ps = 0; ps < TL::PS; ++ps)
 #pragma unroll
           for (int d = 0; d < TL::DT; ++d) {
             const frag a = TL::col(vb, kt * 32, ps, d, lane);
 #pragma unroll
-            for (int n = 0; n < NQ; ++n) st[n].o[d] = TL::A::mma(a, pf[n], st[n].o[d]);
+            for (int n = 0; n < NQ; ++n) st[n].o[d] = TL::A::mma(a, pf[n][kt][ps], st[n].o[d]);
           }
-        }
     }
     dma_wait();
     __syncthreads();
@@ -264,15 +280,14 @@ __global__ __launch_bounds__(NW * 64) void attn_split_kernel(AttnK p) {
 #pragma unroll
       for (int ks = 0; ks < TL::KS; ++ks) s[kt] = TL::A::mma(TL::row(kb, kt * 32, ks, l32, h), qf[ks], s[kt]);
     }
-    st.soft(s, p.c, k0 + BK > all, lim - k0, h);
+    frag pf[KT][TL::PS];
+    st.soft(s, p.c, k0 + BK > all, lim - k0, h, pf);
 #pragma unroll
     for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
-      for (int ps = 0; ps < TL::PS; ++ps) {
-        const frag pf = TL::pack(s[kt], ps);
+      for (int ps = 0; ps < TL::PS; ++ps)
 #pragma unroll
-        for (int d = 0; d < TL::DT; ++d) st.o[d] = TL::A::mma(TL::col(vb, kt * 32, ps, d, lane), pf, st.o[d]);
-      }
+        for (int d = 0; d < TL::DT; ++d) st.o[d] = TL::A::mma(TL::col(vb, kt * 32, ps, d, lane), pf[kt][ps], st.o[d]);
     // the reads above are complete before the next round's DMA overwrites this buffer
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     buf ^= 1;
@@ -442,12 +457,12 @@ static int run_fwd(const FwdPlan& pl, AttnK p, hipStream_t s) {
   p.nblk = pl.nblk;
   p.nsplit = pl.nsplit;
   if (!pl.split) {
-    constexpr int BK = ROWB >= 512 ? 32 : 64;
+    constexpr int BK = ROWB >= 512 ? 32 : 64, SUB = ROWB >= 512 ? 32 : 64, NW = 4, OCC = ROWB == 128 ? 4 : ROWB == 256 ? 2 : 1;
     constexpr int lds = 4 * BK * ROWB;
     static bool attr[kMaxDevices] = {};
-    auto kern = attn_fwd_kernel<T, DP, 1, 4, BK>;
+    auto kern = attn_fwd_kernel<T, DP, 1, NW, BK, SUB, OCC>;
     if (set_lds_attr_once(attr, reinterpret_cast<const void*>(kern), lds) != hipSuccess) return IFD_LAUNCH_STATUS();
-    hipLaunchKernelGGL(kern, dim3(p.nblk * p.B * p.Hq), dim3(256), lds, s, p);
+    hipLaunchKernelGGL(kern, dim3(p.nblk * p.B * p.Hq), dim3(NW * 64), lds, s, p);
     return IFD_LAUNCH_STATUS();
   }
   constexpr int BK = ROWB == 128 ? 64 : 32, NW = ROWB >= 512 ? 2 : 4;
