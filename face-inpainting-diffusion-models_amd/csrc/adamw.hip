@@ -2,7 +2,7 @@
 //   g' = c g; m = b1 m + (1 - b1) g'; v = b2 v + (1 - b2) g'^2;
 //   p = p (1 - lr wd) - lr / (1 - b1^k) m / (sqrt(v) / sqrt(1 - b2^k) + eps)
 // Bound by memory: 16 bytes a value with fp32 tensors and 8-bit states, 28 with 32-bit states, plus the norm's own pass
-// over the gradients. The tensors' addresses travel in the kernel arguments (96 tensors a launch): no table to upload,
+// over the gradients. The tensors' addresses travel in the kernel arguments (128 tensors a launch): no table to upload,
 // nothing kept between steps. A wave owns blocks of 256 values, four per lane; an 8-bit state's scale is its block's.
 //
 // 8-bit states. One byte is a small float, with one fp32 scale per block of 256 (largest magnitude / 1.875):
@@ -21,16 +21,17 @@ namespace ifd {
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 hf16x4 __attribute__((ext_vector_type(4)));
 
-constexpr int AW_T = 96;      // tensors of a launch
+constexpr int AW_T = 128;     // tensors of a launch (its tables fill the 4 KB of kernel arguments)
+constexpr int64_t AW_MAX = (int64_t)1 << 31;  // values of a table entry: a longer tensor takes several
 constexpr int AW_CHUNK = 16;  // blocks of a workgroup
 
 struct AwTab {
   const void* p[AW_T];
   const void* g[AW_T];
-  int64_t n[AW_T];
+  unsigned n[AW_T];
   int chunk0[AW_T];     // first workgroup of the tensor
   int block0[AW_T];     // first state block, relative to AwArgs::block0
-  uint8_t pt[AW_T], gt[AW_T];
+  uint8_t types[AW_T];  // parameter's | gradient's << 4
   int count;
 };
 struct AwArgs {
@@ -152,7 +153,7 @@ __global__ __launch_bounds__(256) void adamw_multi_kernel(const AwTab t, const A
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int ti = aw_find(t, blockIdx.x);
   const int64_t n = t.n[ti];
-  const int pt = t.pt[ti], gt = t.gt[ti];
+  const int pt = t.types[ti] & 15, gt = t.types[ti] >> 4;
   void* pp = const_cast<void*>(t.p[ti]);
   const void* gp = t.g[ti];
   double coef = 1.0;
@@ -235,11 +236,18 @@ __global__ __launch_bounds__(256) void grad_sq_kernel(const AwTab t, double* __r
   const int64_t n = t.n[ti];
   const int nblk = (int)((n + 255) >> 8);
   const int b0 = (blockIdx.x - t.chunk0[ti]) * AW_CHUNK;
+  const void* gp = t.g[ti];
+  const int gt = t.types[ti] >> 4, b1 = min(nblk, b0 + AW_CHUNK);
   double s = 0.0;
-  for (int bi = b0 + wave; bi < min(nblk, b0 + AW_CHUNK); bi += 4) {
-    const f32x4 g = aw_load(t.g[ti], t.gt[ti], (int64_t)bi * 256 + lane * 4, n);
+  for (int bi = b0 + wave; bi < b1; bi += 16) {
+    f32x4 g[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) s += (double)g[j] * (double)g[j];
+    for (int u = 0; u < 4; ++u)  // (a block past the chunk: nothing is read)
+      g[u] = aw_load(gp, gt, (int64_t)(bi + 4 * u) * 256 + lane * 4, bi + 4 * u < b1 ? n : 0);
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s += (double)g[u][j] * (double)g[u][j];
   }
 #pragma unroll
   for (int o = 32; o; o >>= 1) s += __shfl_xor(s, o);
@@ -251,6 +259,7 @@ __global__ __launch_bounds__(1024) void grad_norm_kernel(const double* __restric
                                                          double* __restrict__ out) {
   __shared__ double r[1024];
   double s = 0.0;
+#pragma unroll 8
   for (int64_t i = threadIdx.x; i < n; i += 1024) s += part[i];
   r[threadIdx.x] = s;
   __syncthreads();
@@ -291,28 +300,31 @@ static int for_tables(int nt, const void* const* p, const void* const* g, const 
   AwTab t;
   t.count = 0;
   int64_t blocks = 0, chunks = 0, before = 0;
+  auto flush = [&]() {
+    const int e = t.count ? fn(t, (unsigned)chunks, before) : 0;
+    before += chunks;
+    chunks = 0;
+    t.count = 0;
+    return e;
+  };
   for (int i = 0; i < nt; ++i) {
-    const int64_t nb = cdiv(n[i], 256);
-    if (g[i] && n[i]) {
-      t.p[t.count] = p ? p[i] : nullptr;
-      t.g[t.count] = g[i];
-      t.n[t.count] = n[i];
-      t.pt[t.count] = pt ? pt[i] : 0;
-      t.gt[t.count] = gt[i];
-      t.chunk0[t.count] = (int)chunks;
-      t.block0[t.count] = (int)blocks;
-      chunks += cdiv(nb, AW_CHUNK);
-      ++t.count;
-    }
-    blocks += nb;
-    if (t.count == AW_T || (i == nt - 1 && t.count)) {
-      if (int e = fn(t, (unsigned)chunks, before)) return e;
-      before += chunks;
-      chunks = 0;
-      t.count = 0;
+    for (int64_t at = 0; at < n[i]; at += AW_MAX) {
+      const int64_t k = std::min(n[i] - at, AW_MAX), nb = cdiv(k, 256);
+      if (g[i]) {
+        t.p[t.count] = p ? (const char*)p[i] + at * dtype_bytes(pt[i]) : nullptr;
+        t.g[t.count] = (const char*)g[i] + at * dtype_bytes(gt[i]);
+        t.n[t.count] = (unsigned)k;
+        t.types[t.count] = (uint8_t)((pt ? pt[i] : 0) | gt[i] << 4);
+        t.chunk0[t.count] = (int)chunks;
+        t.block0[t.count] = (int)blocks;
+        chunks += cdiv(nb, AW_CHUNK);
+        if (++t.count == AW_T)
+          if (int e = flush()) return e;
+      }
+      blocks += nb;
     }
   }
-  return 0;
+  return flush();
 }
 
 static const char* tensors_check(int nt, const void* const* g, const int64_t* n, const uint8_t* gt) {

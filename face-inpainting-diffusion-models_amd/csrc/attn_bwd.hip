@@ -8,11 +8,12 @@
 
 namespace ifd {
 
-template <typename T, int DP, int NW, int BK, int AHEAD, int OCC>
-__global__ __launch_bounds__(NW * 64, OCC) void attn_bwd_q_kernel(AttnK p) {
+// (waves and tiles as in the forward kernel)
+template <typename T, int DP, int BK, int AHEAD, int OCC>
+__global__ __launch_bounds__(256, OCC) void attn_bwd_q_kernel(AttnK p) {
   typedef AttnTile<T, DP> TL;
   typedef typename TL::frag frag;
-  constexpr int KT = BK / 32, TB = BK * TL::ROWB;
+  constexpr int NW = 4, KT = BK / 32, TB = BK * TL::ROWB;
   extern __shared__ __attribute__((aligned(1024))) char smem[];
   lds_c* sm = (lds_c*)smem;
   const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, h = lane >> 5;
@@ -160,10 +161,20 @@ __global__ __launch_bounds__(NW * 64, OCC) void attn_bwd_kv_kernel(AttnK p) {
   lds_c* sm = (lds_c*)smem;
   const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, h = lane >> 5;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int id = xcd_order(blockIdx.x, gridDim.x);
-  // one key block's shares are neighbours: they read the same rows
-  const int sp = id % p.nsplit;
-  const int kblk = (id / p.nsplit) % p.nblk, bh = id / p.nsplit / p.nblk;
+  // causal: the first key blocks see most rows and go first, a head's on one XCD; else head by head on each XCD
+  int sp, kblk, bh;
+  if (p.causal) {
+    const int n = p.B * p.Hk * p.nsplit;
+    const int r = blockIdx.x % n, x = (n & 7) ? r : (r & 7) * (n >> 3) + (r >> 3);
+    kblk = blockIdx.x / n;
+    bh = x / p.nsplit;
+    sp = x - bh * p.nsplit;
+  } else {
+    const int id = xcd_order(blockIdx.x, gridDim.x);
+    sp = id % p.nsplit;
+    kblk = (id / p.nsplit) % p.nblk;
+    bh = id / p.nsplit / p.nblk;
+  }
   const int b = bh / p.Hk, hk = bh - b * p.Hk;
   const int len = seq_len(p, b), qs = q_first(p, b);
   const int kb0 = kblk * (NW * 32), key = kb0 + w * 32 + l32;
@@ -337,31 +348,36 @@ __global__ __launch_bounds__(256) void attn_bwd_join_kernel(AttnK p) {
   *reinterpret_cast<quad*>(o + ch) = __builtin_convertvector(v, quad);
 }
 
-// Workgroups of the key pass: 128 keys each. The chip takes two per CU at a time and causal blocks differ in length, so
-// the walk is shared out until there are about four per CU, at least four row tiles each.
+// Workgroups of the key pass: 128 keys each, two per CU at a time. The walk is shared out until they fill the chip once, or
+// twice where a causal mask makes them unlike (2 x 4 heads x 4096 keys x 128: 518 us at 512 workgroups, 343 at 1024, 362 at
+// 2048; without a mask more shares only add sums to join: 4 x 8 x 1024 x 128, 62 + 25 us at 1024, 54 + 14 at 512), at least
+// four row tiles each.
 static int kv_split(const ifd_attention_args& a) {
   const int64_t base = (int64_t)a.B * a.Hk * cdiv(a.Tk, 128), tiles = (int64_t)(a.Hq / a.Hk) * cdiv(a.Tq, 64);
-  const int64_t n = std::min<int64_t>(cdiv(1024, std::max<int64_t>(base, 1)), std::max<int64_t>(tiles / 4, 1));
+  const int64_t n = std::min<int64_t>(cdiv(a.causal ? 1024 : 512, std::max<int64_t>(base, 1)), std::max<int64_t>(tiles / 4, 1));
   return (int)std::min<int64_t>(n, 16);
+}
+
+template <typename T, int DP>
+static int run_bwd_q(AttnK p, hipStream_t s) {
+  constexpr int ROWB = DP * (int)sizeof(T), BK = ROWB >= 512 ? 32 : 64, OCC = ROWB >= 512 ? 1 : 2;
+  constexpr int lds = 4 * BK * ROWB;
+  static bool attr[kMaxDevices] = {};
+  auto kern = attn_bwd_q_kernel<T, DP, BK, 4, OCC>;
+  if (set_lds_attr_once(attr, reinterpret_cast<const void*>(kern), lds) != hipSuccess) return IFD_LAUNCH_STATUS();
+  p.nblk = (int)cdiv(p.Tq, 128);
+  hipLaunchKernelGGL(kern, dim3(p.nblk * p.B * p.Hq), dim3(256), lds, s, p);
+  return IFD_LAUNCH_STATUS();
 }
 
 template <typename T, int DP>
 static int run_bwd(AttnK p, int nsplit, hipStream_t s) {
   constexpr int ROWB = DP * (int)sizeof(T);
-  constexpr int BK = ROWB >= 512 ? 32 : 64, OCC = ROWB >= 512 ? 1 : 2, AHQ = 4, OCCK = OCC;
+  constexpr int BK = ROWB >= 512 ? 32 : 64, OCCK = ROWB >= 512 ? 1 : 2;
   constexpr bool VL = sizeof(T) == 2 && DP == 128;
   constexpr int NWK = 4, BQ = VL ? 32 : BK;
-  {
-    constexpr int lds = 4 * BK * ROWB;
-    static bool attr[kMaxDevices] = {};
-    auto kern = attn_bwd_q_kernel<T, DP, 4, BK, AHQ, OCC>;
-    if (set_lds_attr_once(attr, reinterpret_cast<const void*>(kern), lds) != hipSuccess) return IFD_LAUNCH_STATUS();
-    p.nblk = (int)cdiv(p.Tq, 128);
-    if (p.Tq) {
-      hipLaunchKernelGGL(kern, dim3(p.nblk * p.B * p.Hq), dim3(256), lds, s, p);
-      if (int e = IFD_LAUNCH_STATUS()) return e;
-    }
-  }
+  if (p.Tq)
+    if (int e = run_bwd_q<T, DP>(p, s)) return e;
   if (!p.Tk) return 0;
   constexpr int lds = 2 * (2 * BQ * ROWB + 1024) + (VL ? NWK * 32 * ROWB : 0);
   static bool attr[kMaxDevices] = {};

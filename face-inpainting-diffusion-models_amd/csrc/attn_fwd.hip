@@ -72,14 +72,14 @@ struct AttnRows {
   }
 };
 
-// Many rows. A workgroup of NW waves takes NW * NQ * 32 rows of one (sequence, head); the waves share the K and V tiles
-// (BK keys, two buffers, the next tile's DMA in flight during this one's products). Per wave and tile: S^T = K Q^T with
-// Q in registers, softmax down the registers of each lane (a lane holds one row's scores of half the keys), O^T += V^T P^T.
-template <typename T, int DP, int NQ, int NW, int BK, int SUB, int OCC>
-__global__ __launch_bounds__(NW * 64, OCC) void attn_fwd_kernel(AttnK p) {
+// Many rows. A workgroup's four waves take 32 rows each of one (sequence, head) and share the K and V tiles (BK keys, two
+// buffers, the next tile's DMA in flight during this one's products). Per wave and tile: S^T = K Q^T with Q in registers,
+// softmax down the registers of each lane (a lane holds one row's scores of half the keys), O^T += V^T P^T.
+template <typename T, int DP, int BK, int OCC>
+__global__ __launch_bounds__(256, OCC) void attn_fwd_kernel(AttnK p) {
   typedef AttnTile<T, DP> TL;
   typedef typename TL::frag frag;
-  constexpr int KT = SUB / 32, TB = BK * TL::ROWB;
+  constexpr int NW = 4, KT = BK / 32, TB = BK * TL::ROWB;
   extern __shared__ __attribute__((aligned(1024))) char smem[];
   lds_c* sm = (lds_c*)smem;
   const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, h = lane >> 5;
@@ -98,26 +98,23 @@ __global__ __launch_bounds__(NW * 64, OCC) void attn_fwd_kernel(AttnK p) {
   }
   const int b = bh / p.Hq, hq = bh - b * p.Hq, hk = hq / p.G;
   const int len = seq_len(p, b), qs = q_first(p, b);
-  const int q0 = qblk * (NW * NQ * 32) + w * (NQ * 32);
+  const int q0 = qblk * (NW * 32) + w * 32;
+  const int i = q0 + l32;
+  const int lim = i < p.Tq ? row_limit(p, qs, len, i) : 0;
 
-  frag qf[NQ][TL::KS];
-  int lim[NQ];
-#pragma unroll
-  for (int n = 0; n < NQ; ++n) {
-    const int i = q0 + n * 32 + l32;
-    lim[n] = i < p.Tq ? row_limit(p, qs, len, i) : 0;
+  frag qf[TL::KS];
+  {
     const char* rp = p.q + b * p.qb + hq * p.qh + (int64_t)i * p.qt;
 #pragma unroll
-    for (int ks = 0; ks < TL::KS; ++ks) qf[n][ks] = TL::gload(rp, i < p.Tq, ks, h, p.D);
+    for (int ks = 0; ks < TL::KS; ++ks) qf[ks] = TL::gload(rp, i < p.Tq, ks, h, p.D);
   }
-  AttnRows<T, DP, KT> st[NQ];
-#pragma unroll
-  for (int n = 0; n < NQ; ++n) st[n].init();
+  AttnRows<T, DP, KT> st;
+  st.init();
 
   // keys that any row of the workgroup sees, of the wave; and those that all its rows see
-  const int last = min(p.Tq, (qblk + 1) * (NW * NQ * 32)) - 1;
+  const int last = min(p.Tq, (qblk + 1) * (NW * 32)) - 1;
   const int wg_end = row_limit(p, qs, len, last);
-  const int w_last = min(p.Tq, q0 + NQ * 32) - 1;
+  const int w_last = min(p.Tq, q0 + 32) - 1;
   const int w_end = __builtin_amdgcn_readfirstlane(w_last < q0 ? 0 : row_limit(p, qs, len, w_last));
   const int w_all = __builtin_amdgcn_readfirstlane(w_last < q0 ? 0 : row_limit(p, qs, len, q0));
   const int nt = (wg_end + BK - 1) / BK;
@@ -139,21 +136,17 @@ __global__ __launch_bounds__(NW * 64, OCC) void attn_fwd_kernel(AttnK p) {
   }
   for (int t = 0; t < nt; ++t) {
     if (t + 1 < nt) stage(t + 1);
-#pragma unroll 1
-    for (int sub = 0; sub < BK / SUB; ++sub) {
-      const int k0 = t * BK + sub * SUB;
-      if (k0 >= w_end) break;
-      const lds_c* kb = sm + (t & 1) * (2 * TB) + sub * (SUB * TL::ROWB);
+    const int k0 = t * BK;
+    if (k0 < w_end) {
+      const lds_c* kb = sm + (t & 1) * (2 * TB);
       const lds_c* vb = kb + TB;
-      f32x16 s[NQ][KT];
+      f32x16 s[KT];
+#pragma unroll
+      for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+        for (int x = 0; x < 16; ++x) s[kt][x] = 0.f;
       // KB operands are read ahead of the products that take them
       constexpr int KB = TL::ROWB == 128 ? 4 : 8;
-#pragma unroll
-      for (int n = 0; n < NQ; ++n)
-#pragma unroll
-        for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) s[n][kt][i] = 0.f;
 #pragma unroll
       for (int x0 = 0; x0 < KT * TL::KS; x0 += KB) {
         frag a[KB];
@@ -162,50 +155,39 @@ __global__ __launch_bounds__(NW * 64, OCC) void attn_fwd_kernel(AttnK p) {
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int x = 0; x < KB; ++x)
-#pragma unroll
-          for (int n = 0; n < NQ; ++n)
-            s[n][(x0 + x) / TL::KS] = TL::A::mma(a[x], qf[n][(x0 + x) % TL::KS], s[n][(x0 + x) / TL::KS]);
+          s[(x0 + x) / TL::KS] = TL::A::mma(a[x], qf[(x0 + x) % TL::KS], s[(x0 + x) / TL::KS]);
       }
-      const bool mask = k0 + SUB > w_all;
-      frag pf[NQ][KT][TL::PS];
-#pragma unroll
-      for (int n = 0; n < NQ; ++n) st[n].soft(s[n], p.c, mask, lim[n] - k0, h, pf[n]);
+      frag pf[KT][TL::PS];
+      st.soft(s, p.c, k0 + BK > w_all, lim - k0, h, pf);
 #pragma unroll
       for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
         for (int ps = 0; ps < TL::PS; ++ps)
 #pragma unroll
-          for (int d = 0; d < TL::DT; ++d) {
-            const frag a = TL::col(vb, kt * 32, ps, d, lane);
-#pragma unroll
-            for (int n = 0; n < NQ; ++n) st[n].o[d] = TL::A::mma(a, pf[n][kt][ps], st[n].o[d]);
-          }
+          for (int d = 0; d < TL::DT; ++d)
+            st.o[d] = TL::A::mma(TL::col(vb, kt * 32, ps, d, lane), pf[kt][ps], st.o[d]);
     }
     dma_wait();
     __syncthreads();
   }
+  const float l = st.l + xhalf(st.l);
+  if (i >= p.Tq) return;
+  const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+  if (h == 0)
+    p.lse[((int64_t)b * p.Hq + hq) * p.Tq + i] =
+        l == 0.f ? -INFINITY : (st.m + __builtin_amdgcn_logf(l)) * 0.69314718055994531f;
+  T* op = reinterpret_cast<T*>(p.out + b * p.ob + hq * p.oh + (int64_t)i * p.ot);
 #pragma unroll
-  for (int n = 0; n < NQ; ++n) {
-    const int i = q0 + n * 32 + l32;
-    const float l = st[n].l + xhalf(st[n].l);
-    if (i >= p.Tq) continue;
-    const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-    if (h == 0)
-      p.lse[((int64_t)b * p.Hq + hq) * p.Tq + i] =
-          l == 0.f ? -INFINITY : (st[n].m + __builtin_amdgcn_logf(l)) * 0.69314718055994531f;
-    T* op = reinterpret_cast<T*>(p.out + b * p.ob + hq * p.oh + (int64_t)i * p.ot);
+  for (int d = 0; d < TL::DT; ++d)
 #pragma unroll
-    for (int d = 0; d < TL::DT; ++d)
+    for (int j = 0; j < 4; ++j) {
+      const int ch = d * 32 + 8 * j + 4 * h;
+      if (ch >= p.D) continue;
+      f32x4 v;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int ch = d * 32 + 8 * j + 4 * h;
-        if (ch >= p.D) continue;
-        f32x4 v;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = st[n].o[d][4 * j + e] * inv;
-        *reinterpret_cast<typename TL::A::quad*>(op + ch) = __builtin_convertvector(v, typename TL::A::quad);
-      }
-  }
+      for (int e = 0; e < 4; ++e) v[e] = st.o[d][4 * j + e] * inv;
+      *reinterpret_cast<typename TL::A::quad*>(op + ch) = __builtin_convertvector(v, typename TL::A::quad);
+    }
 }
 
 // Few rows against many keys. The rows of all query heads of one key-value head (row r = token r / G, head r % G) fill
@@ -357,17 +339,21 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnK p) {
   const int bk = (int)(row / rows), r = (int)(row - (int64_t)bk * rows);
   const int b = bk / p.Hk, hk = bk - b * p.Hk, i = r / p.G, hq = hk * p.G + (r - i * p.G);
   const float* w = p.ws + ((int64_t)bk * p.nblk * 32 + r) * p.nsplit * (DP + 2);
-  float m = -INFINITY;
-  for (int s = lane; s < p.nsplit; s += 64) m = fmaxf(m, w[s * (DP + 2)]);
+  // lane s holds split s's statistics (at most 64 splits): the loads below do not wait for each other
+  const bool has = lane < p.nsplit;
+  const float ms = has ? w[lane * (DP + 2)] : -INFINITY, ls = has ? w[lane * (DP + 2) + 1] : 0.f;
+  float m = ms;
 #pragma unroll
   for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
-  float l = 0.f, a[DP / 64] = {};
-  for (int s = 0; s < p.nsplit; ++s) {
-    const float* x = w + s * (DP + 2);
-    const float f = x[0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(x[0] - m);
-    l += f * x[1];
+  const float fs = ms == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ms - m);
+  float l = fs * ls, a[DP / 64] = {};
 #pragma unroll
-    for (int e = 0; e < DP / 64; ++e) a[e] += f * x[2 + lane + 64 * e];
+  for (int o = 32; o; o >>= 1) l += __shfl_xor(l, o);
+#pragma unroll 8
+  for (int s = 0; s < p.nsplit; ++s) {
+    const float f = __shfl(fs, s);
+#pragma unroll
+    for (int e = 0; e < DP / 64; ++e) a[e] += f * w[s * (DP + 2) + 2 + lane + 64 * e];
   }
   const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
   T* op = reinterpret_cast<T*>(p.out + b * p.ob + hq * p.oh + (int64_t)i * p.ot);
@@ -424,7 +410,7 @@ static FwdPlan fwd_plan(const ifd_attention_args& a, int dp, int es) {
   r.nblk = (int)rb;
   const int bk = dp * es == 128 ? 64 : 32;
   const int64_t tiles = cdiv(a.Tk, bk);
-  int64_t n = cdiv(512, base);
+  int64_t n = cdiv(256, base);
   n = std::min<int64_t>(n, cdiv(tiles, 8));
   r.nsplit = (int)std::max<int64_t>(1, std::min<int64_t>(n, 64));
   return r;
@@ -452,19 +438,22 @@ AttnK attention_kernel_args(const ifd_attention_args& a) {
 }
 
 template <typename T, int DP>
+static int run_rows(const AttnK& p, hipStream_t s) {
+  constexpr int ROWB = DP * (int)sizeof(T), BK = ROWB >= 512 ? 32 : 64, OCC = ROWB == 128 ? 4 : ROWB == 256 ? 2 : 1;
+  constexpr int lds = 4 * BK * ROWB;
+  static bool attr[kMaxDevices] = {};
+  auto kern = attn_fwd_kernel<T, DP, BK, OCC>;
+  if (set_lds_attr_once(attr, reinterpret_cast<const void*>(kern), lds) != hipSuccess) return IFD_LAUNCH_STATUS();
+  hipLaunchKernelGGL(kern, dim3(p.nblk * p.B * p.Hq), dim3(256), lds, s, p);
+  return IFD_LAUNCH_STATUS();
+}
+
+template <typename T, int DP>
 static int run_fwd(const FwdPlan& pl, AttnK p, hipStream_t s) {
   constexpr int ROWB = DP * (int)sizeof(T);
   p.nblk = pl.nblk;
   p.nsplit = pl.nsplit;
-  if (!pl.split) {
-    constexpr int BK = ROWB >= 512 ? 32 : 64, SUB = ROWB >= 512 ? 32 : 64, NW = 4, OCC = ROWB == 128 ? 4 : ROWB == 256 ? 2 : 1;
-    constexpr int lds = 4 * BK * ROWB;
-    static bool attr[kMaxDevices] = {};
-    auto kern = attn_fwd_kernel<T, DP, 1, NW, BK, SUB, OCC>;
-    if (set_lds_attr_once(attr, reinterpret_cast<const void*>(kern), lds) != hipSuccess) return IFD_LAUNCH_STATUS();
-    hipLaunchKernelGGL(kern, dim3(p.nblk * p.B * p.Hq), dim3(NW * 64), lds, s, p);
-    return IFD_LAUNCH_STATUS();
-  }
+  if (!pl.split) return run_rows<T, DP>(p, s);
   constexpr int BK = ROWB == 128 ? 64 : 32, NW = ROWB >= 512 ? 2 : 4;
   constexpr int lds = NW * 4 * BK * ROWB;
   static bool attr[kMaxDevices] = {};
