@@ -1,6 +1,7 @@
 // Attention forward: out = softmax(scale q k^T) v and the rows' log-sum-exp (include/ifd_ops.h), one pass over the keys
 // with a running maximum and sum.
 #include "attn_dev.h"
+#include "kernels.h"
 
 namespace ifd {
 
@@ -173,7 +174,7 @@ __global__ __launch_bounds__(256, OCC) void attn_fwd_kernel(AttnK p) {
   const float l = st.l + xhalf(st.l);
   if (i >= p.Tq) return;
   const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-  if (h == 0)
+  if (h == 0 && p.lse)
     p.lse[((int64_t)b * p.Hq + hq) * p.Tq + i] =
         l == 0.f ? -INFINITY : (st.m + __builtin_amdgcn_logf(l)) * 0.69314718055994531f;
   T* op = reinterpret_cast<T*>(p.out + b * p.ob + hq * p.oh + (int64_t)i * p.ot);
@@ -468,6 +469,22 @@ static int run_fwd(const FwdPlan& pl, AttnK p, hipStream_t s) {
     return IFD_LAUNCH_STATUS();
   }
   return 0;
+}
+
+// The UNet's QKVAttention (code/nn.py:222-235) on qkv [N][T][3C]: heads of 64 channels at offsets 0, C, 2C; queries and keys
+// carry `scale` each.
+void launch_attention_rows(const float* qkv, int N, int T, int C, float scale, float* out, hipStream_t s) {
+  AttnK p = {};
+  p.q = (const char*)qkv; p.k = (const char*)(qkv + C); p.v = (const char*)(qkv + 2 * C);
+  p.out = (char*)out;
+  p.qb = p.kb = p.vb = (int64_t)T * 3 * C * 4; p.ob = (int64_t)T * C * 4;
+  p.qt = p.kt = p.vt = 3 * C * 4; p.ot = C * 4;
+  p.qh = p.kh = p.vh = p.oh = 64 * 4;
+  p.B = N; p.Tq = p.Tk = T; p.Hq = p.Hk = C / 64; p.D = 64; p.G = 1;
+  p.scale = scale * scale;
+  p.c = p.scale * 1.4426950408889634f;
+  p.nblk = (int)cdiv(T, 128);
+  (void)run_rows<float, 64>(p, s);  // (the status of the launch is read by the caller)
 }
 
 }  // namespace ifd

@@ -327,6 +327,8 @@ static void launch_attention_mfma(const float* qkv, int N, int C, float scale, f
 }
 
 void launch_attention(const float* qkv, int N, int T, int C, float scale, float* out, hipStream_t s) {
+  // attention_kernel keeps a whole row of scores, 256 at most; longer maps run the tiled kernel with a running softmax
+  if (T > 256) return launch_attention_rows(qkv, N, T, C, scale, out, s);
   if (C % AT_CH == 0) {
     if (T == 256) return launch_attention_mfma<8>(qkv, N, C, scale, out, s);
     if (T == 128) return launch_attention_mfma<4>(qkv, N, C, scale, out, s);

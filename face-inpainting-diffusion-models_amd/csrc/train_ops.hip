@@ -3396,6 +3396,8 @@ int ifd_tr_copy_channels(const float* src, int cs, int soff, float* dst, int cd,
 
 int ifd_tr_attention(const float* qkv, int N, int T, int C, float scale, float* out, void* stream) {
   if (C % 64) { set_error("ifd_tr_attention: 64-channel heads"); return 2; }
+  if (T < 1 || N < 0 || ((int64_t)T + 127) / 128 * (C / 64) * N > 0x7fffffff) { set_error("ifd_tr_attention: sizes"); return 2; }
+  if (!N) return 0;
   launch_attention(qkv, N, T, C, scale, out, (hipStream_t)stream);
   return TR_LAST();
 }

@@ -24,4 +24,10 @@ def __getattr__(name):
     if name == "create_model_and_diffusion":
         from .factory import create_model_and_diffusion
         return create_model_and_diffusion
+    if name == "AdamW":
+        from .optim import AdamW
+        return AdamW
+    if name == "Rotary":
+        from .rotary import Rotary
+        return Rotary
     raise AttributeError(name)

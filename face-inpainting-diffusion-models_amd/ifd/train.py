@@ -27,6 +27,8 @@ import numpy as np
 import torch
 
 from . import _lib
+from .attention import attention, attention_bwd
+from .optim import AdamW
 from .topology import FULL, UNetConfig, layer_plan, state_dict_spec
 
 _c = ctypes
@@ -153,6 +155,11 @@ class UNetTrainer:
     out_layers.0, in_layers.2 -> in_layers.0 without resampling) computes that backward's pass-1 partial sums in
     its epilogue (ifd_tr_conv_x3_gnb): the pass over (dout, x) of ifd_tr_gn_bwd is not run.
 
+    state_bits=8: both AdamW moments as one byte a value and a scale per 256 values (ifd.optim.AdamW, `self.opt`): 2 bytes of
+    state a parameter instead of 8; `seed` seeds their rounding. The gradients then stay unclipped in the grad buffer, a
+    step whose gradient norm is not finite is left out, and norm_coef is fp64. state_dict() holds the parameters alone, as
+    with 32 bits; `opt.state_dict()` the states.
+
     gnb_act (with fuse_gnb, round 6, off by default): that epilogue also writes the GroupNorm's forward output
     silu(z) — the input of the conv whose weight gradient is next (ifd_tr_conv_x3_gnb_act) — so that weight
     gradient runs the plain split kernel on it instead of re-applying GroupNorm + SiLU on load (1.82 vs 1.66 ms
@@ -164,7 +171,7 @@ class UNetTrainer:
 
     def __init__(self, cfg: UNetConfig = FULL, device="cuda", lr=5e-5, weight_decay=0.01, betas=(0.9, 0.999),
                  eps=1e-8, max_norm=1.0, precision="fp32", x3_dgrad=True, x3_wgrad=True, x3_loss_scale_log2=20,
-                 fuse_gn=True, fuse_gnb=True, gnb_act=False):
+                 fuse_gn=True, fuse_gnb=True, gnb_act=False, state_bits=32, seed=0):
         if precision not in ("fp32", "3xf16", "f16"):
             raise ValueError(f"precision must be 'fp32', '3xf16' or 'f16', got {precision!r}")
         self.precision = precision
@@ -186,9 +193,16 @@ class UNetTrainer:
             n += int(np.prod(shape))
         self.numel = n
         z = lambda: torch.zeros(n, device=self.dev, dtype=torch.float32)  # noqa: E731
-        self.flat, self.grad, self.m, self.v = z(), z(), z(), z()
+        self.flat, self.grad = z(), z()
         self.step_count = 0
-        self.norm_coef = torch.zeros(2, device=self.dev)
+        if state_bits == 32:
+            self.opt = None
+            self.m, self.v = z(), z()
+            self.norm_coef = torch.zeros(2, device=self.dev)
+        else:
+            self.opt = AdamW([self.p(k) for k, _ in self.spec], lr=lr, betas=betas, eps=eps, weight_decay=weight_decay,
+                             state_bits=state_bits, max_norm=max_norm, seed=seed)
+            self.norm_coef = self.opt.norm_coef
         self.loss = torch.zeros(1, device=self.dev)
         self._gt_noise_cache = {}
         # timestep_embedding frequencies exactly as the reference builds them (code/nn.py:54-56)
@@ -800,6 +814,15 @@ class UNetTrainer:
                         mode=mode, r=r, ro=ro)
         return out, ro
 
+    # Tokens up to which attention keeps its probabilities (ifd_tr_attention / _bwd, 2 N heads T^2 floats of scratch in the
+    # backward); longer maps (attention at a higher resolution) run ifd.attention, whose backward recomputes them.
+    ATTN_ROWS = 256
+
+    @staticmethod
+    def _heads(qkv, N, T, C):
+        """The q, k, v slices [N, T, heads, 64] of [N, T, 3C] rows."""
+        return qkv.view(N, T, 3, C // 64, 64).unbind(2)
+
     def _attn_fwd(self, L, x, N, r, saved):
         """AttentionBlock._forward (code/nn.py:259-265) with QKVAttention (:222-235)."""
         p, C = L["prefix"], L["cin"]
@@ -808,9 +831,14 @@ class UNetTrainer:
         qkv = self.conv(n, C, N, r, p + "qkv.weight", p + "qkv.bias")
         a = self._empty(N, T, C)
         scale = 1.0 / math.sqrt(math.sqrt(self.cfg.num_head_channels))
-        chk(lib().ifd_tr_attention(P(qkv), N, T, C, scale, P(a), self.s))
+        lse = None
+        if T <= self.ATTN_ROWS:
+            chk(lib().ifd_tr_attention(P(qkv), N, T, C, scale, P(a), self.s))
+        else:  # (64-channel heads chunk-first: slices of the qkv rows)
+            q, k, v = self._heads(qkv, N, T, C)
+            _, lse = attention(q, k, v, scale=scale * scale, out=a.view(N, T, C // 64, 64))
         out = self.conv(a, C, N, r, p + "proj_out.weight", p + "proj_out.bias", res=x)
-        saved[p] = dict(x=x, n=n, st=st, qkv=qkv, a=a, scale=scale)
+        saved[p] = dict(x=x, n=n, st=st, qkv=qkv, a=a, scale=scale, lse=lse)
         return out
 
     def backward(self, dout6, grad_scale=None):
@@ -937,9 +965,15 @@ class UNetTrainer:
             self.wgrad(dout, C, sv["a"], C, N, r, p + "proj_out.weight", p + "proj_out.bias")
             da = self.conv(dout, C, N, r, p + "proj_out.weight", transpose=True)
             dqkv = self._empty(N, T, 3 * C)
-            sf = lib().ifd_tr_attention_bwd_scratch_floats(N, T, C)
-            scratch = self._empty(sf)
-            chk(lib().ifd_tr_attention_bwd(P(sv["qkv"]), P(da), N, T, C, sv["scale"], P(dqkv), P(scratch), sf, self.s))
+            if sv["lse"] is None:
+                sf = lib().ifd_tr_attention_bwd_scratch_floats(N, T, C)
+                scratch = self._empty(sf)
+                chk(lib().ifd_tr_attention_bwd(P(sv["qkv"]), P(da), N, T, C, sv["scale"], P(dqkv), P(scratch), sf, self.s))
+            else:
+                q, k, v = self._heads(sv["qkv"], N, T, C)
+                dq, dk, dv = self._heads(dqkv, N, T, C)
+                attention_bwd(da.view(N, T, C // 64, 64), q, k, v, sv["a"].view(N, T, C // 64, 64), sv["lse"],
+                              scale=sv["scale"] ** 2, dq=dq, dk=dk, dv=dv)
             self.wgrad(dqkv, 3 * C, sv["n"], C, N, r, p + "qkv.weight", p + "qkv.bias")
             dn = self.conv(dqkv, 3 * C, N, r, p + "qkv.weight", transpose=True)
             # the residual's gradient: accumulated into dout in place (dout is not read after this)
@@ -1081,6 +1115,12 @@ class UNetTrainer:
     def optimizer_step(self):
         """clip_grad_norm_(max_norm) + AdamW (code/train_inpainting.py:64-66); norm on device, no sync."""
         self.step_count += 1
+        if self.opt is not None:
+            o = self.opt
+            o.groups[0]["lr"], o.groups[0]["weight_decay"], o.step_count = self.lr, self.wd, self.step_count - 1
+            o.betas, o.eps, o.max_norm = tuple(self.betas), self.eps, self.max_norm
+            o.step([self.g(k) for k, _ in self.spec])
+            return
         work = torch.empty(1024, device=self.dev, dtype=torch.float64)
         b1, b2 = self.betas
         chk(lib().ifd_tr_clip_adamw(P(self.flat), P(self.grad), P(self.m), P(self.v), self.numel, self.max_norm,
