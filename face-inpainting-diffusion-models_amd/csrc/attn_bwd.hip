@@ -112,10 +112,12 @@ __global__ __launch_bounds__(256, OCC) void attn_bwd_q_kernel(AttnK p) {
           }
           __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-          for (int x = 0; x < AHEAD; ++x) {
-            s = TL::A::mma(ka[x], qf[k1 + x], s);
-            dp = TL::A::mma(va[x], gf[k1 + x], dp);
-          }
+          for (int x = 0; x < AHEAD; ++x)
+#pragma unroll
+            for (int j = 0; j < TL::A::MS; ++j) {
+              s = TL::A::mma(ka[x], qf[k1 + x], j, s);
+              dp = TL::A::mma(va[x], gf[k1 + x], j, dp);
+            }
         }
         if (mask) {
 #pragma unroll
@@ -127,8 +129,13 @@ __global__ __launch_bounds__(256, OCC) void attn_bwd_q_kernel(AttnK p) {
 #pragma unroll
         for (int ps = 0; ps < TL::PS; ++ps) {
           const frag f = TL::pack(s, ps);
+          frag a[TL::DT];
 #pragma unroll
-          for (int d = 0; d < TL::DT; ++d) acc[d] = TL::A::mma(TL::col(kb, kt * 32, ps, d, lane), f, acc[d]);
+          for (int d = 0; d < TL::DT; ++d) a[d] = TL::col(kb, kt * 32, ps, d, lane);
+#pragma unroll
+          for (int j = 0; j < TL::A::MS; ++j)
+#pragma unroll
+            for (int d = 0; d < TL::DT; ++d) acc[d] = TL::A::mma(a[d], f, j, acc[d]);
         }
       }
     }
@@ -254,8 +261,13 @@ __global__ __launch_bounds__(NW * 64, OCC) void attn_bwd_kv_kernel(AttnK p) {
       for (int x = 0; x < 16; ++x) s[x] = dp[x] = 0.f;
 #pragma unroll
       for (int ks = 0; ks < TL::KS; ++ks) {
-        s = TL::A::mma(TL::row(qb, qt * 32, ks, l32, h), kf[ks], s);
-        dp = TL::A::mma(TL::row(gb, qt * 32, ks, l32, h), VL ? TL::row(vt, w * 32, ks, l32, h) : vf[VL ? 0 : ks], dp);
+        const frag qa = TL::row(qb, qt * 32, ks, l32, h), ga = TL::row(gb, qt * 32, ks, l32, h);
+        const frag vb = VL ? TL::row(vt, w * 32, ks, l32, h) : vf[VL ? 0 : ks];
+#pragma unroll
+        for (int j = 0; j < TL::A::MS; ++j) {
+          s = TL::A::mma(qa, kf[ks], j, s);
+          dp = TL::A::mma(ga, vb, j, dp);
+        }
       }
       const bool mask = rr < w_hi || rr + 32 > p.Tq;
 #pragma unroll
@@ -278,8 +290,12 @@ __global__ __launch_bounds__(NW * 64, OCC) void attn_bwd_kv_kernel(AttnK p) {
         const frag fp = TL::pack(s, ps), fd = TL::pack(dp, ps);
 #pragma unroll
         for (int d = 0; d < TL::DT; ++d) {
-          dv[d] = TL::A::mma(TL::col(gb, qt * 32, ps, d, lane), fp, dv[d]);
-          dk[d] = TL::A::mma(TL::col(qb, qt * 32, ps, d, lane), fd, dk[d]);
+          const frag ga = TL::col(gb, qt * 32, ps, d, lane), qa = TL::col(qb, qt * 32, ps, d, lane);
+#pragma unroll
+          for (int j = 0; j < TL::A::MS; ++j) {
+            dv[d] = TL::A::mma(ga, fp, j, dv[d]);
+            dk[d] = TL::A::mma(qa, fd, j, dk[d]);
+          }
         }
       }
     }

@@ -41,7 +41,8 @@ struct AttnT<__bf16> {
   typedef bf16x4 quad;
   typedef bf16x2 pair;
   static constexpr int PS = 2;  // contraction steps per 32 rows
-  static __device__ __forceinline__ f32x16 mma(frag a, frag b, f32x16 c) {
+  static constexpr int MS = 1;  // MFMAs per operand pair; products of several accumulators take turns (a dependent MFMA waits)
+  static __device__ __forceinline__ f32x16 mma(frag a, frag b, int, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
   }
 };
@@ -50,8 +51,8 @@ struct AttnT<_Float16> {
   typedef hf16x8 frag;
   typedef hf16x4 quad;
   typedef hf16x2 pair;
-  static constexpr int PS = 2;
-  static __device__ __forceinline__ f32x16 mma(frag a, frag b, f32x16 c) {
+  static constexpr int PS = 2, MS = 1;
+  static __device__ __forceinline__ f32x16 mma(frag a, frag b, int, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
   }
 };
@@ -60,11 +61,9 @@ struct AttnT<float> {
   typedef f32x4 frag;
   typedef f32x4 quad;
   typedef f32x2 pair;
-  static constexpr int PS = 4;
-  static __device__ __forceinline__ f32x16 mma(frag a, frag b, f32x16 c) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[j], b[j], c, 0, 0, 0);
-    return c;
+  static constexpr int PS = 4, MS = 4;
+  static __device__ __forceinline__ f32x16 mma(frag a, frag b, int j, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x2f32(a[j], b[j], c, 0, 0, 0);
   }
 };
 

@@ -146,27 +146,37 @@ __global__ __launch_bounds__(256, OCC) void attn_fwd_kernel(AttnK p) {
       for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
         for (int x = 0; x < 16; ++x) s[kt][x] = 0.f;
-      // KB operands are read ahead of the products that take them
-      constexpr int KB = TL::ROWB == 128 ? 4 : 8;
+      // KB steps' operands are read ahead of the products that take them
+      constexpr int KB = TL::ROWB == 128 ? 2 : 4;
 #pragma unroll
-      for (int x0 = 0; x0 < KT * TL::KS; x0 += KB) {
-        frag a[KB];
+      for (int k1 = 0; k1 < TL::KS; k1 += KB) {
+        frag a[KB][KT];
 #pragma unroll
-        for (int x = 0; x < KB; ++x) a[x] = TL::row(kb, (x0 + x) / TL::KS * 32, (x0 + x) % TL::KS, l32, h);
+        for (int x = 0; x < KB; ++x)
+#pragma unroll
+          for (int kt = 0; kt < KT; ++kt) a[x][kt] = TL::row(kb, kt * 32, k1 + x, l32, h);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int x = 0; x < KB; ++x)
-          s[(x0 + x) / TL::KS] = TL::A::mma(a[x], qf[(x0 + x) % TL::KS], s[(x0 + x) / TL::KS]);
+#pragma unroll
+          for (int j = 0; j < TL::A::MS; ++j)
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt) s[kt] = TL::A::mma(a[x][kt], qf[k1 + x], j, s[kt]);
       }
       frag pf[KT][TL::PS];
       st.soft(s, p.c, k0 + BK > w_all, lim - k0, h, pf);
 #pragma unroll
       for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
-        for (int ps = 0; ps < TL::PS; ++ps)
+        for (int ps = 0; ps < TL::PS; ++ps) {
+          frag a[TL::DT];
 #pragma unroll
-          for (int d = 0; d < TL::DT; ++d)
-            st.o[d] = TL::A::mma(TL::col(vb, kt * 32, ps, d, lane), pf[kt][ps], st.o[d]);
+          for (int d = 0; d < TL::DT; ++d) a[d] = TL::col(vb, kt * 32, ps, d, lane);
+#pragma unroll
+          for (int j = 0; j < TL::A::MS; ++j)
+#pragma unroll
+            for (int d = 0; d < TL::DT; ++d) st.o[d] = TL::A::mma(a[d], pf[kt][ps], j, st.o[d]);
+        }
     }
     dma_wait();
     __syncthreads();
@@ -261,16 +271,26 @@ __global__ __launch_bounds__(NW * 64) void attn_split_kernel(AttnK p) {
 #pragma unroll
       for (int i2 = 0; i2 < 16; ++i2) s[kt][i2] = 0.f;
 #pragma unroll
-      for (int ks = 0; ks < TL::KS; ++ks) s[kt] = TL::A::mma(TL::row(kb, kt * 32, ks, l32, h), qf[ks], s[kt]);
+      for (int ks = 0; ks < TL::KS; ++ks) {
+        const frag a = TL::row(kb, kt * 32, ks, l32, h);
+#pragma unroll
+        for (int j = 0; j < TL::A::MS; ++j) s[kt] = TL::A::mma(a, qf[ks], j, s[kt]);
+      }
     }
     frag pf[KT][TL::PS];
     st.soft(s, p.c, k0 + BK > all, lim - k0, h, pf);
 #pragma unroll
     for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
-      for (int ps = 0; ps < TL::PS; ++ps)
+      for (int ps = 0; ps < TL::PS; ++ps) {
+        frag a[TL::DT];
 #pragma unroll
-        for (int d = 0; d < TL::DT; ++d) st.o[d] = TL::A::mma(TL::col(vb, kt * 32, ps, d, lane), pf[kt][ps], st.o[d]);
+        for (int d = 0; d < TL::DT; ++d) a[d] = TL::col(vb, kt * 32, ps, d, lane);
+#pragma unroll
+        for (int j = 0; j < TL::A::MS; ++j)
+#pragma unroll
+          for (int d = 0; d < TL::DT; ++d) st.o[d] = TL::A::mma(a[d], pf[kt][ps], j, st.o[d]);
+      }
     // the reads above are complete before the next round's DMA overwrites this buffer
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     buf ^= 1;
