@@ -269,20 +269,22 @@ __global__ __launch_bounds__(NW * 64, OCC) void attn_bwd_kv_kernel(AttnK p) {
           dp = TL::A::mma(ga, vb, j, dp);
         }
       }
-      const bool mask = rr < w_hi || rr + 32 > p.Tq;
+      if (rr < w_hi || rr + 32 > p.Tq) {  // rows before the key's first, or past the last (copies of it): p = ds = 0
+#pragma unroll
+        for (int x = 0; x < 16; ++x) {
+          const int r = rr + 8 * (x >> 2) + 4 * h + (x & 3);
+          if (r < lo || r >= p.Tq) s[x] = -INFINITY;
+        }
+      }
 #pragma unroll
       for (int y = 0; y < 4; ++y) {
         const f32x4 ls = lds_quad(qb + 2 * TB + 4 * (qt * 32 + 8 * y + 4 * h));
         const f32x4 de = lds_quad(qb + 2 * TB + 512 + 4 * (qt * 32 + 8 * y + 4 * h));
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const int x = 4 * y + e, r = rr + 8 * y + 4 * h + e;
-          float pv = __builtin_amdgcn_exp2f(fmaf(s[x], p.c, -ls[e]));
-          if (mask && (r < lo || r >= p.Tq)) pv = 0.f;
-          float dsv = pv * (dp[x] - de[e]);
-          if (mask && (r < lo || r >= p.Tq)) dsv = 0.f;
-          s[x] = pv;
-          dp[x] = dsv;
+          const int x = 4 * y + e;
+          s[x] = __builtin_amdgcn_exp2f(fmaf(s[x], p.c, -ls[e]));
+          dp[x] = s[x] * (dp[x] - de[e]);
         }
       }
 #pragma unroll
