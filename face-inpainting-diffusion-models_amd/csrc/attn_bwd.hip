@@ -217,8 +217,18 @@ __global__ __launch_bounds__(NW * 64, OCC) void attn_bwd_kv_kernel(AttnK p) {
   const int it0 = (int)(all * sp / p.nsplit), it1 = (int)(all * (sp + 1) / p.nsplit);
   AttnStage<T, DP, BQ, NW> sg;
   sg.init(w, lane, p.D);
-  auto stage = [&](int it, int buf) {
-    const int hq = hk * p.G + it / ntq, r0 = (tq0 + it % ntq) * BQ, n = min(BQ, p.Tq - r0);
+  // the next pair to stage: (head of the group, row tile)
+  int sg_h = 0, sg_t = 0;
+  if (it0 < it1) {
+    sg_h = it0 / ntq;
+    sg_t = it0 - sg_h * ntq;
+  }
+  auto stage = [&](int buf) {
+    const int hq = hk * p.G + sg_h, r0 = (tq0 + sg_t) * BQ, n = min(BQ, p.Tq - r0);
+    if (++sg_t == ntq) {
+      sg_t = 0;
+      ++sg_h;
+    }
     lds_c* d = sm + buf * BUF;
     sg.load(p.q + b * p.qb + hq * p.qh + (int64_t)r0 * p.qt, p.qt, n, d, w);
     sg.load(p.dout + b * p.gb + hq * p.gh + (int64_t)r0 * p.gt, p.gt, n, d + TB, w);
@@ -233,7 +243,7 @@ __global__ __launch_bounds__(NW * 64, OCC) void attn_bwd_kv_kernel(AttnK p) {
       sv.init(w, lane, p.D);
       sv.load(p.v + b * p.vb + hk * p.vh + (int64_t)kb0 * p.vt, p.vt, min(NW * 32, len - kb0), sm + 2 * BUF, w);
     }
-    stage(it0, 0);
+    stage(0);
     dma_wait();
     if (VL && p.D < DP) {
       // both factors of dp come from LDS here: V's channels past D must be zeros
@@ -246,12 +256,13 @@ __global__ __launch_bounds__(NW * 64, OCC) void attn_bwd_kv_kernel(AttnK p) {
     }
     __syncthreads();
   }
-  int buf = 0;
-  for (int it = it0; it < it1; ++it, buf ^= 1) {
-    if (it + 1 < it1) stage(it + 1, buf ^ 1);
+  int buf = 0, t = it0 < it1 ? sg_t - 1 : 0;  // this round's row tile
+  if (t < 0) t = ntq - 1;
+  for (int it = it0; it < it1; ++it, buf ^= 1, t = t + 1 == ntq ? 0 : t + 1) {
+    if (it + 1 < it1) stage(buf ^ 1);
     const lds_c* qb = sm + buf * BUF;
     const lds_c* gb = qb + TB;
-    const int r0 = (tq0 + it % ntq) * BQ;
+    const int r0 = (tq0 + t) * BQ;
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) {
       const int rr = r0 + qt * 32;
