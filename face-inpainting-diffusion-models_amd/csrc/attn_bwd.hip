@@ -389,10 +389,11 @@ static int kv_split(const ifd_attention_args& a) {
 
 template <typename T, int DP>
 static int run_bwd_q(AttnK p, hipStream_t s) {
-  constexpr int ROWB = DP * (int)sizeof(T), BK = ROWB >= 512 ? 32 : 64, OCC = ROWB >= 512 ? 1 : 2;
-  constexpr int lds = 4 * BK * ROWB;
+  typedef AttnTile<T, DP> TL;
+  constexpr int BK = TL::ROWB >= 512 ? 32 : 64, OCC = TL::ROWB >= 512 ? 1 : 2, AHEAD = TL::KS % 4 ? 3 : 4;
+  constexpr int lds = 4 * BK * TL::ROWB;
   static bool attr[kMaxDevices] = {};
-  auto kern = attn_bwd_q_kernel<T, DP, BK, 4, OCC>;
+  auto kern = attn_bwd_q_kernel<T, DP, BK, AHEAD, OCC>;
   if (set_lds_attr_once(attr, reinterpret_cast<const void*>(kern), lds) != hipSuccess) return IFD_LAUNCH_STATUS();
   p.nblk = (int)cdiv(p.Tq, 128);
   hipLaunchKernelGGL(kern, dim3(p.nblk * p.B * p.Hq), dim3(256), lds, s, p);
@@ -401,7 +402,7 @@ static int run_bwd_q(AttnK p, hipStream_t s) {
 
 template <typename T, int DP>
 static int run_bwd(AttnK p, int nsplit, hipStream_t s) {
-  constexpr int ROWB = DP * (int)sizeof(T);
+  constexpr int ROWB = AttnTile<T, DP>::ROWB;
   constexpr int BK = ROWB >= 512 ? 32 : 64, OCCK = ROWB >= 512 ? 1 : 2;
   constexpr bool VL = sizeof(T) == 2 && DP == 128;
   constexpr int NWK = 4, BQ = VL ? 32 : BK;
@@ -424,6 +425,11 @@ static int run_bwd(AttnK p, int nsplit, hipStream_t s) {
   return 0;
 }
 
+template <typename T>
+static int run_bwd_d(const AttnK& p, int nsplit, hipStream_t s) {
+  return p.D <= 64 ? run_bwd<T, 64>(p, nsplit, s) : p.D <= 96 ? run_bwd<T, 96>(p, nsplit, s) : run_bwd<T, 128>(p, nsplit, s);
+}
+
 }  // namespace ifd
 
 using namespace ifd;
@@ -431,7 +437,7 @@ extern "C" {
 
 int64_t ifd_op_attention_bwd_ws_bytes(const ifd_attention_args* a) {
   if (!a || attention_check(*a) || !a->B) return 0;
-  const int dp = a->D <= 64 ? 64 : 128, n = kv_split(*a);
+  const int dp = a->D <= 64 ? 64 : a->D <= 96 ? 96 : 128, n = kv_split(*a);
   const int64_t part = n > 1 ? (int64_t)a->B * a->Hk * n * a->Tk * 2 * dp : 0;
   return (2 * (int64_t)a->B * a->Hq * a->Tq + part) * 4;
 }
@@ -459,10 +465,8 @@ int ifd_op_attention_bwd(const ifd_attention_args* a, void* ws, int64_t ws_bytes
   AttnK p = attention_kernel_args(*a);
   p.ws = (float*)ws;
   hipStream_t s = (hipStream_t)stream;
-  const bool d64 = a->D <= 64;
-  if (a->dtype == IFD_F32) return d64 ? run_bwd<float, 64>(p, n, s) : run_bwd<float, 128>(p, n, s);
-  if (a->dtype == IFD_BF16) return d64 ? run_bwd<__bf16, 64>(p, n, s) : run_bwd<__bf16, 128>(p, n, s);
-  return d64 ? run_bwd<_Float16, 64>(p, n, s) : run_bwd<_Float16, 128>(p, n, s);
+  return a->dtype == IFD_F32 ? run_bwd_d<float>(p, n, s)
+                             : a->dtype == IFD_BF16 ? run_bwd_d<__bf16>(p, n, s) : run_bwd_d<_Float16>(p, n, s);
 }
 
 }  // extern "C"

@@ -71,8 +71,9 @@ template <typename T, int DP>
 struct AttnTile {
   typedef AttnT<T> A;
   typedef typename A::frag frag;
-  static constexpr int ES = sizeof(T), CE = 16 / ES, NCH = DP / CE, ROWB = DP * ES;
-  static constexpr int KS = NCH / 2, DT = DP / 32, PS = A::PS;
+  // DP: the head width the products cover (64, 96 or 128); a row in LDS takes the next power of two
+  static constexpr int ES = sizeof(T), CE = 16 / ES, NCH = (DP == 96 ? 128 : DP) / CE, ROWB = NCH * 16;
+  static constexpr int KS = DP / CE / 2, DT = DP / 32, PS = A::PS;
 
   static __device__ __forceinline__ int swz(int r) {
     if (ES == 4) return ((r & 7) << 1) | ((r >> 3) & 1);

@@ -147,7 +147,7 @@ __global__ __launch_bounds__(256, OCC) void attn_fwd_kernel(AttnK p) {
 #pragma unroll
         for (int x = 0; x < 16; ++x) s[kt][x] = 0.f;
       // KB steps' operands are read ahead of the products that take them
-      constexpr int KB = TL::ROWB == 128 ? 2 : 4;
+      constexpr int KB = TL::ROWB == 128 ? 2 : TL::KS % 4 ? 3 : 4;
 #pragma unroll
       for (int k1 = 0; k1 < TL::KS; k1 += KB) {
         frag a[KB][KT];
@@ -460,7 +460,7 @@ AttnK attention_kernel_args(const ifd_attention_args& a) {
 
 template <typename T, int DP>
 static int run_rows(const AttnK& p, hipStream_t s) {
-  constexpr int ROWB = DP * (int)sizeof(T), BK = ROWB >= 512 ? 32 : 64, OCC = ROWB == 128 ? 4 : ROWB == 256 ? 2 : 1;
+  constexpr int ROWB = AttnTile<T, DP>::ROWB, BK = ROWB >= 512 ? 32 : 64, OCC = ROWB == 128 ? 4 : ROWB == 256 ? 2 : 1;
   constexpr int lds = 4 * BK * ROWB;
   static bool attr[kMaxDevices] = {};
   auto kern = attn_fwd_kernel<T, DP, BK, OCC>;
@@ -470,11 +470,8 @@ static int run_rows(const AttnK& p, hipStream_t s) {
 }
 
 template <typename T, int DP>
-static int run_fwd(const FwdPlan& pl, AttnK p, hipStream_t s) {
+static int run_split(const AttnK& p, hipStream_t s) {
   constexpr int ROWB = DP * (int)sizeof(T);
-  p.nblk = pl.nblk;
-  p.nsplit = pl.nsplit;
-  if (!pl.split) return run_rows<T, DP>(p, s);
   constexpr int BK = ROWB == 128 ? 64 : 32, NW = ROWB >= 512 ? 2 : 4;
   constexpr int lds = NW * 4 * BK * ROWB;
   static bool attr[kMaxDevices] = {};
@@ -489,6 +486,14 @@ static int run_fwd(const FwdPlan& pl, AttnK p, hipStream_t s) {
     return IFD_LAUNCH_STATUS();
   }
   return 0;
+}
+
+template <typename T>
+static int run_fwd(const FwdPlan& pl, AttnK p, hipStream_t s) {
+  p.nblk = pl.nblk;
+  p.nsplit = pl.nsplit;
+  if (pl.split) return p.D <= 64 ? run_split<T, 64>(p, s) : run_split<T, 128>(p, s);
+  return p.D <= 64 ? run_rows<T, 64>(p, s) : p.D <= 96 ? run_rows<T, 96>(p, s) : run_rows<T, 128>(p, s);
 }
 
 // The UNet's QKVAttention (code/nn.py:222-235) on qkv [N][T][3C]: heads of 64 channels at offsets 0, C, 2C; queries and keys
@@ -537,9 +542,8 @@ int ifd_op_attention(const ifd_attention_args* a, void* ws, int64_t ws_bytes, vo
   AttnK p = attention_kernel_args(*a);
   p.ws = (float*)ws;
   hipStream_t s = (hipStream_t)stream;
-  if (a->dtype == IFD_F32) return dp == 64 ? run_fwd<float, 64>(pl, p, s) : run_fwd<float, 128>(pl, p, s);
-  if (a->dtype == IFD_BF16) return dp == 64 ? run_fwd<__bf16, 64>(pl, p, s) : run_fwd<__bf16, 128>(pl, p, s);
-  return dp == 64 ? run_fwd<_Float16, 64>(pl, p, s) : run_fwd<_Float16, 128>(pl, p, s);
+  return a->dtype == IFD_F32 ? run_fwd<float>(pl, p, s)
+                             : a->dtype == IFD_BF16 ? run_fwd<__bf16>(pl, p, s) : run_fwd<_Float16>(pl, p, s);
 }
 
 }  // extern "C"
