@@ -11,7 +11,7 @@ three slices of a packed projection or a slice of a longer key-value cache; tens
 Row i of sequence b sees key j when j < kv_len[b] (default Tk) and, with causal=True, j <= q_start[b] + i (default
 Tk - Tq: the rows are the last ones). kv_len, q_start: int32 [B] on the GPU, read by the kernels (no synchronisation).
 Keys at and past kv_len are never read, whatever they hold. A row that sees no key gets out = 0, lse = -inf and zero
-gradients. Keys that only the causal mask hides are read: they must be finite in v.
+gradients. Keys that only the causal mask hides are read: v must be finite there, for the backward pass k too.
 
 The backward pass keeps no score matrix: it recomputes the probabilities from lse. Both directions are deterministic.
 Calls run on the current stream of the tensors' device and can be captured into a graph.
@@ -84,7 +84,7 @@ def _pack(q, k, v, scale, causal, kv_len, q_start, out, lse):
 def _into(t, like, name):
     """A caller's output tensor (checked) or a new contiguous one."""
     if t is None:
-        return torch.empty(like.shape, dtype=like.dtype, device=like.device)
+        return torch.empty_like(like, memory_format=torch.contiguous_format)
     if not (t.shape == like.shape and t.dtype == like.dtype and t.device == like.device):
         refuse(f"{name} must be like its input")
     if _lay(t) is not t:

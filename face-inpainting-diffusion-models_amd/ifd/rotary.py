@@ -123,7 +123,7 @@ def _into(t, like, name):
     if like is None:
         return None
     if t is None:
-        return torch.empty(like.shape, dtype=like.dtype, device=like.device)
+        return torch.empty_like(like, memory_format=torch.contiguous_format)
     if not (t.shape == like.shape and t.dtype == like.dtype and t.device == like.device
             and (t.stride(3) == 1 or t.shape[3] == 1)):
         refuse(f"{name} must be like its input, with adjacent channels")
