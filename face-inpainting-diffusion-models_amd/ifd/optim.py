@@ -53,7 +53,8 @@ class AdamW:
         at = 0
         for g in self.groups:
             g["block0"] = at
-            g["sizes"] = [p.numel() for p in g["params"]]
+            g["shapes"] = [p.shape for p in g["params"]]
+            g["sizes"] = (ctypes.c_int64 * len(g["params"]))(*[p.numel() for p in g["params"]])
             at += sum(-(-p.numel() // BLOCK) for p in g["params"])
         self.nblocks = at
         z = lambda n, dt: torch.zeros(n, dtype=dt, device=self.device)  # noqa: E731
@@ -62,23 +63,26 @@ class AdamW:
         self.m_scale, self.v_scale = (z(at, torch.float32), z(at, torch.float32)) if state_bits == 8 else (None, None)
         self.norm_coef = torch.ones(2, dtype=torch.float64, device=self.device)
 
-    def _arrays(self, params, sizes, grads):
+    def _arrays(self, grp, grads):
         """Host arrays of one group: addresses, counts, types (read afresh at every step: tensors may have moved)."""
-        n, dev, types = len(params), self.device, DTYPES
-        gp, gt = [0] * n, bytearray(n)
-        for i, (x, d) in enumerate(zip(params, grads)):
+        n, dev, types = len(grads), self.device.index, DTYPES
+        pp, gp, pt, gt = [], [], [], []
+        for x, d, shape in zip(grp["params"], grads, grp["shapes"]):
+            if x.shape != shape or not x.is_contiguous() or x.get_device() != dev or x.dtype not in types:
+                refuse(f"parameter {len(pp)} is no longer the contiguous {tuple(shape)} tensor on {self.device} it was")
+            pp.append(x.data_ptr())
+            pt.append(types[x.dtype])
             if d is None:
+                gp.append(0)
+                gt.append(0)
                 continue
-            if not (d.dtype in types and d.shape == x.shape and d.is_contiguous() and d.device == dev):
-                refuse(f"gradient {i}: contiguous fp32, bf16 or fp16 of shape {tuple(x.shape)} on {dev} expected, got "
-                       f"{d.dtype} {tuple(d.shape)} on {d.device}")
-            if not (x.is_contiguous() and x.device == dev):
-                refuse(f"parameter {i} is no longer a contiguous tensor on {dev}")
-            gp[i], gt[i] = d.data_ptr(), types[d.dtype]
-        if [x.numel() for x in params] != sizes:
-            refuse("a parameter has changed its size")
-        return ((ctypes.c_void_p * n)(*[x.data_ptr() for x in params]), (ctypes.c_void_p * n)(*gp),
-                (ctypes.c_int64 * n)(*sizes), bytes(types[x.dtype] for x in params), bytes(gt))
+            if d.shape != shape or not d.is_contiguous() or d.get_device() != dev or d.dtype not in types:
+                refuse(f"gradient {len(gp)}: contiguous fp32, bf16 or fp16 of shape {tuple(shape)} on {self.device} expected, "
+                       f"got {d.dtype} {tuple(d.shape)} on {d.device}")
+            gp.append(d.data_ptr())
+            gt.append(types[d.dtype])
+        ptrs = ctypes.c_void_p * n
+        return ptrs(*pp), ptrs(*gp), grp["sizes"], bytes(pt), bytes(gt)
 
     def step(self, grads=None):
         """One step; grads in the order of the parameters (None entries: that tensor is left alone)."""
@@ -89,7 +93,7 @@ class AdamW:
         at, arrays = 0, []
         for grp in self.groups:
             k = len(grp["params"])
-            arrays.append(self._arrays(grp["params"], grp["sizes"], grads[at:at + k]))
+            arrays.append(self._arrays(grp, grads[at:at + k]))
             at += k
         if self.max_norm is not None:
             self._norm(L, arrays)

@@ -260,3 +260,25 @@ def test_agrees_with_the_flat_optimizer():
     torch.cuda.synchronize()
     # both round the same fp32 formulas; the clip coefficient here is formed in fp64: 2 ulp of the parameters
     assert ((p - q).abs() <= 4 * U * p.abs() + 12 * U * 3 * 5e-5).all()
+
+
+def test_wrong_gradients_and_changed_parameters_are_refused():
+    from ifd.optim import AdamW
+    p = [torch.randn(8, 6, device=DEV), torch.randn(5, device=DEV)]
+    opt = AdamW(p, lr=LR)
+    good = [torch.randn(8, 6, device=DEV), torch.randn(5, device=DEV)]
+    for bad, msg in (([good[0]], "1 gradients for 2"), ([good[0].t(), good[1]], "gradient 0"),
+                     ([good[0].double(), good[1]], "gradient 0"), ([good[0], good[1].cpu()], "gradient 1"),
+                     ([good[0], torch.randn(10, device=DEV)[::2]], "gradient 1")):
+        with pytest.raises(ValueError, match=msg):
+            opt.step(bad)
+    assert opt.step_count == 0
+    p[1].data = torch.randn(300, device=DEV)
+    with pytest.raises(ValueError, match="parameter 1"):
+        opt.step(good)
+    graph = torch.cuda.CUDAGraph()
+    opt2 = AdamW([good[0]], lr=LR)
+    with torch.cuda.graph(graph):
+        good[1].mul_(1.0)
+        with pytest.raises(ValueError, match="captured"):
+            opt2.step([good[0]])
