@@ -18,9 +18,6 @@
 
 namespace ifd {
 
-typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
-typedef _Float16 hf16x4 __attribute__((ext_vector_type(4)));
-
 constexpr int AW_T = 128;     // tensors of a launch (its tables fill the 4 KB of kernel arguments)
 constexpr int64_t AW_MAX = (int64_t)1 << 31;  // values of a table entry: a longer tensor takes several
 constexpr int AW_CHUNK = 16;  // blocks of a workgroup
@@ -53,62 +50,50 @@ __device__ __forceinline__ int aw_find(const AwTab& t, int wg) {
   return __builtin_amdgcn_readfirstlane(n - 1);
 }
 
-__device__ __forceinline__ f32x4 aw_load(const void* base, int dt, int64_t i, int64_t n) {
-  f32x4 r = {0.f, 0.f, 0.f, 0.f};
-  if (dt == IFD_F32) {
-    const float* q = reinterpret_cast<const float*>(base) + i;
-    if (i + 4 <= n && ((uintptr_t)base & 15) == 0) return *reinterpret_cast<const f32x4*>(q);
+// Values [i, i + 4) of a block, of which `left` lie inside the tensor (4: all). `block` is the same for the wave, and so is
+// `whole`: a block inside the tensor whose address allows vector loads.
+template <typename T>
+struct AwMem {
+  typedef T quad __attribute__((ext_vector_type(4)));
+  static __device__ __forceinline__ f32x4 load(const void* block, int i, int left, bool whole) {
+    const T* q = reinterpret_cast<const T*>(block) + i;
+    if (whole) return __builtin_convertvector(*reinterpret_cast<const quad*>(q), f32x4);
+    f32x4 r = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-      if (i + j < n) r[j] = q[j];
-  } else if (dt == IFD_BF16) {
-    const __bf16* q = reinterpret_cast<const __bf16*>(base) + i;
-    if (i + 4 <= n && ((uintptr_t)base & 7) == 0)
-      return __builtin_convertvector(*reinterpret_cast<const bf16x4*>(q), f32x4);
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (i + j < n) r[j] = (float)q[j];
-  } else {
-    const _Float16* q = reinterpret_cast<const _Float16*>(base) + i;
-    if (i + 4 <= n && ((uintptr_t)base & 7) == 0)
-      return __builtin_convertvector(*reinterpret_cast<const hf16x4*>(q), f32x4);
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (i + j < n) r[j] = (float)q[j];
+      if (j < left) r[j] = (float)q[j];
+    return r;
   }
-  return r;
+  static __device__ __forceinline__ void store(void* block, int i, int left, bool whole, f32x4 v) {
+    T* q = reinterpret_cast<T*>(block) + i;
+    const quad x = __builtin_convertvector(v, quad);
+    if (whole) {
+      *reinterpret_cast<quad*>(q) = x;
+      return;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (j < left) q[j] = x[j];
+  }
+};
+__device__ __forceinline__ int aw_bytes(int dt) { return dt == IFD_F32 ? 4 : 2; }
+__device__ __forceinline__ f32x4 aw_load(const void* base, int dt, int bi, int lane, int64_t n) {
+  const char* b = reinterpret_cast<const char*>(base) + (int64_t)bi * (256 * aw_bytes(dt));
+  const int64_t left = n - (int64_t)bi * 256;
+  const bool whole = left >= 256 && !((uintptr_t)b & (4 * aw_bytes(dt) - 1));
+  const int l4 = (int)(left < 256 ? left : 256) - 4 * lane;
+  if (dt == IFD_F32) return AwMem<float>::load(b, 4 * lane, l4, whole);
+  if (dt == IFD_BF16) return AwMem<__bf16>::load(b, 4 * lane, l4, whole);
+  return AwMem<_Float16>::load(b, 4 * lane, l4, whole);
 }
-__device__ __forceinline__ void aw_store(void* base, int dt, int64_t i, int64_t n, f32x4 v) {
-  if (dt == IFD_F32) {
-    float* q = reinterpret_cast<float*>(base) + i;
-    if (i + 4 <= n && ((uintptr_t)base & 15) == 0) {
-      *reinterpret_cast<f32x4*>(q) = v;
-      return;
-    }
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (i + j < n) q[j] = v[j];
-  } else if (dt == IFD_BF16) {
-    __bf16* q = reinterpret_cast<__bf16*>(base) + i;
-    const bf16x4 x = __builtin_convertvector(v, bf16x4);
-    if (i + 4 <= n && ((uintptr_t)base & 7) == 0) {
-      *reinterpret_cast<bf16x4*>(q) = x;
-      return;
-    }
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (i + j < n) q[j] = x[j];
-  } else {
-    _Float16* q = reinterpret_cast<_Float16*>(base) + i;
-    const hf16x4 x = __builtin_convertvector(v, hf16x4);
-    if (i + 4 <= n && ((uintptr_t)base & 7) == 0) {
-      *reinterpret_cast<hf16x4*>(q) = x;
-      return;
-    }
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (i + j < n) q[j] = x[j];
-  }
+__device__ __forceinline__ void aw_store(void* base, int dt, int bi, int lane, int64_t n, f32x4 v) {
+  char* b = reinterpret_cast<char*>(base) + (int64_t)bi * (256 * aw_bytes(dt));
+  const int64_t left = n - (int64_t)bi * 256;
+  const bool whole = left >= 256 && !((uintptr_t)b & (4 * aw_bytes(dt) - 1));
+  const int l4 = (int)(left < 256 ? left : 256) - 4 * lane;
+  if (dt == IFD_F32) return AwMem<float>::store(b, 4 * lane, l4, whole, v);
+  if (dt == IFD_BF16) return AwMem<__bf16>::store(b, 4 * lane, l4, whole, v);
+  return AwMem<_Float16>::store(b, 4 * lane, l4, whole, v);
 }
 
 // multiply / xor-shift mix (the multipliers: 2^32 times the fractions of the golden ratio, sqrt 2 and sqrt 3, odd)
@@ -133,24 +118,28 @@ __device__ __forceinline__ double m_value(unsigned c) {  // without the scale
 }
 __device__ __forceinline__ double v_value(unsigned c) { return hi_double(c ? 0x3E000000u + (c << 17) : 0u); }
 
+// The byte of y = |x| / scale: the random bits lie in the double's high word, so the low word never decides. What lies under
+// the smallest value (1.125 2^-bias) is that value; for m, at random, that or 0.
 __device__ __forceinline__ unsigned m_code(double x, double inv, unsigned r16) {
-  const double tiny = 0x1.2p-15;
   const double y = fabs(x) * inv;
-  // (the random bits lie in the high word: the low word of y never decides)
-  const int k = (int)(((unsigned)__double2hiint(fmax(y, tiny)) + (r16 << 1)) >> 17) - ((1023 - 15) << 3);
-  if (y * 65536.0 + tiny * (double)r16 < tiny * 65536.0) return 0;
-  return (unsigned)min(max(k, 1), 127) | (x < 0.0 ? 128u : 0u);
+  const unsigned hi = (unsigned)__double2hiint(y), tiny = 0x3F020000u;
+  unsigned k = min(((max(hi, tiny) + (r16 << 1)) >> 17) - ((1023u - 15u) << 3), 127u);
+  if (hi < tiny) {
+    const double t = 0x1.2p-15;
+    if (y * 65536.0 + t * (double)r16 < t * 65536.0) k = 0;
+  }
+  return k ? k | (((unsigned)__double2hiint(x) >> 24) & 128u) : 0u;
 }
 __device__ __forceinline__ unsigned v_code(double x, double inv, unsigned r16) {
-  const double tiny = 0x1.2p-31;
   const double y = x * inv;
-  const int k = (int)(((unsigned)__double2hiint(fmax(y, tiny)) + (r16 << 1)) >> 17) - ((1023 - 31) << 3);
-  return y > 0.0 ? (unsigned)min(max(k, 1), 255) : 0u;
+  const unsigned hi = (unsigned)__double2hiint(y), tiny = 0x3E020000u;
+  const unsigned k = min(((max(hi, tiny) + (r16 << 1)) >> 17) - ((1023u - 31u) << 3), 255u);
+  return y > 0.0 ? k : 0u;
 }
 
 template <int BITS>
 __global__ __launch_bounds__(256) void adamw_multi_kernel(const AwTab t, const AwArgs a) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int ti = aw_find(t, blockIdx.x);
   const int64_t n = t.n[ti];
   const int pt = t.types[ti] & 15, gt = t.types[ti] >> 4;
@@ -162,25 +151,26 @@ __global__ __launch_bounds__(256) void adamw_multi_kernel(const AwTab t, const A
     if (!(norm < __builtin_huge_val())) return;  // a NaN or infinite gradient: no step
     coef = a.clip[1];
   }
+  const double w1 = a.w1 * coef, w2 = a.w2 * (coef * coef);
   const int nblk = (int)((n + 255) >> 8);
   const int b0 = (blockIdx.x - t.chunk0[ti]) * AW_CHUNK;
   for (int bi = b0 + wave; bi < min(nblk, b0 + AW_CHUNK); bi += 4) {
-    const int64_t i = (int64_t)bi * 256 + lane * 4;
-    const int64_t blk = a.block0 + t.block0[ti] + bi, e = blk * 256 + lane * 4;
-    const f32x4 p0 = aw_load(pp, pt, i, n), g0 = aw_load(gp, gt, i, n);
+    const int left = (int)min(n - (int64_t)bi * 256, (int64_t)256) - 4 * lane;  // this lane's values inside the tensor
+    const int64_t blk = a.block0 + t.block0[ti] + bi, e = blk * 256;
+    const f32x4 p0 = aw_load(pp, pt, bi, lane, n), g0 = aw_load(gp, gt, bi, lane, n);
     f32x4 mf, vf;
     if (BITS == 8) {
-      unsigned char* mc = reinterpret_cast<unsigned char*>(a.m);
-      unsigned char* vc = reinterpret_cast<unsigned char*>(a.v);
-      const unsigned cm = *reinterpret_cast<const unsigned*>(mc + e), cv = *reinterpret_cast<const unsigned*>(vc + e);
-      const double sm = a.ms[blk], sv = a.vs[blk];
+      unsigned* mc = reinterpret_cast<unsigned*>(reinterpret_cast<unsigned char*>(a.m) + e);
+      unsigned* vc = reinterpret_cast<unsigned*>(reinterpret_cast<unsigned char*>(a.v) + e);
+      const unsigned cm = mc[lane], cv = vc[lane];
+      const double sm = a.b1 * (double)a.ms[blk], sv = a.b2 * (double)a.vs[blk];
       double m[4], v[4];
       double xm = 0.0, xv = 0.0;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const double g = (double)g0[j] * coef;
-        m[j] = a.b1 * (m_value((cm >> (8 * j)) & 255u) * sm) + a.w1 * g;
-        v[j] = a.b2 * (v_value((cv >> (8 * j)) & 255u) * sv) + a.w2 * (g * g);
+        const double g = g0[j];
+        m[j] = fma(m_value((cm >> (8 * j)) & 255u), sm, w1 * g);
+        v[j] = fma(v_value((cv >> (8 * j)) & 255u), sv, w2 * (g * g));
         mf[j] = (float)m[j];
         vf[j] = (float)v[j];
         xm = fmax(xm, fabs(m[j]));
@@ -192,46 +182,46 @@ __global__ __launch_bounds__(256) void adamw_multi_kernel(const AwTab t, const A
       unsigned nm = 0, nv = 0;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const unsigned r = aw_mix((unsigned)(e + j) + a.key);
-        if (i + j < n) {  // what lies behind the tensor's end stays 0
+        const unsigned r = aw_mix((unsigned)e + 4u * lane + j + a.key);
+        if (j < left) {  // what lies behind the tensor's end stays 0
           nm |= m_code(m[j], im, r & 0xFFFFu) << (8 * j);
           nv |= v_code(v[j], iv, r >> 16) << (8 * j);
         }
       }
-      *reinterpret_cast<unsigned*>(mc + e) = nm;
-      *reinterpret_cast<unsigned*>(vc + e) = nv;
+      mc[lane] = nm;
+      vc[lane] = nv;
       if (lane == 0) {
         a.ms[blk] = am;
         a.vs[blk] = av;
       }
     } else {
-      float* mm = reinterpret_cast<float*>(a.m) + e;
-      float* vv = reinterpret_cast<float*>(a.v) + e;
-      const float w1 = (float)a.w1, b2 = (float)a.b2, w2 = (float)a.w2, c = (float)coef;
-      mf = *reinterpret_cast<const f32x4*>(mm);
-      vf = *reinterpret_cast<const f32x4*>(vv);
+      f32x4* mm = reinterpret_cast<f32x4*>(reinterpret_cast<float*>(a.m) + e);
+      f32x4* vv = reinterpret_cast<f32x4*>(reinterpret_cast<float*>(a.v) + e);
+      const float w1f = (float)a.w1, b2 = (float)a.b2, w2f = (float)a.w2, c = (float)coef;
+      mf = mm[lane];
+      vf = vv[lane];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const float g = g0[j] * c;
-        mf[j] = mf[j] + (g - mf[j]) * w1;
-        vf[j] = vf[j] * b2 + w2 * g * g;
+        mf[j] = mf[j] + (g - mf[j]) * w1f;
+        vf[j] = vf[j] * b2 + w2f * g * g;
       }
-      *reinterpret_cast<f32x4*>(mm) = mf;
-      *reinterpret_cast<f32x4*>(vv) = vf;
+      mm[lane] = mf;
+      vv[lane] = vf;
     }
     f32x4 q;
 #pragma unroll
     for (int j = 0; j < 4; ++j)  // hardware square root and reciprocal: 1 ulp each, of the step
       q[j] = p0[j] * a.decay -
              a.step * (mf[j] * __builtin_amdgcn_rcpf(fmaf(__builtin_amdgcn_sqrtf(vf[j]), a.rbc2s, a.eps)));
-    aw_store(pp, pt, i, n, q);
+    aw_store(pp, pt, bi, lane, n, q);
   }
 }
 
 // sums of squares in fp64, one per workgroup
 __global__ __launch_bounds__(256) void grad_sq_kernel(const AwTab t, double* __restrict__ part) {
   __shared__ double r[4];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int ti = aw_find(t, blockIdx.x);
   const int64_t n = t.n[ti];
   const int nblk = (int)((n + 255) >> 8);
@@ -242,8 +232,8 @@ __global__ __launch_bounds__(256) void grad_sq_kernel(const AwTab t, double* __r
   for (int bi = b0 + wave; bi < b1; bi += 16) {
     f32x4 g[4];
 #pragma unroll
-    for (int u = 0; u < 4; ++u)  // (a block past the chunk: nothing is read)
-      g[u] = aw_load(gp, gt, (int64_t)(bi + 4 * u) * 256 + lane * 4, bi + 4 * u < b1 ? n : 0);
+    for (int u = 0; u < 4; ++u)
+      g[u] = bi + 4 * u < b1 ? aw_load(gp, gt, bi + 4 * u, lane, n) : f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int u = 0; u < 4; ++u)
 #pragma unroll
