@@ -14,6 +14,7 @@
 // Everything that decides a byte is computed in fp64 (full rate here), so it does not depend on how the compiler orders
 // fp32 roundings; the step itself uses the moments before they are rounded, in fp32.
 #include <cmath>
+#include "lanes.h"
 #include "ops.h"
 
 namespace ifd {
@@ -106,10 +107,11 @@ __host__ __device__ __forceinline__ unsigned aw_mix(unsigned x) {
   return x ^ (x >> 16);
 }
 
-__device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-  for (int o = 32; o; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
-  return v;
+// 1 / x to the last bit or so: the hardware's estimate and two Newton steps
+__device__ __forceinline__ double recip(double x) {
+  double r = __builtin_amdgcn_rcp(x);
+  r = fma(r, fma(-x, r, 1.0), r);
+  return fma(r, fma(-x, r, 1.0), r);
 }
 __device__ __forceinline__ double hi_double(unsigned hi) { return __hiloint2double((int)hi, 0); }
 __device__ __forceinline__ double m_value(unsigned c) {  // without the scale
@@ -124,7 +126,7 @@ __device__ __forceinline__ unsigned m_code(double x, double inv, unsigned r16) {
   const double y = fabs(x) * inv;
   const unsigned hi = (unsigned)__double2hiint(y), tiny = 0x3F020000u;
   unsigned k = min(((max(hi, tiny) + (r16 << 1)) >> 17) - ((1023u - 15u) << 3), 127u);
-  if (hi < tiny) {
+  if (__any(hi < tiny)) {  // (rare: no lane pays for it otherwise)
     const double t = 0x1.2p-15;
     if (y * 65536.0 + t * (double)r16 < t * 65536.0) k = 0;
   }
@@ -177,16 +179,19 @@ __global__ __launch_bounds__(256) void adamw_multi_kernel(const AwTab t, const A
         xv = fmax(xv, v[j]);
       }
       // the scale rounds max |x| / 1.875 to fp32: rounding keeps order, so the largest rounded value of the lanes is it
-      const float am = wave_max((float)(xm * (1.0 / 1.875))), av = wave_max((float)(xv * (1.0 / 1.875)));
-      const double im = am > 0.f ? 1.0 / (double)am : 0.0, iv = av > 0.f ? 1.0 / (double)av : 0.0;
+      const float am = wave_max_nonneg((float)(xm * (1.0 / 1.875))), av = wave_max_nonneg((float)(xv * (1.0 / 1.875)));
+      const double im = am > 0.f ? recip(am) : 0.0, iv = av > 0.f ? recip(av) : 0.0;
       unsigned nm = 0, nv = 0;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const unsigned r = aw_mix((unsigned)e + 4u * lane + j + a.key);
-        if (j < left) {  // what lies behind the tensor's end stays 0
-          nm |= m_code(m[j], im, r & 0xFFFFu) << (8 * j);
-          nv |= v_code(v[j], iv, r >> 16) << (8 * j);
-        }
+        nm |= m_code(m[j], im, r & 0xFFFFu) << (8 * j);
+        nv |= v_code(v[j], iv, r >> 16) << (8 * j);
+      }
+      if (left < 4) {  // what lies behind the tensor's end stays 0
+        const unsigned in = left > 0 ? (1u << (8 * left)) - 1 : 0u;
+        nm &= in;
+        nv &= in;
       }
       mc[lane] = nm;
       vc[lane] = nv;

@@ -8,6 +8,7 @@
 // the token and the lane alone: it is computed once per token and reused for every head, and the lane groups that hold
 // different heads of a token compute a share of its V angles each and exchange them (one each for eight groups and V = 8).
 #include <type_traits>
+#include "lanes.h"
 #include "ops.h"
 
 namespace ifd {
@@ -118,7 +119,7 @@ __global__ __launch_bounds__(256) void qk_rope_kernel(QkK p) {
           float ss = 0.f;
 #pragma unroll
           for (int j = 0; j < 2 * V; ++j) ss = fmaf(m[j], m[j], ss);
-          for (int o = p.lg >> 1; o; o >>= 1) ss += __shfl_xor(ss, o);
+          ss = group_sum(ss, p.lg);
           rstd = __builtin_amdgcn_rsqf(fmaf(ss, p.rD, p.eps));  // 1 ulp
         }
         if (!BWD) {
@@ -152,8 +153,7 @@ __global__ __launch_bounds__(256) void qk_rope_kernel(QkK p) {
               y[j] *= w[isk][j];
               dot = fmaf(y[j], m[j], dot);
             }
-            for (int o = p.lg >> 1; o; o >>= 1) dot += __shfl_xor(dot, o);
-            dot *= p.rD;
+            dot = group_sum(dot, p.lg) * p.rD;
 #pragma unroll
             for (int j = 0; j < 2 * V; ++j) y[j] = rstd * (y[j] - m[j] * dot);
           }
