@@ -97,6 +97,25 @@ def same_device(*tensors):
     return dev
 
 
+def no_grad(*tensors):
+    """These operators record nothing for autograd: a call that autograd would have to follow is refused, not cut off."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                refuse("the operator records no gradients: call it under torch.no_grad() (or with detached tensors) and its "
+                       "backward function yourself")
+
+
+def output(t, like, name):
+    """Checks a caller's output tensor: like its input, every element a place of its own; marks it as written."""
+    if not (t.shape == like.shape and t.dtype == like.dtype and t.device == like.device):
+        refuse(f"{name} must be like its input")
+    if any(s == 0 and n > 1 for s, n in zip(t.stride(), t.shape)):
+        refuse(f"{name} has elements that share their place")
+    torch.autograd.graph.increment_version(t)
+    return t
+
+
 def workspace(nbytes, dev):
     """Scratch of one call, from torch's stream-ordered allocator (None when the call needs none)."""
     return torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None

@@ -11,10 +11,11 @@ three slices of a packed projection or a slice of a longer key-value cache; tens
 Row i of sequence b sees key j when j < kv_len[b] (default Tk) and, with causal=True, j <= q_start[b] + i (default
 Tk - Tq: the rows are the last ones). kv_len, q_start: int32 [B] on the GPU, read by the kernels (no synchronisation).
 Keys at and past kv_len are never read, whatever they hold. A row that sees no key gets out = 0, lse = -inf and zero
-gradients. Keys that only the causal mask hides are read: v must be finite there, for the backward pass k too.
+gradients. Output tensors of the caller (out, dq, dk, dv) must not overlap the inputs. Keys that only the causal mask hides are read: v must be finite there, for the backward pass k too.
 
 The backward pass keeps no score matrix: it recomputes the probabilities from lse. Both directions are deterministic.
-Calls run on the current stream of the tensors' device and can be captured into a graph.
+Calls run on the current stream of the tensors' device and can be captured into a graph. They record nothing for autograd:
+tensors that require gradients are refused unless under torch.no_grad().
 """
 from __future__ import annotations
 
@@ -23,7 +24,7 @@ import struct
 
 import torch
 
-from ._ops import DTYPES, call, lib, refuse, same_device, workspace
+from ._ops import DTYPES, call, lib, no_grad, output, refuse, same_device, workspace
 
 # ifd_attention_args (include/ifd_ops.h): packed here because filling a ctypes structure field by field costs more than
 # the smallest kernels run (_ops.AttentionArgs has the same layout)
@@ -66,6 +67,7 @@ def _inputs(q, k, v, scale, kv_len, q_start):
     if not 0.0 < scale < 3e38:
         refuse(f"scale must be positive and finite, got {scale}")
     dev = same_device(q, k, v)
+    no_grad(q, k, v)
     if kv_len is not None:
         kv_len = _int_arg(kv_len, B, "kv_len", dev)
     if q_start is not None:
@@ -81,21 +83,37 @@ def _pack(q, k, v, scale, causal, kv_len, q_start, out, lse):
                      *out.stride()[:3])
 
 
-def _into(t, like, name):
+def _may_overlap(a, b):
+    """Whether two [batch, tokens, heads, channels] tensors could share elements. Told apart: other storages, ranges one
+    behind the other, and different channel ranges of the same token rows (slices of one packed buffer)."""
+    if a.untyped_storage().data_ptr() != b.untyped_storage().data_ptr() or not a.numel() or not b.numel():
+        return False
+    end = lambda t: t.storage_offset() + sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1  # noqa: E731
+    if min(a.stride() + b.stride()) < 0 or a.storage_offset() >= end(b) or b.storage_offset() >= end(a):
+        return min(a.stride() + b.stride()) < 0
+    row = a.stride(1)
+    if a.stride()[:2] != b.stride()[:2] or row <= 0 or a.stride(0) % row:
+        return True
+    lo = [t.storage_offset() % row for t in (a, b)]
+    hi = [o + (t.shape[2] - 1) * t.stride(2) + t.shape[3] for o, t in zip(lo, (a, b))]
+    return max(hi) > row or not (hi[0] <= lo[1] or hi[1] <= lo[0])
+
+
+def _into(t, like, name, *inputs):
     """A caller's output tensor (checked) or a new contiguous one."""
     if t is None:
         return torch.empty_like(like, memory_format=torch.contiguous_format)
-    if not (t.shape == like.shape and t.dtype == like.dtype and t.device == like.device):
-        refuse(f"{name} must be like its input")
-    if _lay(t) is not t:
+    if not (t.dim() == 4 and _lay(t) is t):
         refuse(f"{name}: adjacent channels, 16-byte aligned, strides in multiples of 16 bytes")
-    return t
+    if any(_may_overlap(t, x) for x in inputs):
+        refuse(f"{name} overlaps an input")
+    return output(t, like, name)
 
 
 def attention(q, k, v, scale=None, causal=False, kv_len=None, q_start=None, out=None):
     """(out, lse): attention of every query row, and its log-sum-exp fp32 [B, Hq, Tq]."""
     q, k, v, scale, kv_len, q_start, dev = _inputs(q, k, v, scale, kv_len, q_start)
-    out = _into(out, q, "out")
+    out = _into(out, q, "out", q, k, v)
     lse = torch.empty((q.shape[0], q.shape[2], q.shape[1]), dtype=torch.float32, device=dev)
     a = _pack(q, k, v, scale, causal, kv_len, q_start, out, lse) + _NO_BWD
     L = lib()
@@ -115,8 +133,10 @@ def attention_bwd(dout, q, k, v, out, lse, scale=None, causal=False, kv_len=None
     if lse.shape != (q.shape[0], q.shape[2], q.shape[1]) or lse.dtype != torch.float32:
         refuse("lse must be the forward's, fp32 [B, Hq, Tq]")
     same_device(q, dout, out, lse)
+    no_grad(dout, out)
     dout, out, lse = _lay(dout), _lay(out), lse.contiguous()
-    dq, dk, dv = _into(dq, q, "dq"), _into(dk, k, "dk"), _into(dv, v, "dv")
+    ins = (q, k, v, dout, out)
+    dq, dk, dv = _into(dq, q, "dq", *ins), _into(dk, k, "dk", *ins), _into(dv, v, "dv", *ins)
     a = _pack(q, k, v, scale, causal, kv_len, q_start, out, lse) + _BWD.pack(
         dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), *dout.stride()[:3], *dq.stride()[:3],
         *dk.stride()[:3], *dv.stride()[:3])

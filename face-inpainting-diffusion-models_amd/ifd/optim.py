@@ -109,6 +109,8 @@ class AdamW:
             a.eps, a.wd = self.eps, grp["weight_decay"]
             a.norm_coef = None if self.max_norm is None else self.norm_coef.data_ptr()
             call(L.ifd_op_adamw, dev, ctypes.byref(a))
+        if any([p.requires_grad for p in self.params]):  # (autograd learns that saved parameters have changed)
+            torch.autograd.graph.increment_version(self.params)
 
     def _norm(self, L, arrays):
         if len(arrays) == 1:

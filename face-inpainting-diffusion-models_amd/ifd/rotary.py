@@ -8,7 +8,8 @@ q: [B, T, Hq, D], k: [B, T, Hk, D], one type (fp32, bf16, fp16), D <= 128 and ev
 slices of a packed projection). n = x / sqrt(mean x^2 + eps) * w over each head's channels; the first `rope.rot` channels
 are then turned in pairs by the angle pos * inv_freq (fp64, so that far positions keep their angle) and scaled by
 rope.mscale. norm=False leaves out the norm, rope=None the rotation, wq / wk=None the weights; k=None takes queries alone.
-pos: int64 [B, T] or [T]. Statistics and products are fp32, each output is rounded once. Deterministic.
+pos: int64 [B, T] or [T]. Statistics and products are fp32, each output is rounded once. Deterministic. An output may be its input's own tensor. Nothing
+is recorded for autograd: tensors that require gradients are refused unless under torch.no_grad().
 """
 from __future__ import annotations
 
@@ -17,7 +18,7 @@ import struct
 
 import torch
 
-from ._ops import DTYPES, call, lib, refuse, same_device, workspace
+from ._ops import DTYPES, call, lib, no_grad, output, refuse, same_device, workspace
 
 # ifd_qk_args (include/ifd_ops.h; _ops.QkArgs has the same layout)
 _HEAD, _MORE = struct.Struct("9i2fi 8P 14q"), struct.Struct("6P 12q")
@@ -93,6 +94,7 @@ def _inputs(q, k, wq, wk, pos, rope, eps, norm):
     if not norm and not (wq is None and wk is None):
         refuse("weights without the norm")
     dev = same_device(q, k)
+    no_grad(q, k, wq, wk)
     if wq is not None:
         wq = _weight(wq, D, "wq", dev)
     if wk is not None:
@@ -124,10 +126,9 @@ def _into(t, like, name):
         return None
     if t is None:
         return torch.empty_like(like, memory_format=torch.contiguous_format)
-    if not (t.shape == like.shape and t.dtype == like.dtype and t.device == like.device
-            and (t.stride(3) == 1 or t.shape[3] == 1)):
+    if t.dim() != 4 or (t.stride(3) != 1 and t.shape[3] != 1):
         refuse(f"{name} must be like its input, with adjacent channels")
-    return t
+    return output(t, like, name)
 
 
 def qk_norm_rope(q, k, wq=None, wk=None, pos=None, rope=None, eps=1e-6, norm=True, q_out=None, k_out=None):
@@ -147,6 +148,7 @@ def qk_norm_rope_bwd(gq, gk, q, k, wq=None, wk=None, pos=None, rope=None, eps=1e
     if gq.shape != q.shape or gq.dtype != q.dtype or (k is not None and (gk.shape != k.shape or gk.dtype != k.dtype)):
         refuse("gq, gk must be like q, k")
     same_device(q, gq, gk)
+    no_grad(gq, gk)
     gq, gk = _rows(gq), None if gk is None else _rows(gk)
     dq, dk = _into(dq, q, "dq"), _into(dk, k, "dk")
     dwq = None if wq is None else torch.empty(q.shape[3], dtype=torch.float32, device=dev)

@@ -217,3 +217,15 @@ def test_adamw_python_refusals():
                           (([p, p],), {}, "twice"), (([p],), {}, "GPU tensor"), (([{"params": [p]}, p],), {}, "groups")):
         with pytest.raises(ValueError, match=msg):
             AdamW(*args, **kw)
+
+
+def test_overlap_of_outputs_and_inputs():
+    from ifd.attention import _may_overlap
+    x = torch.zeros(2, 6, 8, 16)
+    q, k, v = x[:, :, :4], x[:, :, 4:6], x[:, :, 6:]
+    assert not _may_overlap(q, k) and not _may_overlap(k, q) and not _may_overlap(v, k) and not _may_overlap(q, torch.zeros_like(q))
+    assert _may_overlap(q, q) and _may_overlap(q, x[:, :, 3:5]) and _may_overlap(x[:, 1:, :4], x[:, :5, :4])
+    assert not _may_overlap(x[:1], x[1:]) and not _may_overlap(x[:, :0], x)
+    assert _may_overlap(x, x.transpose(1, 2))
+    y = torch.zeros(2, 4, 6, 16)  # [B, H, T, D] in memory: other rows, so nothing is told apart
+    assert _may_overlap(y.transpose(1, 2)[:, :, :2], y.transpose(1, 2)[:, :, 1:])

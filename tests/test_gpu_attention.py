@@ -399,3 +399,63 @@ def test_norm_rotation_attention_and_optimizer_together():
         move, gn = (p - b).cpu().double(), r / n
         ok = gn.abs() > 1e-4
         assert ((move + 1e-3 * torch.sign(r))[ok].abs() <= 1e-3 * (1e-8 / 1e-4 + 1e-3) + 2.0 ** -23 * b.cpu().abs()[ok]).all()
+
+
+def test_refusals_that_need_tensors_on_the_gpu():
+    from ifd.attention import attention, attention_bwd
+    from ifd.rotary import qk_norm_rope
+    q, k, v, dout = _inputs(2, 8, 8, 2, 1, 64, BF, seed=0)
+    for kw, msg in ((dict(kv_len=_ints([8])), "kv_len"), (dict(kv_len=_ints([8, 8]).long()), "kv_len"),
+                    (dict(q_start=torch.zeros(2, dtype=torch.int32)), "q_start"), (dict(out=q), "overlaps"),
+                    (dict(out=torch.empty(2, 8, 2, 64, device=DEV)), "like"),
+                    (dict(out=torch.empty(2, 8, 2, 65, dtype=BF, device=DEV)[..., 1:]), "16-byte"),
+                    (dict(out=torch.empty(1, 8, 2, 64, dtype=BF, device=DEV).expand(2, -1, -1, -1)), "share their place")):
+        with pytest.raises(ValueError, match=msg):
+            attention(q, k, v, **kw)
+    with pytest.raises(ValueError, match="GPU tensor"):
+        attention(q, k, v.cpu())
+    out, lse = attention(q, k, v)
+    for kw, msg in ((dict(dq=dout), "overlaps"), (dict(dk=k), "overlaps"), (dict(dv=torch.empty_like(q)), "like")):
+        with pytest.raises(ValueError, match=msg):
+            attention_bwd(dout, q, k, v, out, lse, **kw)
+    with pytest.raises(ValueError, match="lse"):
+        attention_bwd(dout, q, k, v, out, lse[:, :1])
+    p = q.clone().requires_grad_()
+    for call in (lambda: attention(p, k, v), lambda: attention_bwd(dout, p, k, v, out, lse), lambda: qk_norm_rope(p, k)):
+        with pytest.raises(ValueError, match="records no gradients"):
+            call()
+        with torch.no_grad():
+            call()
+    # in-place outputs count as writes: autograd notices a saved tensor that has changed
+    y = (q.clone().requires_grad_() * k[:, :, :1]).sum()
+    kk = k.clone()
+    w = torch.ones(64, device=DEV, dtype=BF, requires_grad=True)
+    y = (w * kk).sum()
+    with torch.no_grad():
+        qk_norm_rope(q, kk, k_out=kk)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+
+
+def test_norm_and_rotation_captured_and_replayed():
+    from ifd.rotary import Rotary, qk_norm_rope, qk_norm_rope_bwd
+    rope = Rotary(64, device=DEV)
+    q, k, _, g = _inputs(4, 1, 1, 8, 2, 64, BF, seed=1)
+    gk = torch.randn_like(k)
+    w = torch.ones(64, device=DEV)
+    pos = torch.zeros(4, 1, dtype=torch.int64, device=DEV)
+    args = (w, w, pos, rope)
+    with torch.cuda.stream(torch.cuda.Stream()):
+        qk_norm_rope(q, k, *args), qk_norm_rope_bwd(g, gk, q, k, *args)
+    torch.cuda.synchronize()
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        a = qk_norm_rope(q, k, *args)
+        b = qk_norm_rope_bwd(g, gk, q, k, *args)
+    for it in range(3):
+        for t in (q, k, g, gk, w):
+            t.copy_(torch.randn(t.shape, device=DEV))
+        pos.fill_(100 * it)
+        gr.replay()
+        torch.cuda.synchronize()
+        assert _same(a, qk_norm_rope(q, k, *args)) and _same(b, qk_norm_rope_bwd(g, gk, q, k, *args))
