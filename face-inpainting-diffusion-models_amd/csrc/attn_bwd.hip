@@ -80,7 +80,7 @@ __global__ __launch_bounds__(256, OCC) void attn_bwd_q_kernel(AttnK p) {
   const char* kp = p.k + b * p.kb + hk * p.kh;
   const char* vp = p.v + b * p.vb + hk * p.vh;
   auto stage = [&](int t) {
-    const int k0 = t * BK, n = min(BK, len - k0);
+    const int k0 = t * BK, n = min(BK, wg_end - k0);
     lds_c* d = sm + (t & 1) * (2 * TB);
     sg.load(kp + (int64_t)k0 * p.kt, p.kt, n, d, w);
     sg.load(vp + (int64_t)k0 * p.vt, p.vt, n, d + TB, w);
@@ -152,7 +152,7 @@ __global__ __launch_bounds__(256, OCC) void attn_bwd_q_kernel(AttnK p) {
       if (ch >= p.D) continue;
       f32x4 v;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = acc[d][4 * j + e] * p.scale;
+      for (int e = 0; e < 4; ++e) v[e] = lim ? acc[d][4 * j + e] * p.scale : 0.f;  // (no key seen: 0, whatever dout holds)
       *reinterpret_cast<typename TL::A::quad*>(op + ch) = __builtin_convertvector(v, typename TL::A::quad);
     }
 }
@@ -183,7 +183,7 @@ __global__ __launch_bounds__(NW * 64, OCC) void attn_bwd_kv_kernel(AttnK p) {
     bh = id / p.nsplit / p.nblk;
   }
   const int b = bh / p.Hk, hk = bh - b * p.Hk;
-  const int len = seq_len(p, b), qs = q_first(p, b);
+  const int qs = q_first(p, b), len = row_limit(p, qs, seq_len(p, b), p.Tq - 1);  // keys that some row sees
   const int kb0 = kblk * (NW * 32), key = kb0 + w * 32 + l32;
   const bool ok = key < len;
   // rows [lo, Tq) see this lane's key, [wg_lo, Tq) some key of the workgroup
@@ -192,6 +192,7 @@ __global__ __launch_bounds__(NW * 64, OCC) void attn_bwd_kv_kernel(AttnK p) {
     return n < 0 ? 0 : (n > p.Tq ? p.Tq : (int)n);
   };
   const int lo = first_row(key), wg_lo = first_row(kb0);
+  const int row0 = first_row(0);  // row tiles begin here: rows that see no key are not read
   const int w_lo = __builtin_amdgcn_readfirstlane(first_row(kb0 + w * 32));
   const int w_hi = __builtin_amdgcn_readfirstlane(first_row(kb0 + w * 32 + 31));
 
@@ -212,7 +213,7 @@ __global__ __launch_bounds__(NW * 64, OCC) void attn_bwd_kv_kernel(AttnK p) {
 #pragma unroll
     for (int x = 0; x < 16; ++x) dk[d][x] = dv[d][x] = 0.f;
 
-  const int tq0 = wg_lo / BQ, ntq = kb0 < len && wg_lo < p.Tq ? (p.Tq + BQ - 1) / BQ - tq0 : 0;
+  const int tq0 = (wg_lo - row0) / BQ, ntq = kb0 < len && wg_lo < p.Tq ? (p.Tq - row0 + BQ - 1) / BQ - tq0 : 0;
   const int64_t all = (int64_t)ntq * p.G;
   const int it0 = (int)(all * sp / p.nsplit), it1 = (int)(all * (sp + 1) / p.nsplit);
   AttnStage<T, DP, BQ, NW> sg;
@@ -224,7 +225,7 @@ __global__ __launch_bounds__(NW * 64, OCC) void attn_bwd_kv_kernel(AttnK p) {
     sg_t = it0 - sg_h * ntq;
   }
   auto stage = [&](int buf) {
-    const int hq = hk * p.G + sg_h, r0 = (tq0 + sg_t) * BQ, n = min(BQ, p.Tq - r0);
+    const int hq = hk * p.G + sg_h, r0 = row0 + (tq0 + sg_t) * BQ, n = min(BQ, p.Tq - r0);
     if (++sg_t == ntq) {
       sg_t = 0;
       ++sg_h;
@@ -262,7 +263,7 @@ __global__ __launch_bounds__(NW * 64, OCC) void attn_bwd_kv_kernel(AttnK p) {
     if (it + 1 < it1) stage(buf ^ 1);
     const lds_c* qb = sm + buf * BUF;
     const lds_c* gb = qb + TB;
-    const int r0 = (tq0 + t) * BQ;
+    const int r0 = row0 + (tq0 + t) * BQ;
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) {
       const int rr = r0 + qt * 32;
@@ -367,7 +368,7 @@ __global__ __launch_bounds__(256) void attn_bwd_join_kernel(AttnK p) {
   const int64_t bh = row / p.Tk;
   const int key = (int)(row - bh * p.Tk), b = (int)(bh / p.Hk), hk = (int)(bh - (int64_t)b * p.Hk);
   f32x4 v = {0.f, 0.f, 0.f, 0.f};
-  if (key < seq_len(p, b)) {
+  if (key < row_limit(p, q_first(p, b), seq_len(p, b), p.Tq - 1)) {
     const float* w = p.ws + 2 * (int64_t)p.B * p.Hq * p.Tq + (bh * p.nsplit * p.Tk + key) * (2 * DP) + isv * DP + ch;
     for (int s = 0; s < p.nsplit; ++s) v += *reinterpret_cast<const f32x4*>(w + (int64_t)s * p.Tk * (2 * DP));
     if (!isv) v *= p.scale;

@@ -209,7 +209,7 @@ __device__ __forceinline__ int seq_len(const AttnK& p, int b) {
   const int n = p.kv_len[b];
   return n < 0 ? 0 : (n > p.Tk ? p.Tk : n);
 }
-// keys that row i of sequence b sees: [0, limit)
+// keys that row i of sequence b sees: [0, limit); what the last of some rows sees bounds what is loaded for them
 __device__ __forceinline__ int row_limit(const AttnK& p, int qs, int len, int i) {
   if (!p.causal) return len;
   const int64_t n = (int64_t)qs + i + 1;  // q_start is any int32

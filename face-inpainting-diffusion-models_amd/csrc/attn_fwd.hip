@@ -125,7 +125,7 @@ __global__ __launch_bounds__(256, OCC) void attn_fwd_kernel(AttnK p) {
   const char* kp = p.k + b * p.kb + hk * p.kh;
   const char* vp = p.v + b * p.vb + hk * p.vh;
   auto stage = [&](int t) {
-    const int k0 = t * BK, n = min(BK, len - k0);
+    const int k0 = t * BK, n = min(BK, wg_end - k0);
     lds_c* d = sm + (t & 1) * (2 * TB);
     sg.load(kp + (int64_t)k0 * p.kt, p.kt, n, d, w);
     sg.load(vp + (int64_t)k0 * p.vt, p.vt, n, d + TB, w);
@@ -247,7 +247,7 @@ __global__ __launch_bounds__(NW * 64) void attn_split_kernel(AttnK p) {
   const char* kp = p.k + b * p.kb + hk * p.kh;
   const char* vp = p.v + b * p.vb + hk * p.vh;
   auto stage = [&](int t, int buf) {
-    const int k0 = t * BK, n = min(BK, len - k0);
+    const int k0 = t * BK, n = min(BK, end - k0);
     lds_c* d = sm + buf * (2 * TB);
     sg.load(kp + (int64_t)k0 * p.kt, p.kt, n, d, 0);
     sg.load(vp + (int64_t)k0 * p.vt, p.vt, n, d + TB, 0);
@@ -394,7 +394,7 @@ const char* attention_check(const ifd_attention_args& a) {
   const int es = (int)dtype_bytes(a.dtype), ce = 16 / es;
   if (a.D > 128 || a.D % ce) return "head width: at most 128, a multiple of 8 (16-bit) or 4 (fp32)";
   if (!(a.scale > 0.f) || !(a.scale < 3e38f)) return "scale must be positive and finite";
-  if (a.Tk > 0x3fffffff || (int64_t)a.Tq * (a.Hq / a.Hk) > 0x3fffffff || (int64_t)a.B * a.Hq > 0x3fffffff) 
+  if (a.Tk > 0x3fffffff || (int64_t)a.Tq * (a.Hq / a.Hk) > 0x3fffffff || (int64_t)a.B * a.Hq > 0x3fffffff)
     return "sizes beyond 2^30 rows";
   return nullptr;
 }
@@ -498,7 +498,7 @@ static int run_fwd(const FwdPlan& pl, AttnK p, hipStream_t s) {
 
 // The UNet's QKVAttention (code/nn.py:222-235) on qkv [N][T][3C]: heads of 64 channels at offsets 0, C, 2C; queries and keys
 // carry `scale` each.
-void launch_attention_rows(const float* qkv, int N, int T, int C, float scale, float* out, hipStream_t s) {
+int launch_attention_rows(const float* qkv, int N, int T, int C, float scale, float* out, hipStream_t s) {
   AttnK p = {};
   p.q = (const char*)qkv; p.k = (const char*)(qkv + C); p.v = (const char*)(qkv + 2 * C);
   p.out = (char*)out;
@@ -509,7 +509,7 @@ void launch_attention_rows(const float* qkv, int N, int T, int C, float scale, f
   p.scale = scale * scale;
   p.c = p.scale * 1.4426950408889634f;
   p.nblk = (int)cdiv(T, 128);
-  (void)run_rows<float, 64>(p, s);  // (the status of the launch is read by the caller)
+  return run_rows<float, 64>(p, s);
 }
 
 }  // namespace ifd

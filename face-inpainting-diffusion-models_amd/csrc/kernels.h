@@ -18,9 +18,9 @@ void launch_temb(const int64_t* t, const float* freqs, int mc, const float* w0t,
                  const float* b2, int E, int N, float* h1, float* emb, hipStream_t s);
 void launch_emb_proj(const float* emb, int E, int N, const float* wt, const float* b, int J, float* out,
                      hipStream_t s);
-void launch_attention(const float* qkv, int N, int T, int C, float scale, float* out, hipStream_t s);
+int launch_attention(const float* qkv, int N, int T, int C, float scale, float* out, hipStream_t s);
 // attn_fwd.hip: the same for any T (C a multiple of 64, N * C / 64 * T / 128 within one launch)
-void launch_attention_rows(const float* qkv, int N, int T, int C, float scale, float* out, hipStream_t s);
+int launch_attention_rows(const float* qkv, int N, int T, int C, float scale, float* out, hipStream_t s);
 void launch_step(int mode, const StepCoeffs& sc, const float* out6, float* img, const float* gt, const float* mask,
                  const float* noise, const float* known, int N, int HW, hipStream_t s);
 // act + AvgPool2d(2,2) of an NHWC tensor (the down-ResBlock's h_upd, code/nn.py:190-195) for the

@@ -317,16 +317,17 @@ __global__ __launch_bounds__(256, 1) void attention_mfma_kernel(const float* __r
 }
 
 template <int KT>
-static void launch_attention_mfma(const float* qkv, int N, int C, float scale, float* out, hipStream_t s) {
+static int launch_attention_mfma(const float* qkv, int N, int C, float scale, float* out, hipStream_t s) {
   constexpr int T = 32 * KT;
   const size_t lds = (size_t)T * (AM_KS + AM_VS) * sizeof(float);
   static bool attr[kMaxDevices] = {};
   (void)set_lds_attr_once(attr, reinterpret_cast<const void*>(&attention_mfma_kernel<KT>), (int)lds);
   dim3 grid((T + 127) / 128, C / AT_CH, N);
   hipLaunchKernelGGL(attention_mfma_kernel<KT>, grid, dim3(256), lds, s, qkv, C, scale, out);
+  return IFD_LAUNCH_STATUS();
 }
 
-void launch_attention(const float* qkv, int N, int T, int C, float scale, float* out, hipStream_t s) {
+int launch_attention(const float* qkv, int N, int T, int C, float scale, float* out, hipStream_t s) {
   // attention_kernel keeps a whole row of scores, 256 at most; longer maps run the tiled kernel with a running softmax
   if (T > 256) return launch_attention_rows(qkv, N, T, C, scale, out, s);
   if (C % AT_CH == 0) {
@@ -337,6 +338,7 @@ void launch_attention(const float* qkv, int N, int T, int C, float scale, float*
   }
   dim3 grid((T + AT_QB - 1) / AT_QB, C / AT_CH, N);
   hipLaunchKernelGGL(attention_kernel, grid, dim3(256), 0, s, qkv, T, C, scale, out);
+  return IFD_LAUNCH_STATUS();
 }
 
 // ---------------------------------------------------------------------------------------------

@@ -3398,8 +3398,7 @@ int ifd_tr_attention(const float* qkv, int N, int T, int C, float scale, float* 
   if (C % 64) { set_error("ifd_tr_attention: 64-channel heads"); return 2; }
   if (T < 1 || N < 0 || ((int64_t)T + 127) / 128 * (C / 64) * N > 0x7fffffff) { set_error("ifd_tr_attention: sizes"); return 2; }
   if (!N) return 0;
-  launch_attention(qkv, N, T, C, scale, out, (hipStream_t)stream);
-  return TR_LAST();
+  return launch_attention(qkv, N, T, C, scale, out, (hipStream_t)stream);
 }
 
 int64_t ifd_tr_attention_bwd_scratch_floats(int N, int T, int C) { return 2 * (int64_t)N * (C / 64) * T * T; }

@@ -1120,8 +1120,9 @@ int Model::run_attn(const AttnP& a, const float* in, int N, int Hin, float* out,
   const float scale = (float)(1.0 / std::sqrt(std::sqrt((double)cfg_.num_head_channels)));
   IFD_REQUIRE(cfg_.num_head_channels == 64, "attention kernel is specialised for 64-channel heads");
   prof_begin(s, &g0, "attention_kernel");
-  launch_attention(qkv, N, T, a.C, scale, ao, s);
+  e = launch_attention(qkv, N, T, a.C, scale, ao, s);
   prof_end(s, g0, "attention_kernel", 4.0 * N * (double)T * T * a.C, 4.0 * N * (double)T * a.C * 4);
+  IFD_LAUNCH_OK(e, "attention");
   return run_conv(a.proj, ao, a.C, nullptr, 0, N, Hin, Hin, XF_NONE, ACT_NONE, nullptr, nullptr, nullptr, 0, nullptr,
                   0, in, XF_NONE, Hin, out, EPI_NHWC, s);
 }

@@ -116,6 +116,22 @@ def output(t, like, name):
     return t
 
 
+def may_overlap(a, b):
+    """Whether two [batch, tokens, heads, channels] tensors could share elements. Told apart: other storages, ranges one
+    behind the other, and different channel ranges of the same token rows (slices of one packed buffer)."""
+    if a.untyped_storage().data_ptr() != b.untyped_storage().data_ptr() or not a.numel() or not b.numel():
+        return False
+    end = lambda t: t.storage_offset() + sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1  # noqa: E731
+    if min(a.stride() + b.stride()) < 0 or a.storage_offset() >= end(b) or b.storage_offset() >= end(a):
+        return min(a.stride() + b.stride()) < 0
+    row = a.stride(1)
+    if a.stride()[:2] != b.stride()[:2] or row <= 0 or a.stride(0) % row:
+        return True
+    lo = [t.storage_offset() % row for t in (a, b)]
+    hi = [o + (t.shape[2] - 1) * t.stride(2) + t.shape[3] for o, t in zip(lo, (a, b))]
+    return max(hi) > row or not (hi[0] <= lo[1] or hi[1] <= lo[0])
+
+
 def workspace(nbytes, dev):
     """Scratch of one call, from torch's stream-ordered allocator (None when the call needs none)."""
     return torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None

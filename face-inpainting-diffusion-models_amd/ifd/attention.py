@@ -10,8 +10,10 @@ three slices of a packed projection or a slice of a longer key-value cache; tens
 
 Row i of sequence b sees key j when j < kv_len[b] (default Tk) and, with causal=True, j <= q_start[b] + i (default
 Tk - Tq: the rows are the last ones). kv_len, q_start: int32 [B] on the GPU, read by the kernels (no synchronisation).
-Keys at and past kv_len are never read, whatever they hold. A row that sees no key gets out = 0, lse = -inf and zero
-gradients. Output tensors of the caller (out, dq, dk, dv) must not overlap the inputs. Keys that only the causal mask hides are read: v must be finite there, for the backward pass k too.
+Keys that no row of their sequence sees (at and past kv_len, or behind the last row's) change nothing, whatever they hold.
+A key that some rows see and others not must be finite in v (for the backward pass in k too), or it may spoil those others.
+A row that sees no key gets out = 0, lse = -inf and zero gradients, whatever q and dout hold there. Output tensors of the
+caller (out, dq, dk, dv) must not overlap the inputs nor each other.
 
 The backward pass keeps no score matrix: it recomputes the probabilities from lse. Both directions are deterministic.
 Calls run on the current stream of the tensors' device and can be captured into a graph. They record nothing for autograd:
@@ -24,7 +26,7 @@ import struct
 
 import torch
 
-from ._ops import DTYPES, call, lib, no_grad, output, refuse, same_device, workspace
+from ._ops import DTYPES, call, lib, may_overlap as _may_overlap, no_grad, output, refuse, same_device, workspace
 
 # ifd_attention_args (include/ifd_ops.h): packed here because filling a ctypes structure field by field costs more than
 # the smallest kernels run (_ops.AttentionArgs has the same layout)
@@ -83,22 +85,6 @@ def _pack(q, k, v, scale, causal, kv_len, q_start, out, lse):
                      *out.stride()[:3])
 
 
-def _may_overlap(a, b):
-    """Whether two [batch, tokens, heads, channels] tensors could share elements. Told apart: other storages, ranges one
-    behind the other, and different channel ranges of the same token rows (slices of one packed buffer)."""
-    if a.untyped_storage().data_ptr() != b.untyped_storage().data_ptr() or not a.numel() or not b.numel():
-        return False
-    end = lambda t: t.storage_offset() + sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1  # noqa: E731
-    if min(a.stride() + b.stride()) < 0 or a.storage_offset() >= end(b) or b.storage_offset() >= end(a):
-        return min(a.stride() + b.stride()) < 0
-    row = a.stride(1)
-    if a.stride()[:2] != b.stride()[:2] or row <= 0 or a.stride(0) % row:
-        return True
-    lo = [t.storage_offset() % row for t in (a, b)]
-    hi = [o + (t.shape[2] - 1) * t.stride(2) + t.shape[3] for o, t in zip(lo, (a, b))]
-    return max(hi) > row or not (hi[0] <= lo[1] or hi[1] <= lo[0])
-
-
 def _into(t, like, name, *inputs):
     """A caller's output tensor (checked) or a new contiguous one."""
     if t is None:
@@ -106,7 +92,7 @@ def _into(t, like, name, *inputs):
     if not (t.dim() == 4 and _lay(t) is t):
         refuse(f"{name}: adjacent channels, 16-byte aligned, strides in multiples of 16 bytes")
     if any(_may_overlap(t, x) for x in inputs):
-        refuse(f"{name} overlaps an input")
+        refuse(f"{name} overlaps an input or another output")
     return output(t, like, name)
 
 
@@ -136,7 +122,9 @@ def attention_bwd(dout, q, k, v, out, lse, scale=None, causal=False, kv_len=None
     no_grad(dout, out)
     dout, out, lse = _lay(dout), _lay(out), lse.contiguous()
     ins = (q, k, v, dout, out)
-    dq, dk, dv = _into(dq, q, "dq", *ins), _into(dk, k, "dk", *ins), _into(dv, v, "dv", *ins)
+    dq = _into(dq, q, "dq", *ins)
+    dk = _into(dk, k, "dk", *ins, dq)
+    dv = _into(dv, v, "dv", *ins, dq, dk)
     a = _pack(q, k, v, scale, causal, kv_len, q_start, out, lse) + _BWD.pack(
         dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), *dout.stride()[:3], *dq.stride()[:3],
         *dk.stride()[:3], *dv.stride()[:3])

@@ -50,6 +50,8 @@ class AdamW:
             need(p.dtype in DTYPES and p.is_contiguous(), "parameters must be contiguous fp32, bf16 or fp16 tensors")
         need(len({id(p) for p in self.params}) == len(self.params), "a parameter is listed twice")
         self.device = same_device(*self.params)
+        at = sorted((p.data_ptr(), p.data_ptr() + p.numel() * p.element_size()) for p in self.params if p.numel())
+        need(all(a[1] <= b[0] for a, b in zip(at, at[1:])), "two parameters share memory")
         at = 0
         for g in self.groups:
             g["block0"] = at

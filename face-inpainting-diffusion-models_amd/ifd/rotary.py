@@ -8,8 +8,9 @@ q: [B, T, Hq, D], k: [B, T, Hk, D], one type (fp32, bf16, fp16), D <= 128 and ev
 slices of a packed projection). n = x / sqrt(mean x^2 + eps) * w over each head's channels; the first `rope.rot` channels
 are then turned in pairs by the angle pos * inv_freq (fp64, so that far positions keep their angle) and scaled by
 rope.mscale. norm=False leaves out the norm, rope=None the rotation, wq / wk=None the weights; k=None takes queries alone.
-pos: int64 [B, T] or [T]. Statistics and products are fp32, each output is rounded once. Deterministic. An output may be its input's own tensor. Nothing
-is recorded for autograd: tensors that require gradients are refused unless under torch.no_grad().
+pos: int64 [B, T] or [T]. Statistics and products are fp32, each output is rounded once. Deterministic. An output may be the
+tensor of its own input (of its own gradient, backward) and must else overlap no input and no other output. Nothing is
+recorded for autograd: tensors that require gradients are refused unless under torch.no_grad().
 """
 from __future__ import annotations
 
@@ -18,7 +19,7 @@ import struct
 
 import torch
 
-from ._ops import DTYPES, call, lib, no_grad, output, refuse, same_device, workspace
+from ._ops import DTYPES, call, lib, may_overlap, no_grad, output, refuse, same_device, workspace
 
 # ifd_qk_args (include/ifd_ops.h; _ops.QkArgs has the same layout)
 _HEAD, _MORE = struct.Struct("9i2fi 8P 14q"), struct.Struct("6P 12q")
@@ -121,20 +122,27 @@ def _pack(q, k, wq, wk, pos, rope, eps, norm, q_out, k_out):
                       *q.stride()[:3], *ks, *qos, *kos, *ps)
 
 
-def _into(t, like, name):
+def _into(t, like, name, place, *others):
+    """A caller's output (checked) or a new one. It may be `place` itself (each head is read, then written, by the same
+    lanes), else it must be apart from it, and from `others` in any case."""
     if like is None:
         return None
     if t is None:
         return torch.empty_like(like, memory_format=torch.contiguous_format)
     if t.dim() != 4 or (t.stride(3) != 1 and t.shape[3] != 1):
         refuse(f"{name} must be like its input, with adjacent channels")
+    if t is not place and t.data_ptr() == place.data_ptr() and t.stride() == place.stride():
+        place = t
+    if (t is not place and may_overlap(t, place)) or any(x is not None and may_overlap(t, x) for x in others):
+        refuse(f"{name} overlaps an input or another output")
     return output(t, like, name)
 
 
 def qk_norm_rope(q, k, wq=None, wk=None, pos=None, rope=None, eps=1e-6, norm=True, q_out=None, k_out=None):
     """(q_out, k_out); q_out=q and k_out=k work in place. k=None: (q_out, None)."""
     q, k, wq, wk, dev = _inputs(q, k, wq, wk, pos, rope, eps, norm)
-    q_out, k_out = _into(q_out, q, "q_out"), _into(k_out, k, "k_out")
+    q_out = _into(q_out, q, "q_out", q, k)
+    k_out = _into(k_out, k, "k_out", k, q, q_out)
     call(lib().ifd_op_qk_norm_rope, dev, _pack(q, k, wq, wk, pos, rope, eps, norm, q_out, k_out) + _NO_BWD)
     return q_out, k_out
 
@@ -150,7 +158,8 @@ def qk_norm_rope_bwd(gq, gk, q, k, wq=None, wk=None, pos=None, rope=None, eps=1e
     same_device(q, gq, gk)
     no_grad(gq, gk)
     gq, gk = _rows(gq), None if gk is None else _rows(gk)
-    dq, dk = _into(dq, q, "dq"), _into(dk, k, "dk")
+    dq = _into(dq, q, "dq", gq, q, k, gk)
+    dk = _into(dk, k, "dk", gk, q, k, gq, dq)
     dwq = None if wq is None else torch.empty(q.shape[3], dtype=torch.float32, device=dev)
     dwk = None if wk is None else torch.empty(q.shape[3], dtype=torch.float32, device=dev)
     gkp, gks = _ptr_st(gk)

@@ -24,8 +24,9 @@ extern "C" {
  * {batch, token, head} in elements, the channel stride is 1. Hq is a multiple of Hk: query head h reads key-value head
  * h / (Hq / Hk). lse is fp32 [B][Hq][Tq], contiguous.
  * Row i of sequence b sees key j when j < kv_len[b] (NULL: Tk; values are clamped to [0, Tk]) and, with causal != 0,
- * j <= q_start[b] + i (NULL: q_start = Tk - Tq). A row that sees no key gets out 0, lse -inf and no gradient. Keys at
- * and past kv_len are not read; their dk, dv are written as zeros.
+ * j <= q_start[b] + i (NULL: q_start = Tk - Tq). A row that sees no key gets out 0, lse -inf and no gradient, whatever q
+ * and dout hold there. Keys that no row of their sequence sees (at and past kv_len, or behind the last row's) are not
+ * read; their dk, dv are written as zeros. A key that some rows see must be finite in v (backward: in k too).
  * D <= 128 and a multiple of 8 (16-bit types) or 4 (fp32); pointers and strides in multiples of 16 bytes; scale > 0.
  * Scores, softmax statistics and every sum are fp32. The 16-bit types round P (and dS) once to the tensors' type as
  * operands of the second matrix products. */

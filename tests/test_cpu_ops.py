@@ -229,3 +229,27 @@ def test_overlap_of_outputs_and_inputs():
     assert _may_overlap(x, x.transpose(1, 2))
     y = torch.zeros(2, 4, 6, 16)  # [B, H, T, D] in memory: other rows, so nothing is told apart
     assert _may_overlap(y.transpose(1, 2)[:, :, :2], y.transpose(1, 2)[:, :, 1:])
+
+
+def test_overlap_of_parameters_and_of_two_outputs(monkeypatch):
+    from ifd import _ops, attention, optim, rotary
+    for m in (_ops, attention, optim, rotary):
+        if hasattr(m, "same_device"):
+            monkeypatch.setattr(m, "same_device", lambda *t: t[0].device)
+    x = torch.zeros(100)
+    with pytest.raises(ValueError, match="share memory"):
+        optim.AdamW([x[:60], x[50:]])
+    optim.AdamW([x[:50], x[50:], x[:0]])
+    q, k = torch.zeros(1, 3, 2, 16), torch.zeros(1, 3, 2, 16)
+    o = torch.zeros(1, 3, 4, 16)
+    with pytest.raises(ValueError, match="k_out overlaps"):
+        rotary.qk_norm_rope(q, k, q_out=o[:, :, :2], k_out=o[:, :, 1:3])
+    with pytest.raises(ValueError, match="q_out overlaps"):
+        rotary.qk_norm_rope(q, k, q_out=k)
+    with pytest.raises(ValueError, match="q_out overlaps"):
+        rotary.qk_norm_rope(o[:, :, :2], None, q_out=o[:, :, 1:3])
+    with pytest.raises(ValueError, match="dq overlaps"):
+        rotary.qk_norm_rope_bwd(q.clone(), k.clone(), q, k, dq=q)
+    lse = torch.zeros(1, 2, 3)
+    with pytest.raises(ValueError, match="dv overlaps"):
+        attention.attention_bwd(q.clone(), q, k, k.clone(), q.clone(), lse, dk=o[:, :, :2], dv=o[:, :, :2])

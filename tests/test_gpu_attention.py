@@ -459,3 +459,23 @@ def test_norm_and_rotation_captured_and_replayed():
         gr.replay()
         torch.cuda.synchronize()
         assert _same(a, qk_norm_rope(q, k, *args)) and _same(b, qk_norm_rope_bwd(g, gk, q, k, *args))
+
+
+@pytest.mark.parametrize("Tq,dt,D", [(1, BF, 64), (40, HF, 128), (200, F32, 64), (200, BF, 128), (333, BF, 96)])
+def test_anything_behind_the_last_row_and_in_rows_without_keys(Tq, dt, D):
+    """A cache's unused end without kv_len (causal, q_start tells where the rows are), and rows before the first key: what
+    the keys that no row sees, and q and dout of the rows that see no key, hold changes nothing."""
+    B, Tk, Hq, Hk = 3, 500, 4, 2
+    q, k, v, dout = _inputs(B, Tq, Tk, Hq, Hk, D, dt, seed=Tq + 1)
+    start = [100, 0, -Tq // 3 if Tq > 1 else -1]
+    kw = dict(causal=True, q_start=_ints(start))
+    want = _both(q, k, v, dout, **kw)
+    r = _ref(q, k, v, _visible(B, Tq, Tk, True, None, start), D ** -0.5, dout, want[0])
+    _check_fwd(want[0], want[1], r, dt)
+    _check_bwd(*want[2:], r, dt)
+    for junk in (float("nan"), float("inf"), -float("inf")):
+        q2, k2, v2, d2 = q.clone(), k.clone(), v.clone(), dout.clone()
+        for b, s in enumerate(start):
+            k2[b, max(s + Tq, 0):], v2[b, max(s + Tq, 0):] = junk, junk
+            q2[b, :max(-s, 0)], d2[b, :max(-s, 0)] = junk, junk
+        assert _same(_both(q2, k2, v2, d2, **kw), want), junk
