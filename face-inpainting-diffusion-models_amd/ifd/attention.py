@@ -53,17 +53,18 @@ def _int_arg(t, B, name, dev):
 
 def _inputs(q, k, v, scale, kv_len, q_start):
     """Checked inputs: (q, k, v as the kernels read them, scale, kv_len, q_start, device)."""
+    dt = q.dtype
     if not q.dim() == k.dim() == v.dim() == 4:
         refuse("q, k, v must be [batch, tokens, heads, channels]")
     B, _, Hq, D = q.shape
     kB, Tk, Hk, kD = k.shape
-    if not (q.dtype in DTYPES and k.dtype == q.dtype and v.dtype == q.dtype):
+    if not (dt in DTYPES and k.dtype is dt and v.dtype is dt):
         refuse(f"q, k, v must have one type, fp32, bf16 or fp16, got {q.dtype}, {k.dtype}, {v.dtype}")
     if kB != B or kD != D or v.shape != k.shape:
         refuse(f"k, v must be [{B}, tokens, heads, {D}] and alike, got {tuple(k.shape)} and {tuple(v.shape)}")
     if not (Hk > 0 and Hq > 0 and Hq % Hk == 0):
         refuse(f"{Hq} query heads are not a multiple of {Hk} key-value heads")
-    if not 0 < D <= 128 or D * q.element_size() & 15:
+    if not 0 < D <= 128 or D & (3 if dt is torch.float32 else 7):
         refuse(f"head width {D}: at most 128 and a multiple of {16 // q.element_size()}")
     scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
     if not 0.0 < scale < 3e38:

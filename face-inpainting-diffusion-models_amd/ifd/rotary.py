@@ -65,17 +65,15 @@ class Rotary:
 
 
 def _rows(t):
-    return t if t.stride(3) == 1 or t.shape[3] == 1 else t.contiguous()
+    return t if t.stride()[3] == 1 or t.shape[3] == 1 else t.contiguous()
 
 
 def _weight(w, D, name, dev):
+    if w.dtype is torch.float32 and w.shape == (D,) and w.device == dev and w.is_contiguous():
+        return w
     if not (w.shape == (D,) and w.is_floating_point() and w.device == dev):
         refuse(f"{name} must be a float [{D}] on {dev}")
-    return w if w.dtype == torch.float32 and w.is_contiguous() else w.detach().float().contiguous()
-
-
-def _ptr_st(t):
-    return (0, _NO_ST) if t is None else (t.data_ptr(), t.stride()[:3])
+    return w.detach().float().contiguous()
 
 
 def _inputs(q, k, wq, wk, pos, rope, eps, norm):
@@ -84,8 +82,10 @@ def _inputs(q, k, wq, wk, pos, rope, eps, norm):
     B, T, _, D = q.shape
     if q.dtype not in DTYPES or (k is not None and k.dtype != q.dtype):
         refuse("q, k must have one type: fp32, bf16 or fp16")
-    if k is not None and (k.shape[0] != B or k.shape[1] != T or k.shape[3] != D):
-        refuse(f"k must be [{B}, {T}, heads, {D}], got {tuple(k.shape)}")
+    if k is not None:
+        kB, kT, _, kD = k.shape
+        if kB != B or kT != T or kD != D:
+            refuse(f"k must be [{B}, {T}, heads, {D}], got {tuple(k.shape)}")
     if not 0 < D <= 128 or D & 1:
         refuse(f"head width {D}: at most 128 and even")
     if not eps >= 0.0:
@@ -101,7 +101,7 @@ def _inputs(q, k, wq, wk, pos, rope, eps, norm):
     if wk is not None:
         wk = _weight(wk, D, "wk", dev)
     if rope is not None:
-        if pos.dtype != torch.int64 or pos.shape not in ((B, T), (T,)):
+        if pos.dtype is not torch.int64 or pos.shape not in ((B, T), (T,)):
             refuse(f"pos must be int64 [{B}, {T}] or [{T}]")
         if pos.device != dev or rope.turns.device != dev:
             refuse(f"pos and the rotation's frequencies must be on {dev}")
@@ -110,14 +110,14 @@ def _inputs(q, k, wq, wk, pos, rope, eps, norm):
 
 def _pack(q, k, wq, wk, pos, rope, eps, norm, q_out, k_out):
     B, T, Hq, D = q.shape
-    kp, ks = _ptr_st(k)
-    qo, qos = _ptr_st(q_out)
-    ko, kos = _ptr_st(k_out)
+    kp, ks, Hk = (0, _NO_ST, 0) if k is None else (k.data_ptr(), k.stride()[:3], k.shape[2])
+    qo, qos = (0, _NO_ST) if q_out is None else (q_out.data_ptr(), q_out.stride()[:3])
+    ko, kos = (0, _NO_ST) if k_out is None else (k_out.data_ptr(), k_out.stride()[:3])
     rot, il, ms, pp, tp, ps = 0, 0, 1.0, 0, 0, (0, 0)
     if rope is not None:
         rot, il, ms, pp, tp = rope.rot, rope.interleaved, rope.mscale, pos.data_ptr(), rope.turns.data_ptr()
         ps = pos.stride() if pos.dim() == 2 else (0, pos.stride(0))
-    return _HEAD.pack(DTYPES[q.dtype], B, T, Hq, 0 if k is None else k.shape[2], D, rot, il, 1 if norm else 0, eps, ms, 0,
+    return _HEAD.pack(DTYPES[q.dtype], B, T, Hq, Hk, D, rot, il, 1 if norm else 0, eps, ms, 0,
                       q.data_ptr(), kp, qo, ko, 0 if wq is None else wq.data_ptr(), 0 if wk is None else wk.data_ptr(), pp, tp,
                       *q.stride()[:3], *ks, *qos, *kos, *ps)
 
@@ -162,8 +162,7 @@ def qk_norm_rope_bwd(gq, gk, q, k, wq=None, wk=None, pos=None, rope=None, eps=1e
     dk = _into(dk, k, "dk", gk, q, k, gq, dq)
     dwq = None if wq is None else torch.empty(q.shape[3], dtype=torch.float32, device=dev)
     dwk = None if wk is None else torch.empty(q.shape[3], dtype=torch.float32, device=dev)
-    gkp, gks = _ptr_st(gk)
-    dkp, dks = _ptr_st(dk)
+    gkp, gks, dkp, dks = (0, _NO_ST, 0, _NO_ST) if k is None else (gk.data_ptr(), gk.stride()[:3], dk.data_ptr(), dk.stride()[:3])
     a = _pack(q, k, wq, wk, pos, rope, eps, norm, None, None) + _MORE.pack(
         gq.data_ptr(), gkp, dq.data_ptr(), dkp, 0 if dwq is None else dwq.data_ptr(), 0 if dwk is None else dwk.data_ptr(),
         *gq.stride()[:3], *gks, *dq.stride()[:3], *dks)
