@@ -4,30 +4,30 @@
 // Two passes, each owning its outputs, so that nothing is added atomically and the result does not depend on timing:
 // attn_bwd_q_kernel (a wave owns 32 query rows; three products per score tile) also leaves each row's lse2 and delta for
 // attn_bwd_kv_kernel (a wave owns 32 keys; four products). Seven products against the five of one pass with atomics on dq.
+// Short calls run both side by side in one launch (attn_bwd_both_kernel).
 #include "attn_dev.h"
 
 namespace ifd {
 
 // (waves and tiles as in the forward kernel)
-template <typename T, int DP, int BK, int AHEAD, int OCC>
-__global__ __launch_bounds__(256, OCC) void attn_bwd_q_kernel(AttnK p) {
+template <typename T, int DP, int BK, int AHEAD, bool STATS>
+__device__ __forceinline__ void attn_bwd_q(const AttnK& p, lds_c* sm, int blk) {
   typedef AttnTile<T, DP> TL;
   typedef typename TL::frag frag;
   constexpr int NW = 4, KT = BK / 32, TB = BK * TL::ROWB;
-  extern __shared__ __attribute__((aligned(1024))) char smem[];
-  lds_c* sm = (lds_c*)smem;
+  const int nblk = (p.Tq + NW * 32 - 1) / (NW * 32);
   const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, h = lane >> 5;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int BH = p.B * p.Hq;
   int bh, qblk;
   if (p.causal) {
-    const int r = blockIdx.x % BH;
-    qblk = p.nblk - 1 - blockIdx.x / BH;
+    const int r = blk % BH;
+    qblk = nblk - 1 - blk / BH;
     bh = (BH & 7) ? r : (r & 7) * (BH >> 3) + (r >> 3);
   } else {
-    const int id = xcd_order(blockIdx.x, BH * p.nblk);
-    bh = id / p.nblk;
-    qblk = id - bh * p.nblk;
+    const int id = xcd_order(blk, BH * nblk);
+    bh = id / nblk;
+    qblk = id - bh * nblk;
   }
   const int b = bh / p.Hq, hq = bh - b * p.Hq, hk = hq / p.G;
   const int len = seq_len(p, b), qs = q_first(p, b);
@@ -58,7 +58,7 @@ __global__ __launch_bounds__(256, OCC) void attn_bwd_q_kernel(AttnK p) {
     const float l = p.lse[srow];
     if (l != -INFINITY) lse2 = l * 1.4426950408889634f;
     if (lim == 0) delta = 0.f;
-    if (h == 0) {
+    if (STATS && h == 0) {
       p.ws[srow] = lse2;
       p.ws[(int64_t)p.B * p.Hq * p.Tq + srow] = delta;
     }
@@ -159,28 +159,28 @@ __global__ __launch_bounds__(256, OCC) void attn_bwd_q_kernel(AttnK p) {
 
 // A workgroup owns NW * 32 keys of one key-value head and walks over the (query head, row tile) pairs of its share:
 // with nsplit > 1 the pairs are dealt to nsplit workgroups, whose fp32 sums attn_bwd_join_kernel adds in order.
-template <typename T, int DP, int NW, int BQ, bool VL, int OCC>
-__global__ __launch_bounds__(NW * 64, OCC) void attn_bwd_kv_kernel(AttnK p) {
+// FUSED: lse2 and delta of the share's rows are found here, ahead of the walk, instead of read from the row pass.
+template <typename T, int DP, int NW, int BQ, bool VL, bool FUSED>
+__device__ __forceinline__ void attn_bwd_kv(const AttnK& p, lds_c* sm, int blk) {
   typedef AttnTile<T, DP> TL;
   typedef typename TL::frag frag;
-  constexpr int QT = BQ / 32, TB = BQ * TL::ROWB, BUF = 2 * TB + 1024;  // Q, dout, lse2[BQ], delta[BQ]
-  extern __shared__ __attribute__((aligned(1024))) char smem[];
-  lds_c* sm = (lds_c*)smem;
+  constexpr int QT = BQ / 32, TB = BQ * TL::ROWB, BUF = 2 * TB + (FUSED ? 0 : 1024);  // Q, dout, lse2[BQ], delta[BQ]
+  const int nblk = (p.Tk + NW * 32 - 1) / (NW * 32);
   const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, h = lane >> 5;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   // causal: the first key blocks see most rows and go first, a head's on one XCD; else head by head on each XCD
   int sp, kblk, bh;
   if (p.causal) {
     const int n = p.B * p.Hk * p.nsplit;
-    const int r = blockIdx.x % n, x = (n & 7) ? r : (r & 7) * (n >> 3) + (r >> 3);
-    kblk = blockIdx.x / n;
+    const int r = blk % n, x = (n & 7) ? r : (r & 7) * (n >> 3) + (r >> 3);
+    kblk = blk / n;
     bh = x / p.nsplit;
     sp = x - bh * p.nsplit;
   } else {
-    const int id = xcd_order(blockIdx.x, gridDim.x);
+    const int id = xcd_order(blk, nblk * p.B * p.Hk * p.nsplit);
     sp = id % p.nsplit;
-    kblk = (id / p.nsplit) % p.nblk;
-    bh = id / p.nsplit / p.nblk;
+    kblk = (id / p.nsplit) % nblk;
+    bh = id / p.nsplit / nblk;
   }
   const int b = bh / p.Hk, hk = bh - b * p.Hk;
   const int qs = q_first(p, b), len = row_limit(p, qs, seq_len(p, b), p.Tq - 1);  // keys that some row sees
@@ -198,6 +198,7 @@ __global__ __launch_bounds__(NW * 64, OCC) void attn_bwd_kv_kernel(AttnK p) {
 
   frag kf[TL::KS], vf[VL ? 1 : TL::KS];
   const lds_c* vt = sm + 2 * BUF;  // VL: the workgroup's V rows stay in LDS, for want of registers
+  lds_c* tab = sm + 2 * BUF + (VL ? NW * 32 * TL::ROWB : 0);  // FUSED: lse2[32], delta[32] of each 32 rows of the share
   {
     const char* rk = p.k + b * p.kb + hk * p.kh + (int64_t)key * p.kt;
     const char* rv = p.v + b * p.vb + hk * p.vh + (int64_t)key * p.vt;
@@ -233,7 +234,7 @@ __global__ __launch_bounds__(NW * 64, OCC) void attn_bwd_kv_kernel(AttnK p) {
     lds_c* d = sm + buf * BUF;
     sg.load(p.q + b * p.qb + hq * p.qh + (int64_t)r0 * p.qt, p.qt, n, d, w);
     sg.load(p.dout + b * p.gb + hq * p.gh + (int64_t)r0 * p.gt, p.gt, n, d + TB, w);
-    if (w < 2) {  // lse2 by wave 0, delta by wave 1
+    if (!FUSED && w < 2) {  // lse2 by wave 0, delta by wave 1
       const float* st = p.ws + (w ? (int64_t)p.B * p.Hq * p.Tq : 0) + ((int64_t)b * p.Hq + hq) * p.Tq + r0;
       dma_word(st, 4 * min(lane, n - 1), d + 2 * TB + w * 512);
     }
@@ -244,7 +245,36 @@ __global__ __launch_bounds__(NW * 64, OCC) void attn_bwd_kv_kernel(AttnK p) {
       sv.init(w, lane, p.D);
       sv.load(p.v + b * p.vb + hk * p.vh + (int64_t)kb0 * p.vt, p.vt, min(NW * 32, len - kb0), sm + 2 * BUF, w);
     }
+    const int h0 = sg_h, t0 = sg_t;
     stage(0);
+    if (FUSED) {
+      int hq = hk * p.G + h0, tt = t0, qt = w;  // this wave's 32 rows: row tile tt, part qt
+      for (int x = w; x < (it1 - it0) * QT; x += NW, qt += NW) {
+        for (; qt >= QT; qt -= QT)
+          if (++tt == ntq) {
+            tt = 0;
+            ++hq;
+          }
+        const int i = row0 + (tq0 + tt) * BQ + qt * 32 + l32;
+        const bool in = i < p.Tq;
+        const char* rg = p.dout + b * p.gb + hq * p.gh + (int64_t)i * p.gt;
+        const char* ro = p.out + b * p.ob + hq * p.oh + (int64_t)i * p.ot;
+        float delta = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < TL::KS; ++ks) {
+          const frag gf = TL::gload(rg, in, ks, h, p.D), of = TL::gload(ro, in, ks, h, p.D);
+#pragma unroll
+          for (int j = 0; j < TL::CE; ++j) delta = fmaf((float)gf[j], (float)of[j], delta);
+        }
+        delta += xhalf(delta);
+        if (h == 0) {
+          const float l = in ? p.lse[((int64_t)b * p.Hq + hq) * p.Tq + i] : -INFINITY;
+          auto* st = (__attribute__((address_space(3))) float*)(tab + x * 256) + l32;
+          st[0] = l == -INFINITY ? INFINITY : l * 1.4426950408889634f;
+          st[32] = delta;
+        }
+      }
+    }
     dma_wait();
     if (VL && p.D < DP) {
       // both factors of dp come from LDS here: V's channels past D must be zeros
@@ -290,8 +320,9 @@ __global__ __launch_bounds__(NW * 64, OCC) void attn_bwd_kv_kernel(AttnK p) {
       }
 #pragma unroll
       for (int y = 0; y < 4; ++y) {
-        const f32x4 ls = lds_quad(qb + 2 * TB + 4 * (qt * 32 + 8 * y + 4 * h));
-        const f32x4 de = lds_quad(qb + 2 * TB + 512 + 4 * (qt * 32 + 8 * y + 4 * h));
+        const lds_c* st = FUSED ? tab + ((it - it0) * QT + qt) * 256 : qb + 2 * TB + 4 * (qt * 32);
+        const f32x4 ls = lds_quad(st + 4 * (8 * y + 4 * h));
+        const f32x4 de = lds_quad(st + (FUSED ? 128 : 512) + 4 * (8 * y + 4 * h));
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int x = 4 * y + e;
@@ -355,6 +386,26 @@ __global__ __launch_bounds__(NW * 64, OCC) void attn_bwd_kv_kernel(AttnK p) {
     }
 }
 
+template <typename T, int DP, int BK, int AHEAD, int OCC>
+__global__ __launch_bounds__(256, OCC) void attn_bwd_q_kernel(AttnK p) {
+  extern __shared__ __attribute__((aligned(1024))) char smem[];
+  attn_bwd_q<T, DP, BK, AHEAD, true>(p, (lds_c*)smem, blockIdx.x);
+}
+template <typename T, int DP, int NW, int BQ, bool VL, int OCC>
+__global__ __launch_bounds__(NW * 64, OCC) void attn_bwd_kv_kernel(AttnK p) {
+  extern __shared__ __attribute__((aligned(1024))) char smem[];
+  attn_bwd_kv<T, DP, NW, BQ, VL, false>(p, (lds_c*)smem, blockIdx.x);
+}
+// Both passes side by side: the first nq workgroups take rows, the others keys.
+template <typename T, int DP, int BK, int AHEAD, int BQ, bool VL, int OCC>
+__global__ __launch_bounds__(256, OCC) void attn_bwd_both_kernel(AttnK p, int nq) {
+  extern __shared__ __attribute__((aligned(1024))) char smem[];
+  if ((int)blockIdx.x < nq)
+    attn_bwd_q<T, DP, BK, AHEAD, false>(p, (lds_c*)smem, blockIdx.x);
+  else
+    attn_bwd_kv<T, DP, 4, BQ, VL, true>(p, (lds_c*)smem, blockIdx.x - nq);
+}
+
 // dk, dv = the shares' sums in order; one thread per four channels of a (key, dk | dv) row.
 template <typename T, int DP>
 __global__ __launch_bounds__(256) void attn_bwd_join_kernel(AttnK p) {
@@ -378,46 +429,58 @@ __global__ __launch_bounds__(256) void attn_bwd_join_kernel(AttnK p) {
   *reinterpret_cast<quad*>(o + ch) = __builtin_convertvector(v, quad);
 }
 
-// Workgroups of the key pass: 128 keys each, two per CU at a time. The walk is shared out until they fill the chip once, or
-// twice where a causal mask makes them unlike (2 x 4 heads x 4096 keys x 128: 518 us at 512 workgroups, 343 at 1024, 362 at
-// 2048; without a mask more shares only add sums to join: 4 x 8 x 1024 x 128, 62 + 25 us at 1024, 54 + 14 at 512), at least
-// four row tiles each.
+// Shares of the key pass: workgroups of 128 keys (two per CU at a time) deal their walk out among each other. With a causal
+// mask, whose workgroups are unlike, until they fill the chip twice (2 x 4 heads x 4096 keys x 128: 518 us at 512
+// workgroups, 343 at 1024, 362 at 2048); without one only until they fill it once together with the row pass, more would
+// only add sums to join (8 x 8 x 512 x 64: 32 us in one share, 46 in two; 1 x 2 x 4096 x 64: 85 us in eight, 108 in four).
+// At least four row tiles each; fp32, whose products take eight times as long, two while every workgroup has a CU to
+// itself (2 x 4 x 130 x 64: 32 us against 47; past that, 2 x 3 x 1000 x 64, 142 against 121).
 static int kv_split(const ifd_attention_args& a) {
-  const int64_t base = (int64_t)a.B * a.Hk * cdiv(a.Tk, 128), tiles = (int64_t)(a.Hq / a.Hk) * cdiv(a.Tq, 64);
-  const int64_t n = std::min<int64_t>(cdiv(a.causal ? 1024 : 512, std::max<int64_t>(base, 1)), std::max<int64_t>(tiles / 4, 1));
-  return (int)std::min<int64_t>(n, 16);
+  const int64_t base = std::max<int64_t>((int64_t)a.B * a.Hk * cdiv(a.Tk, 128), 1), nq = (int64_t)a.B * a.Hq * cdiv(a.Tq, 128);
+  const int64_t tiles = (int64_t)(a.Hq / a.Hk) * cdiv(a.Tq, 64);
+  int64_t n = std::min(a.causal ? cdiv(1024, base) : (640 - nq) / base, tiles / 4);
+  if (a.dtype == IFD_F32) n = std::max(n, std::min((256 - nq) / base, tiles / 2));
+  return (int)std::min<int64_t>(std::max<int64_t>(n, 1), 16);
 }
 
-template <typename T, int DP>
-static int run_bwd_q(AttnK p, hipStream_t s) {
-  typedef AttnTile<T, DP> TL;
-  constexpr int BK = TL::ROWB >= 512 ? 32 : 64, OCC = TL::ROWB >= 512 ? 1 : 2, AHEAD = TL::KS % 4 ? 3 : 4;
-  constexpr int lds = 4 * BK * TL::ROWB;
-  static bool attr[kMaxDevices] = {};
-  auto kern = attn_bwd_q_kernel<T, DP, BK, AHEAD, OCC>;
-  if (set_lds_attr_once(attr, reinterpret_cast<const void*>(kern), lds) != hipSuccess) return IFD_LAUNCH_STATUS();
-  p.nblk = (int)cdiv(p.Tq, 128);
-  hipLaunchKernelGGL(kern, dim3(p.nblk * p.B * p.Hq), dim3(256), lds, s, p);
-  return IFD_LAUNCH_STATUS();
-}
+// Short calls run both passes in one launch. Each pass alone leaves most of the chip waiting for its longest workgroups;
+// side by side they fill it, for the price of finding lse2 and delta twice (us as two launches, as one: 2 x 8|2 heads x 512
+// x 128 bf16 causal 48, 33; 4 x 8 x 256 x 64 fp32 75, 49; 1 x 1 x 16 x 64 22, 5; 16 x 8 x 256 x 128, 1024 workgroups, 39,
+// 34). FUSE_ROWS: rows of a share (their lse2 and delta stay in 4 KB of LDS); FUSE_WGS: workgroups of both.
+constexpr int FUSE_ROWS = 512, FUSE_WGS = 1024;
 
 template <typename T, int DP>
 static int run_bwd(AttnK p, int nsplit, hipStream_t s) {
-  constexpr int ROWB = AttnTile<T, DP>::ROWB;
-  constexpr int BK = ROWB >= 512 ? 32 : 64, OCCK = ROWB >= 512 ? 1 : 2;
+  typedef AttnTile<T, DP> TL;
+  constexpr int ROWB = TL::ROWB, BK = ROWB >= 512 ? 32 : 64, OCC = ROWB >= 512 ? 1 : 2, AHEAD = TL::KS % 4 ? 3 : 4;
   constexpr bool VL = sizeof(T) == 2 && DP == 128;
-  constexpr int NWK = 4, BQ = VL ? 32 : BK;
-  if (p.Tq)
-    if (int e = run_bwd_q<T, DP>(p, s)) return e;
-  if (!p.Tk) return 0;
-  constexpr int lds = 2 * (2 * BQ * ROWB + 1024) + (VL ? NWK * 32 * ROWB : 0);
-  static bool attr[kMaxDevices] = {};
-  auto kern = attn_bwd_kv_kernel<T, DP, NWK, BQ, VL, OCCK>;
-  if (set_lds_attr_once(attr, reinterpret_cast<const void*>(kern), lds) != hipSuccess) return IFD_LAUNCH_STATUS();
-  p.nblk = (int)cdiv(p.Tk, 32 * NWK);
+  constexpr int BQ = VL ? 32 : BK;
+  constexpr int lds_q = 4 * BK * ROWB, lds_kv = 4 * BQ * ROWB + (VL ? 128 * ROWB : 0);  // (without lse2 and delta)
+  const int64_t nq = cdiv(p.Tq, 128) * p.B * p.Hq, nkv = cdiv(p.Tk, 128) * p.B * p.Hk * nsplit;
   p.nsplit = nsplit;
-  hipLaunchKernelGGL(kern, dim3(p.nblk * p.B * p.Hk * nsplit), dim3(64 * NWK), lds, s, p);
-  if (int e = IFD_LAUNCH_STATUS()) return e;
+  if (nq && nkv && nq + nkv <= FUSE_WGS && cdiv(cdiv(p.Tq, BQ) * p.G, nsplit) * BQ <= FUSE_ROWS) {
+    constexpr int lds = std::max(lds_q, lds_kv + FUSE_ROWS * 8);
+    static bool attr[kMaxDevices] = {};
+    auto kern = attn_bwd_both_kernel<T, DP, BK, AHEAD, BQ, VL, OCC>;
+    if (set_lds_attr_once(attr, reinterpret_cast<const void*>(kern), lds) != hipSuccess) return IFD_LAUNCH_STATUS();
+    hipLaunchKernelGGL(kern, dim3((unsigned)(nq + nkv)), dim3(256), lds, s, p, (int)nq);
+    if (int e = IFD_LAUNCH_STATUS()) return e;
+  } else {
+    if (nq) {
+      static bool attr[kMaxDevices] = {};
+      auto kern = attn_bwd_q_kernel<T, DP, BK, AHEAD, OCC>;
+      if (set_lds_attr_once(attr, reinterpret_cast<const void*>(kern), lds_q) != hipSuccess) return IFD_LAUNCH_STATUS();
+      hipLaunchKernelGGL(kern, dim3((unsigned)nq), dim3(256), lds_q, s, p);
+      if (int e = IFD_LAUNCH_STATUS()) return e;
+    }
+    if (!nkv) return 0;
+    constexpr int lds = lds_kv + 2048;
+    static bool attr[kMaxDevices] = {};
+    auto kern = attn_bwd_kv_kernel<T, DP, 4, BQ, VL, OCC>;
+    if (set_lds_attr_once(attr, reinterpret_cast<const void*>(kern), lds) != hipSuccess) return IFD_LAUNCH_STATUS();
+    hipLaunchKernelGGL(kern, dim3((unsigned)nkv), dim3(256), lds, s, p);
+    if (int e = IFD_LAUNCH_STATUS()) return e;
+  }
   if (nsplit > 1) {
     auto join = attn_bwd_join_kernel<T, DP>;
     hipLaunchKernelGGL(join, dim3((unsigned)cdiv((int64_t)p.B * p.Hk * p.Tk * (DP / 2), 256)), dim3(256), 0, s, p);

@@ -479,3 +479,14 @@ def test_anything_behind_the_last_row_and_in_rows_without_keys(Tq, dt, D):
             k2[b, max(s + Tq, 0):], v2[b, max(s + Tq, 0):] = junk, junk
             q2[b, :max(-s, 0)], d2[b, :max(-s, 0)] = junk, junk
         assert _same(_both(q2, k2, v2, d2, **kw), want), junk
+
+
+@pytest.mark.parametrize("case", [(1, 2500, 130, 4, 1, 64, BF, True, None, None), (1, 2500, 130, 4, 1, 128, HF, False, [97], None),
+                                  (1, 2500, 66, 4, 1, 80, F32, True, None, [-7]), (40, 64, 64, 16, 16, 40, HF, True, None, None),
+                                  (24, 200, 130, 8, 8, 128, BF, False, None, None), (1, 1, 4000, 4, 4, 64, F32, False, None, None),
+                                  (1, 4000, 1, 2, 1, 96, BF, False, None, None), (2, 130, 130, 4, 1, 64, F32, False, None, None)],
+                         ids=lambda c: "-".join(str(x).replace("torch.", "") for x in c[:8]))
+def test_backward_as_two_launches_and_as_one(case):
+    """Long shares and many workgroups (row pass and key pass one after the other), and short calls around them (both in one
+    launch)."""
+    test_forward_and_backward(case)
