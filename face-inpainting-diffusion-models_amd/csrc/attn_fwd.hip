@@ -1,5 +1,6 @@
 // Attention forward: out = softmax(scale q k^T) v and the rows' log-sum-exp (include/ifd_ops.h), one pass over the keys
 // with a running maximum and sum.
+#include <type_traits>
 #include "attn_dev.h"
 #include "kernels.h"
 
@@ -73,10 +74,17 @@ struct AttnRows {
   }
 };
 
+// Partial results of a row (r = token * G + head of the group) and split: O [DP], reference point, sum, two unused.
+template <int DP>
+__device__ __forceinline__ float* part_row(const AttnK& p, int b, int hk, int r, int sp) {
+  return p.ws + ((((int64_t)b * p.Hk + hk) * p.Tq * p.G + r) * p.nsplit + sp) * (DP + 4);
+}
+
 // Many rows. A workgroup's four waves take 32 rows each of one (sequence, head) and share the K and V tiles (BK keys, two
 // buffers, the next tile's DMA in flight during this one's products). Per wave and tile: S^T = K Q^T with Q in registers,
 // softmax down the registers of each lane (a lane holds one row's scores of half the keys), O^T += V^T P^T.
-template <typename T, int DP, int BK, int OCC>
+// SPLIT: the keys are dealt to nsplit workgroups, whose results attn_join_kernel joins.
+template <typename T, int DP, int BK, int OCC, bool SPLIT>
 __global__ __launch_bounds__(256, OCC) void attn_fwd_kernel(AttnK p) {
   typedef AttnTile<T, DP> TL;
   typedef typename TL::frag frag;
@@ -86,16 +94,17 @@ __global__ __launch_bounds__(256, OCC) void attn_fwd_kernel(AttnK p) {
   const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, h = lane >> 5;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   // causal: longest blocks first, a head's blocks on one XCD; else head by head on each XCD
-  const int BH = p.B * p.Hq;
+  const int BH = p.B * p.Hq, nblk = (p.Tq + NW * 32 - 1) / (NW * 32);
+  const int blk = SPLIT ? blockIdx.x / p.nsplit : blockIdx.x, sp = SPLIT ? blockIdx.x - blk * p.nsplit : 0;
   int bh, qblk;
   if (p.causal) {
-    const int r = blockIdx.x % BH;
-    qblk = p.nblk - 1 - blockIdx.x / BH;
+    const int r = blk % BH;
+    qblk = nblk - 1 - blk / BH;
     bh = (BH & 7) ? r : (r & 7) * (BH >> 3) + (r >> 3);
   } else {
-    const int id = xcd_order(blockIdx.x, BH * p.nblk);
-    bh = id / p.nblk;
-    qblk = id - bh * p.nblk;
+    const int id = xcd_order(blk, BH * nblk);
+    bh = id / nblk;
+    qblk = id - bh * nblk;
   }
   const int b = bh / p.Hq, hq = bh - b * p.Hq, hk = hq / p.G;
   const int len = seq_len(p, b), qs = q_first(p, b);
@@ -118,7 +127,12 @@ __global__ __launch_bounds__(256, OCC) void attn_fwd_kernel(AttnK p) {
   const int w_last = min(p.Tq, q0 + 32) - 1;
   const int w_end = __builtin_amdgcn_readfirstlane(w_last < q0 ? 0 : row_limit(p, qs, len, w_last));
   const int w_all = __builtin_amdgcn_readfirstlane(w_last < q0 ? 0 : row_limit(p, qs, len, q0));
-  const int nt = (wg_end + BK - 1) / BK;
+  int tb = 0, nt = (wg_end + BK - 1) / BK;  // this workgroup's tiles: [tb, nt)
+  if (SPLIT) {
+    const int per = (nt + p.nsplit - 1) / p.nsplit;
+    tb = sp * per;
+    nt = min(nt, tb + per);
+  }
 
   AttnStage<T, DP, BK, NW> sg;
   sg.init(w, lane, p.D);
@@ -126,20 +140,20 @@ __global__ __launch_bounds__(256, OCC) void attn_fwd_kernel(AttnK p) {
   const char* vp = p.v + b * p.vb + hk * p.vh;
   auto stage = [&](int t) {
     const int k0 = t * BK, n = min(BK, wg_end - k0);
-    lds_c* d = sm + (t & 1) * (2 * TB);
+    lds_c* d = sm + ((t - tb) & 1) * (2 * TB);
     sg.load(kp + (int64_t)k0 * p.kt, p.kt, n, d, w);
     sg.load(vp + (int64_t)k0 * p.vt, p.vt, n, d + TB, w);
   };
-  if (nt > 0) {
-    stage(0);
+  if (tb < nt) {
+    stage(tb);
     dma_wait();
     __syncthreads();
   }
-  for (int t = 0; t < nt; ++t) {
+  for (int t = tb; t < nt; ++t) {
     if (t + 1 < nt) stage(t + 1);
     const int k0 = t * BK;
     if (k0 < w_end) {
-      const lds_c* kb = sm + (t & 1) * (2 * TB);
+      const lds_c* kb = sm + ((t - tb) & 1) * (2 * TB);
       const lds_c* vb = kb + TB;
       f32x16 s[KT];
 #pragma unroll
@@ -183,6 +197,23 @@ __global__ __launch_bounds__(256, OCC) void attn_fwd_kernel(AttnK p) {
   }
   const float l = st.l + xhalf(st.l);
   if (i >= p.Tq) return;
+  if (SPLIT) {
+    float* po = part_row<DP>(p, b, hk, i * p.G + hq - hk * p.G, sp);
+#pragma unroll
+    for (int d = 0; d < TL::DT; ++d)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        f32x4 v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = st.o[d][4 * j + e];
+        *reinterpret_cast<f32x4*>(po + d * 32 + 8 * j + 4 * h) = v;
+      }
+    if (h == 0) {
+      po[DP] = st.m;
+      po[DP + 1] = l;
+    }
+    return;
+  }
   const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
   if (h == 0 && p.lse)
     p.lse[((int64_t)b * p.Hq + hq) * p.Tq + i] =
@@ -319,8 +350,7 @@ __global__ __launch_bounds__(NW * 64) void attn_split_kernel(AttnK p) {
     lt += f[x] * xf[32 + l32];
   }
   // thread (row l32, group tid / 32): channels group, group + 2 NW, ...
-  const int64_t prow = (((int64_t)b * p.Hk + hk) * p.nblk + rb) * 32 + l32;
-  float* po = p.nsplit > 1 ? p.ws + (prow * p.nsplit + sp) * (DP + 2) : nullptr;
+  float* po = p.nsplit > 1 ? part_row<DP>(p, b, hk, r, sp) : nullptr;
   const float inv = lt > 0.f ? 1.f / lt : (lt == 0.f ? 0.f : lt);
   T* op = reinterpret_cast<T*>(p.out + b * p.ob + hq * p.oh + (int64_t)i * p.ot);
   for (int g = tid >> 5; g < DP / 4; g += 2 * NW) {
@@ -331,57 +361,80 @@ __global__ __launch_bounds__(NW * 64) void attn_split_kernel(AttnK p) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) v[e] += f[x] * xf[e * 32];
     }
+    if (!ok) continue;
     if (po) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) po[2 + 4 * g + e] = v[e];
-    } else if (ok && 4 * g < p.D) {
+      *reinterpret_cast<f32x4*>(po + 4 * g) = v;
+    } else if (4 * g < p.D) {
       v *= inv;
       *reinterpret_cast<typename TL::A::quad*>(op + 4 * g) = __builtin_convertvector(v, typename TL::A::quad);
     }
   }
-  if (tid < 32) {
+  if (tid < 32 && ok) {
     if (po) {
-      po[0] = m;
-      po[1] = lt;
-    } else if (ok) {
+      po[DP] = m;
+      po[DP + 1] = lt;
+    } else {
       p.lse[((int64_t)b * p.Hq + hq) * p.Tq + i] =
           lt == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(lt)) * 0.69314718055994531f;
     }
   }
 }
 
-// One wave per row: the splits' partial results in order.
+// The splits' partial results in order: W lanes per row, four channels each; the splits' statistics are spread over the
+// lanes, so that no load waits for another.
 template <typename T, int DP>
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnK p) {
-  const int lane = threadIdx.x & 63;
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  constexpr int W = DP == 64 ? 16 : 32, U = 64 / W;  // at most 64 splits
+  const int li = threadIdx.x & (W - 1), first = threadIdx.x & 63 & ~(W - 1), ch = 4 * li;
+  const int64_t row = (int64_t)blockIdx.x * (256 / W) + threadIdx.x / W;
   const int rows = p.Tq * p.G;
   if (row >= (int64_t)p.B * p.Hk * rows) return;
   const int bk = (int)(row / rows), r = (int)(row - (int64_t)bk * rows);
   const int b = bk / p.Hk, hk = bk - b * p.Hk, i = r / p.G, hq = hk * p.G + (r - i * p.G);
-  const float* w = p.ws + ((int64_t)bk * p.nblk * 32 + r) * p.nsplit * (DP + 2);
-  // lane s holds split s's statistics (at most 64 splits): the loads below do not wait for each other
-  const bool has = lane < p.nsplit;
-  const float ms = has ? w[lane * (DP + 2)] : -INFINITY, ls = has ? w[lane * (DP + 2) + 1] : 0.f;
-  float m = ms;
+  const float* w = part_row<DP>(p, b, hk, r, 0);
+  float f[U], ls[U], m = -INFINITY, l = 0.f;
 #pragma unroll
-  for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
-  const float fs = ms == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ms - m);
-  float l = fs * ls, a[DP / 64] = {};
-#pragma unroll
-  for (int o = 32; o; o >>= 1) l += __shfl_xor(l, o);
-#pragma unroll 8
-  for (int s = 0; s < p.nsplit; ++s) {
-    const float f = __shfl(fs, s);
-#pragma unroll
-    for (int e = 0; e < DP / 64; ++e) a[e] += f * w[s * (DP + 2) + 2 + lane + 64 * e];
+  for (int u = 0; u < U; ++u) {
+    const int s = u * W + li;
+    f[u] = s < p.nsplit ? w[s * (DP + 4) + DP] : -INFINITY;
+    ls[u] = s < p.nsplit ? w[s * (DP + 4) + DP + 1] : 0.f;
+    m = fmaxf(m, f[u]);
   }
-  const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-  T* op = reinterpret_cast<T*>(p.out + b * p.ob + hq * p.oh + (int64_t)i * p.ot);
 #pragma unroll
-  for (int e = 0; e < DP / 64; ++e)
-    if (lane + 64 * e < p.D) op[lane + 64 * e] = (T)(a[e] * inv);
-  if (lane == 0)
+  for (int o = W / 2; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    f[u] = f[u] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(f[u] - m);
+    l += f[u] * ls[u];
+  }
+#pragma unroll
+  for (int o = W / 2; o; o >>= 1) l += __shfl_xor(l, o);
+  f32x4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int n = min(p.nsplit - u * W, W);
+    auto some = [&](int s0, auto k) {  // (loads past the last split read it again, with a factor of 0)
+      f32x4 x[k.value];
+#pragma unroll
+      for (int e = 0; e < k.value; ++e)
+        if (ch < DP) x[e] = *reinterpret_cast<const f32x4*>(w + (u * W + min(s0 + e, n - 1)) * (DP + 4) + ch);
+#pragma unroll
+      for (int e = 0; e < k.value; ++e) {
+        const float fs = __shfl(f[u], first + min(s0 + e, n - 1));
+        if (ch < DP && s0 + e < n) v += fs * x[e];
+      }
+    };
+    if (n <= 4) {
+      if (n > 0) some(0, std::integral_constant<int, 4>{});
+    } else {
+      for (int s = 0; s < n; s += 16) some(s, std::integral_constant<int, 16>{});
+    }
+  }
+  v *= l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+  if (ch < p.D)
+    *reinterpret_cast<typename AttnT<T>::quad*>(reinterpret_cast<T*>(p.out + b * p.ob + hq * p.oh + (int64_t)i * p.ot) + ch) =
+        __builtin_convertvector(v, typename AttnT<T>::quad);
+  if (li == 0)
     p.lse[((int64_t)b * p.Hq + hq) * p.Tq + i] =
         l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * 0.69314718055994531f;
 }
@@ -410,30 +463,37 @@ const char* attention_tensor_check(const ifd_attention_args& a, const void* p, c
 }
 
 struct FwdPlan {
-  bool split;
-  int nblk, nsplit;
+  bool few;  // attn_split_kernel, else attn_fwd_kernel
+  int dp, nsplit;
+  int64_t wgs;
 };
 
-// The tile of 32 rows per (sequence, key-value head) reads every key once for all the heads of a group, but its products
-// have no reuse between waves: it is taken while the rows of a group fill few tiles, or while the many-row kernel's
-// workgroups (128 rows each) would leave most of the chip idle.
-static FwdPlan fwd_plan(const ifd_attention_args& a, int dp, int es) {
-  const int G = a.Hq / a.Hk;
+// Which kernel, and into how many shares of the keys. attn_split_kernel reads every key once for all heads of a group, but
+// its waves share no tiles: it is taken for up to 32 rows a head, or 128 rows a group of narrow heads (us, it against
+// attn_fwd_kernel: 2 x 8|4 heads x 24 x 3000 x 96 bf16 13, 18; 8 x 8|4 x 64 x 700 x 64 fp32 19, 36; the other way round
+// 4 x 8|2 x 100 x 4096 x 128 bf16 39, 27; 2 x 4|1 x 120 x 16000 x 64 fp16 30, 22). attn_fwd_kernel shares the keys out while
+// its workgroups would fill half the chip's CUs at most: to two a CU (in one share and in this many: 4 x 8 x 200 x 8192 x 64
+// bf16 103, 36; 3 x 6|3 x 500 x 3000 x 80 fp32 348, 131; 2 x 8 x 1024 x 4096 x 64 fp16 58, 38; with 256 workgroups in one
+// share already, 4 x 8 x 1024 x 1024 x 64, two take 29 instead of 21), of eight tiles at least, four in fp32, whose tiles
+// take longer to multiply (4 x 8|2 x 100 x 4096 x 128 bf16 27 in shares of eight tiles, 30 of four; 2 x 4 x 700 x 128 fp32
+// causal 62 and 37).
+static FwdPlan fwd_plan(const ifd_attention_args& a) {
+  const int G = a.Hq / a.Hk, es = (int)dtype_bytes(a.dtype);
   FwdPlan r;
-  const int64_t rows = (int64_t)a.Tq * G, rb = cdiv(rows, 32), base = (int64_t)a.B * a.Hk * rb;
-  const int64_t big = cdiv(a.Tq, 128) * a.B * a.Hq;
-  r.split = rows <= 32 || (big < 64 && a.Tk >= 256);
-  if (!r.split) {
-    r.nblk = (int)cdiv(a.Tq, 128);
-    r.nsplit = 1;
-    return r;
+  const int64_t rows = (int64_t)a.Tq * G;
+  r.few = a.Tq <= 32 || rows <= (a.D <= 64 ? 128 : 32);
+  if (!r.few) {
+    r.dp = a.D <= 64 ? 64 : a.D <= 96 ? 96 : 128;
+    r.wgs = cdiv(a.Tq, 128) * a.B * a.Hq;
+    const int64_t tiles = cdiv(a.Tk, r.dp * es >= 512 ? 32 : 64);
+    r.nsplit = r.wgs > 128 ? 1 : (int)std::max<int64_t>(1, std::min<int64_t>({512 / r.wgs, tiles / (es == 4 ? 4 : 8), 64}));
+  } else {
+    r.dp = a.D <= 64 ? 64 : 128;
+    r.wgs = cdiv(rows, 32) * a.B * a.Hk;
+    const int64_t tiles = cdiv(a.Tk, r.dp * es == 128 ? 64 : 32);
+    r.nsplit = (int)std::max<int64_t>(1, std::min<int64_t>({cdiv(256, r.wgs), cdiv(tiles, 8), 64}));
   }
-  r.nblk = (int)rb;
-  const int bk = dp * es == 128 ? 64 : 32;
-  const int64_t tiles = cdiv(a.Tk, bk);
-  int64_t n = cdiv(256, base);
-  n = std::min<int64_t>(n, cdiv(tiles, 8));
-  r.nsplit = (int)std::max<int64_t>(1, std::min<int64_t>(n, 64));
+  r.wgs *= r.nsplit;
   return r;
 }
 
@@ -458,42 +518,48 @@ AttnK attention_kernel_args(const ifd_attention_args& a) {
   return p;
 }
 
-template <typename T, int DP>
-static int run_rows(const AttnK& p, hipStream_t s) {
+template <typename T, int DP, bool SPLIT>
+static int run_rows(const AttnK& p, int64_t wgs, hipStream_t s) {
   constexpr int ROWB = AttnTile<T, DP>::ROWB, BK = ROWB >= 512 ? 32 : 64, OCC = ROWB == 128 ? 4 : ROWB == 256 ? 2 : 1;
   constexpr int lds = 4 * BK * ROWB;
   static bool attr[kMaxDevices] = {};
-  auto kern = attn_fwd_kernel<T, DP, BK, OCC>;
+  auto kern = attn_fwd_kernel<T, DP, BK, OCC, SPLIT>;
   if (set_lds_attr_once(attr, reinterpret_cast<const void*>(kern), lds) != hipSuccess) return IFD_LAUNCH_STATUS();
-  hipLaunchKernelGGL(kern, dim3(p.nblk * p.B * p.Hq), dim3(256), lds, s, p);
+  hipLaunchKernelGGL(kern, dim3((unsigned)wgs), dim3(256), lds, s, p);
   return IFD_LAUNCH_STATUS();
 }
 
 template <typename T, int DP>
-static int run_split(const AttnK& p, hipStream_t s) {
+static int run_few(const AttnK& p, int64_t wgs, hipStream_t s) {
   constexpr int ROWB = DP * (int)sizeof(T);
   constexpr int BK = ROWB == 128 ? 64 : 32, NW = ROWB >= 512 ? 2 : 4;
   constexpr int lds = NW * 4 * BK * ROWB;
   static bool attr[kMaxDevices] = {};
   auto kern = attn_split_kernel<T, DP, NW, BK>;
   if (set_lds_attr_once(attr, reinterpret_cast<const void*>(kern), lds) != hipSuccess) return IFD_LAUNCH_STATUS();
-  hipLaunchKernelGGL(kern, dim3(p.nsplit * p.nblk * p.B * p.Hk), dim3(NW * 64), lds, s, p);
-  if (int e = IFD_LAUNCH_STATUS()) return e;
-  if (p.nsplit > 1) {
-    const int64_t rows = (int64_t)p.B * p.Hq * p.Tq;
-    auto join = attn_join_kernel<T, DP>;
-    hipLaunchKernelGGL(join, dim3((unsigned)cdiv(rows, 4)), dim3(256), 0, s, p);
-    return IFD_LAUNCH_STATUS();
-  }
-  return 0;
+  hipLaunchKernelGGL(kern, dim3((unsigned)wgs), dim3(NW * 64), lds, s, p);
+  return IFD_LAUNCH_STATUS();
+}
+
+template <typename T, int DP>
+static int run_fwd_d(const FwdPlan& pl, const AttnK& p, hipStream_t s) {
+  int e;
+  if constexpr (DP == 96)
+    e = pl.nsplit > 1 ? run_rows<T, DP, true>(p, pl.wgs, s) : run_rows<T, DP, false>(p, pl.wgs, s);
+  else
+    e = pl.few ? run_few<T, DP>(p, pl.wgs, s)
+               : pl.nsplit > 1 ? run_rows<T, DP, true>(p, pl.wgs, s) : run_rows<T, DP, false>(p, pl.wgs, s);
+  if (e || pl.nsplit == 1) return e;
+  auto join = attn_join_kernel<T, DP>;
+  hipLaunchKernelGGL(join, dim3((unsigned)cdiv((int64_t)p.B * p.Hq * p.Tq, DP == 64 ? 16 : 8)), dim3(256), 0, s, p);
+  return IFD_LAUNCH_STATUS();
 }
 
 template <typename T>
 static int run_fwd(const FwdPlan& pl, AttnK p, hipStream_t s) {
-  p.nblk = pl.nblk;
+  p.nblk = (int)cdiv((int64_t)p.Tq * p.G, 32);  // (attn_split_kernel's row tiles)
   p.nsplit = pl.nsplit;
-  if (pl.split) return p.D <= 64 ? run_split<T, 64>(p, s) : run_split<T, 128>(p, s);
-  return p.D <= 64 ? run_rows<T, 64>(p, s) : p.D <= 96 ? run_rows<T, 96>(p, s) : run_rows<T, 128>(p, s);
+  return pl.dp == 64 ? run_fwd_d<T, 64>(pl, p, s) : pl.dp == 96 ? run_fwd_d<T, 96>(pl, p, s) : run_fwd_d<T, 128>(pl, p, s);
 }
 
 // The UNet's QKVAttention (code/nn.py:222-235) on qkv [N][T][3C]: heads of 64 channels at offsets 0, C, 2C; queries and keys
@@ -508,8 +574,7 @@ int launch_attention_rows(const float* qkv, int N, int T, int C, float scale, fl
   p.B = N; p.Tq = p.Tk = T; p.Hq = p.Hk = C / 64; p.D = 64; p.G = 1;
   p.scale = scale * scale;
   p.c = p.scale * 1.4426950408889634f;
-  p.nblk = (int)cdiv(T, 128);
-  return run_rows<float, 64>(p, s);
+  return run_rows<float, 64, false>(p, cdiv(T, 128) * N * (C / 64), s);
 }
 
 }  // namespace ifd
@@ -519,10 +584,8 @@ extern "C" {
 
 int64_t ifd_op_attention_ws_bytes(const ifd_attention_args* a) {
   if (!a || attention_check(*a) || !a->B || !a->Tq) return 0;
-  const int dp = a->D <= 64 ? 64 : 128;
-  const FwdPlan pl = fwd_plan(*a, dp, (int)dtype_bytes(a->dtype));
-  if (!pl.split || pl.nsplit == 1) return 0;
-  return (int64_t)a->B * a->Hk * pl.nblk * 32 * pl.nsplit * (dp + 2) * 4;
+  const FwdPlan pl = fwd_plan(*a);
+  return pl.nsplit == 1 ? 0 : (int64_t)a->B * a->Hq * a->Tq * pl.nsplit * (pl.dp + 4) * 4;
 }
 
 int ifd_op_attention(const ifd_attention_args* a, void* ws, int64_t ws_bytes, void* stream) {
@@ -530,15 +593,14 @@ int ifd_op_attention(const ifd_attention_args* a, void* ws, int64_t ws_bytes, vo
   const char* why = attention_check(*a);
   IFD_OP_REQUIRE(!why, why);
   if (!a->B || !a->Tq) return 0;
-  const int es = (int)dtype_bytes(a->dtype), dp = a->D <= 64 ? 64 : 128;
   if ((why = attention_tensor_check(*a, a->q, a->q_s)) || (why = attention_tensor_check(*a, a->out, a->out_s)) ||
       (a->Tk && ((why = attention_tensor_check(*a, a->k, a->k_s)) || (why = attention_tensor_check(*a, a->v, a->v_s)))))
     IFD_OP_REQUIRE(false, why);
   IFD_OP_REQUIRE(a->lse != nullptr, "a null lse");
-  IFD_OP_REQUIRE(ws_bytes >= ifd_op_attention_ws_bytes(a) && (ws || !ifd_op_attention_ws_bytes(a)),
-                 "workspace too small");
-  const FwdPlan pl = fwd_plan(*a, dp, es);
-  IFD_OP_REQUIRE((int64_t)pl.nsplit * pl.nblk * a->B * a->Hq < 0x7fffffff, "sizes beyond one launch");
+  const int64_t need = ifd_op_attention_ws_bytes(a);
+  IFD_OP_REQUIRE(ws_bytes >= need && (ws || !need) && !((uintptr_t)ws & 15), "workspace too small or not aligned to 16 bytes");
+  const FwdPlan pl = fwd_plan(*a);
+  IFD_OP_REQUIRE(pl.wgs < 0x7fffffff, "sizes beyond one launch");
   AttnK p = attention_kernel_args(*a);
   p.ws = (float*)ws;
   hipStream_t s = (hipStream_t)stream;

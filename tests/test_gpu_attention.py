@@ -490,3 +490,14 @@ def test_backward_as_two_launches_and_as_one(case):
     """Long shares and many workgroups (row pass and key pass one after the other), and short calls around them (both in one
     launch)."""
     test_forward_and_backward(case)
+
+
+@pytest.mark.parametrize("case", [(1, 150, 1100, 2, 1, 64, BF, False, None, None), (1, 150, 700, 2, 2, 128, F32, True, None, None),
+                                  (2, 140, 1500, 4, 2, 80, HF, True, [1499, 600], [1300, 500]),
+                                  (3, 200, 1100, 2, 1, 96, F32, True, [0, 1100, 70], [-150, 900, 0]),
+                                  (1, 129, 2100, 1, 1, 128, BF, True, None, [-100]), (1, 40, 1700, 3, 1, 72, HF, False, None, None),
+                                  (2, 16, 1000, 8, 1, 128, BF, True, [999, 3], [980, 0]), (1, 33, 300, 4, 1, 64, F32, True, None, None)],
+                         ids=lambda c: "-".join(str(x).replace("torch.", "") for x in c[:8]))
+def test_rows_whose_keys_are_shared_out(case):
+    """Enough rows for the many-row kernel and enough keys to split them, with ragged lengths and rows without keys."""
+    test_forward_and_backward(case)
