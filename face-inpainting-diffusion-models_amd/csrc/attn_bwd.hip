@@ -349,16 +349,33 @@ __device__ __forceinline__ void attn_bwd_kv(const AttnK& p, lds_c* sm, int blk) 
           dp[x] = s[x] * (dp[x] - de[e]);
         }
       }
+      if constexpr (TL::ES == 4) {  // the products of 32 rows are added up by themselves first, one sum at a time
 #pragma unroll
-      for (int ps = 0; ps < TL::PS; ++ps) {
-        const frag fp = TL::pack(s, ps), fd = TL::pack(dp, ps);
+        for (int y = 0; y < 2 * TL::DT; ++y) {
+          f32x16 z;
 #pragma unroll
-        for (int d = 0; d < TL::DT; ++d) {
-          const frag ga = TL::col(gb, qt * 32, ps, d, lane), qa = TL::col(qb, qt * 32, ps, d, lane);
+          for (int x = 0; x < 16; ++x) z[x] = 0.f;
 #pragma unroll
-          for (int j = 0; j < TL::A::MS; ++j) {
-            dv[d] = TL::A::mma(ga, fp, j, dv[d]);
-            dk[d] = TL::A::mma(qa, fd, j, dk[d]);
+          for (int ps = 0; ps < TL::PS; ++ps) {
+            const frag f = TL::pack(y & 1 ? dp : s, ps), a = TL::col(y & 1 ? qb : gb, qt * 32, ps, y >> 1, lane);
+#pragma unroll
+            for (int j = 0; j < TL::A::MS; ++j) z = TL::A::mma(a, f, j, z);
+          }
+#pragma unroll
+          for (int x = 0; x < 16; ++x) (y & 1 ? dk : dv)[y >> 1][x] += z[x];
+        }
+      } else {
+#pragma unroll
+        for (int ps = 0; ps < TL::PS; ++ps) {
+          const frag fp = TL::pack(s, ps), fd = TL::pack(dp, ps);
+#pragma unroll
+          for (int d = 0; d < TL::DT; ++d) {
+            const frag ga = TL::col(gb, qt * 32, ps, d, lane), qa = TL::col(qb, qt * 32, ps, d, lane);
+#pragma unroll
+            for (int j = 0; j < TL::A::MS; ++j) {
+              dv[d] = TL::A::mma(ga, fp, j, dv[d]);
+              dk[d] = TL::A::mma(qa, fd, j, dk[d]);
+            }
           }
         }
       }

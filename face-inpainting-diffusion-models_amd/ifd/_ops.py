@@ -132,9 +132,9 @@ def may_overlap(a, b):
     return max(hi) > row or not (hi[0] <= lo[1] or hi[1] <= lo[0])
 
 
-def workspace(nbytes, dev):
-    """Scratch of one call, from torch's stream-ordered allocator (None when the call needs none)."""
-    return torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+def workspace(nbytes, t):
+    """Scratch of one call on t's device, from torch's stream-ordered allocator (None when the call needs none)."""
+    return t.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
 
 
 def call(fn, dev, *args):

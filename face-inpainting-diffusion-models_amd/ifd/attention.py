@@ -101,11 +101,11 @@ def attention(q, k, v, scale=None, causal=False, kv_len=None, q_start=None, out=
     """(out, lse): attention of every query row, and its log-sum-exp fp32 [B, Hq, Tq]."""
     q, k, v, scale, kv_len, q_start, dev = _inputs(q, k, v, scale, kv_len, q_start)
     out = _into(out, q, "out", q, k, v)
-    lse = torch.empty((q.shape[0], q.shape[2], q.shape[1]), dtype=torch.float32, device=dev)
+    lse = q.new_empty((q.shape[0], q.shape[2], q.shape[1]), dtype=torch.float32)
     a = _pack(q, k, v, scale, causal, kv_len, q_start, out, lse) + _NO_BWD
     L = lib()
     n = L.ifd_op_attention_ws_bytes(a)
-    ws = workspace(n, dev)
+    ws = workspace(n, q)
     call(L.ifd_op_attention, dev, a, None if ws is None else ws.data_ptr(), n)
     return out, lse
 
@@ -131,6 +131,6 @@ def attention_bwd(dout, q, k, v, out, lse, scale=None, causal=False, kv_len=None
         *dk.stride()[:3], *dv.stride()[:3])
     L = lib()
     n = L.ifd_op_attention_bwd_ws_bytes(a)
-    ws = workspace(n, dev)
+    ws = workspace(n, q)
     call(L.ifd_op_attention_bwd, dev, a, None if ws is None else ws.data_ptr(), n)
     return dq, dk, dv

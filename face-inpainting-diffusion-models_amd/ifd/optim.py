@@ -123,7 +123,7 @@ class AdamW:
             cnt = (ctypes.c_int64 * n)(*[x for a in arrays for x in a[2]])
             gt = b"".join(a[4] for a in arrays)
         nb = L.ifd_op_grad_norm_ws_bytes(len(cnt), cnt)
-        ws = workspace(nb, self.device)
+        ws = workspace(nb, self.m)
         call(L.ifd_op_grad_norm, self.device, len(cnt), g, cnt, gt, float(self.max_norm), self.norm_coef.data_ptr(),
              None if ws is None else ws.data_ptr(), nb)
 

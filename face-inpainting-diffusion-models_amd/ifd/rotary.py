@@ -160,14 +160,14 @@ def qk_norm_rope_bwd(gq, gk, q, k, wq=None, wk=None, pos=None, rope=None, eps=1e
     gq, gk = _rows(gq), None if gk is None else _rows(gk)
     dq = _into(dq, q, "dq", gq, q, k, gk)
     dk = _into(dk, k, "dk", gk, q, k, gq, dq)
-    dwq = None if wq is None else torch.empty(q.shape[3], dtype=torch.float32, device=dev)
-    dwk = None if wk is None else torch.empty(q.shape[3], dtype=torch.float32, device=dev)
+    dwq = None if wq is None else q.new_empty(q.shape[3], dtype=torch.float32)
+    dwk = None if wk is None else q.new_empty(q.shape[3], dtype=torch.float32)
     gkp, gks, dkp, dks = (0, _NO_ST, 0, _NO_ST) if k is None else (gk.data_ptr(), gk.stride()[:3], dk.data_ptr(), dk.stride()[:3])
     a = _pack(q, k, wq, wk, pos, rope, eps, norm, None, None) + _MORE.pack(
         gq.data_ptr(), gkp, dq.data_ptr(), dkp, 0 if dwq is None else dwq.data_ptr(), 0 if dwk is None else dwk.data_ptr(),
         *gq.stride()[:3], *gks, *dq.stride()[:3], *dks)
     L = lib()
     n = L.ifd_op_qk_norm_rope_bwd_ws_bytes(a)
-    ws = workspace(n, dev)
+    ws = workspace(n, q)
     call(L.ifd_op_qk_norm_rope_bwd, dev, a, None if ws is None else ws.data_ptr(), n)
     return dq, dk, dwq, dwk

@@ -212,7 +212,8 @@ int ifd_tr_add(const float* a, const float* b, float* out, int64_t n, void* stre
 /* dst[p][doff+c] (=|+=) src[p][soff+c], c < nc: the skip concat (code/unet.py:170) and its gradient split */
 int ifd_tr_copy_channels(const float* src, int cs, int soff, float* dst, int cd, int doff, int nc, int64_t npix,
                          int accumulate, void* stream);
-/* QKVAttention (code/nn.py:222-235) on qkv [N][T][3C] -> out [N][T][C], and its backward (dqkv written). */
+/* QKVAttention (code/nn.py:222-235) on qkv [N][T][3C] -> out [N][T][C] (any T), and its backward (dqkv written; the
+ * probabilities are kept in scratch: for T > 256 ifd_op_attention_bwd of ifd_ops.h, which recomputes them, needs far less). */
 int ifd_tr_attention(const float* qkv, int N, int T, int C, float scale, float* out, void* stream);
 int64_t ifd_tr_attention_bwd_scratch_floats(int N, int T, int C);
 int ifd_tr_attention_bwd(const float* qkv, const float* dout, int N, int T, int C, float scale, float* dqkv,
