@@ -72,11 +72,15 @@ __global__ __launch_bounds__(256) void qk_rope_kernel(QkK p) {
       const int first = tok_sub * p.hs * p.lg + sub;  // this lane's twin in the token's first group
       for (int j0 = 0; j0 < V; j0 += p.hs) {
         double f = rotated && j0 + head0 < V ? p.turns[u + j0 + head0] * ps : 0.0;
+        // turns -> the nearest quarter and the rest, which alone is rounded to fp32 (at most 1/8 turn: 2^-27 off)
         f -= rint(f);
-        float s, c;
-        sincospif(2.f * (float)f, &s, &c);
-        s *= p.mscale;
-        c *= p.mscale;
+        const double quarter = rint(4.0 * f);
+        const int k = (int)quarter;
+        float s0, c0;
+        sincospif(2.f * (float)fma(quarter, -0.25, f), &s0, &c0);
+        float s = k & 1 ? c0 : s0, c = k & 1 ? s0 : c0;
+        s *= k & 2 ? -p.mscale : p.mscale;
+        c *= (k + 1) & 2 ? -p.mscale : p.mscale;
 #pragma unroll
         for (int j = 0; j < V; ++j)
           if (j >= j0 && j < j0 + p.hs) {
