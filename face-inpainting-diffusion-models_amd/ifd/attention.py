@@ -34,10 +34,9 @@ _FWD, _BWD = struct.Struct("8if i 7P 12q"), struct.Struct("4P 12q")
 _NO_BWD = bytes(_BWD.size)
 
 
-def _lay(t):
-    """t itself when the kernels can read it, else a contiguous copy."""
+def _lay(t, e):
+    """t itself when the kernels can read it (elements of e bytes), else a contiguous copy."""
     s0, s1, s2, s3 = t.stride()
-    e = t.element_size()
     if s3 == 1 and 0 <= s1 * e < 1 << 24 and not ((s0 | s1 | s2) * e | t.data_ptr()) & 15:
         return t
     return t.clone(memory_format=torch.contiguous_format)
@@ -64,8 +63,9 @@ def _inputs(q, k, v, scale, kv_len, q_start):
         refuse(f"k, v must be [{B}, tokens, heads, {D}] and alike, got {tuple(k.shape)} and {tuple(v.shape)}")
     if not (Hk > 0 and Hq > 0 and Hq % Hk == 0):
         refuse(f"{Hq} query heads are not a multiple of {Hk} key-value heads")
-    if not 0 < D <= 128 or D & (3 if dt is torch.float32 else 7):
-        refuse(f"head width {D}: at most 128 and a multiple of {16 // q.element_size()}")
+    e = 4 if dt is torch.float32 else 2
+    if not 0 < D <= 128 or D * e & 15:
+        refuse(f"head width {D}: at most 128 and a multiple of {16 // e}")
     scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
     if not 0.0 < scale < 3e38:
         refuse(f"scale must be positive and finite, got {scale}")
@@ -75,7 +75,7 @@ def _inputs(q, k, v, scale, kv_len, q_start):
         kv_len = _int_arg(kv_len, B, "kv_len", dev)
     if q_start is not None:
         q_start = _int_arg(q_start, B, "q_start", dev)
-    return _lay(q), _lay(k), _lay(v), scale, kv_len, q_start, dev
+    return _lay(q, e), _lay(k, e), _lay(v, e), scale, kv_len, q_start, dev
 
 
 def _pack(q, k, v, scale, causal, kv_len, q_start, out, lse):
@@ -90,7 +90,7 @@ def _into(t, like, name, *inputs):
     """A caller's output tensor (checked) or a new contiguous one."""
     if t is None:
         return torch.empty_like(like, memory_format=torch.contiguous_format)
-    if not (t.dim() == 4 and _lay(t) is t):
+    if not (t.dim() == 4 and _lay(t, t.element_size()) is t):
         refuse(f"{name}: adjacent channels, 16-byte aligned, strides in multiples of 16 bytes")
     if any(_may_overlap(t, x) for x in inputs):
         refuse(f"{name} overlaps an input or another output")
@@ -114,14 +114,16 @@ def attention_bwd(dout, q, k, v, out, lse, scale=None, causal=False, kv_len=None
     """(dq, dk, dv) from the gradient of `out`; out, lse and the other arguments as the forward call had them.
     Keys at and past kv_len get zero gradients."""
     q, k, v, scale, kv_len, q_start, dev = _inputs(q, k, v, scale, kv_len, q_start)
+    shape, dt = q.shape, q.dtype
     for n, t in (("dout", dout), ("out", out)):
-        if not (t.shape == q.shape and t.dtype == q.dtype):
+        if not (t.shape == shape and t.dtype is dt):
             refuse(f"{n} must be like q")
-    if lse.shape != (q.shape[0], q.shape[2], q.shape[1]) or lse.dtype != torch.float32:
+    if lse.shape != (shape[0], shape[2], shape[1]) or lse.dtype is not torch.float32:
         refuse("lse must be the forward's, fp32 [B, Hq, Tq]")
     same_device(q, dout, out, lse)
     no_grad(dout, out)
-    dout, out, lse = _lay(dout), _lay(out), lse.contiguous()
+    e = 4 if dt is torch.float32 else 2
+    dout, out, lse = _lay(dout, e), _lay(out, e), lse.contiguous()
     ins = (q, k, v, dout, out)
     dq = _into(dq, q, "dq", *ins)
     dk = _into(dk, k, "dk", *ins, dq)
