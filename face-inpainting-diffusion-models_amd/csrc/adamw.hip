@@ -3,7 +3,8 @@
 //   p = p (1 - lr wd) - lr / (1 - b1^k) m / (sqrt(v) / sqrt(1 - b2^k) + eps)
 // Bound by memory: 16 bytes a value with fp32 tensors and 8-bit states, 28 with 32-bit states, plus the norm's own pass
 // over the gradients. The tensors' addresses travel in the kernel arguments (128 tensors a launch): no table to upload,
-// nothing kept between steps. A wave owns blocks of 256 values, four per lane; an 8-bit state's scale is its block's.
+// nothing kept between steps. 93.6 M values, 8-bit states: step 289 us, 5.2 TB/s; norm 120. A wave owns blocks of 256
+// values, four per lane; an 8-bit state's scale is its block's.
 //
 // 8-bit states. One byte is a small float, with one fp32 scale per block of 256 (largest magnitude / 1.875):
 //   m: sign, 4 exponent bits, 3 fraction bits: 2^(e - 15) (1 + f / 8);  v: 5 exponent bits, 3 fraction bits: 2^(e - 31)
@@ -21,7 +22,7 @@ namespace ifd {
 
 constexpr int AW_T = 128;     // tensors of a launch (its tables fill the 4 KB of kernel arguments)
 constexpr int64_t AW_MAX = (int64_t)1 << 31;  // values of a table entry: a longer tensor takes several
-constexpr int AW_CHUNK = 16;  // blocks of a workgroup
+constexpr int AW_CHUNK = 16;  // blocks of a workgroup (93.6 M values, norm, step and values: 596 us; 604 with 8, 597 with 32)
 
 struct AwTab {
   const void* p[AW_T];

@@ -231,12 +231,15 @@ static const char* qk_check(const ifd_qk_args& a) {
   for (int64_t s : {a.q_s[2] * a.Hq, a.gq_s[2] * a.Hq, a.dq_s[2] * a.Hq, a.q_out_s[2] * a.Hq, a.k_s[2] * a.Hk,
                     a.gk_s[2] * a.Hk, a.dk_s[2] * a.Hk, a.k_out_s[2] * a.Hk})
     if (s > lim || s < -lim) return "a token's heads reach over more than 2 GiB";
-  if ((int64_t)a.Hq + a.Hk > 1 << 20 || (int64_t)a.B * a.T * (a.Hq + a.Hk) >= (int64_t)1 << 31) return "sizes: 2^31 head rows and more";
+  if ((int64_t)a.Hq + a.Hk > 1 << 20 || (int64_t)a.B * a.T * (a.Hq + a.Hk) >= (int64_t)1 << 31)
+    return "sizes: 2^31 head rows and more";
   return nullptr;
 }
 
-constexpr int QK_FWD_WGS = 1024;
-constexpr int QK_WGS = 512;  // workgroups of the backward pass (each leaves one partial row of weight gradients)
+// Workgroups: enough to fill the chip, few enough that each walks over many tokens (4 x 4096 x 20 heads x 128 bf16, forward:
+// 29.6 us with 1024, 5.7 TB/s; 30.2 with 2048, 36.5 with 512. Backward, where each leaves one partial row of weight
+// gradients: 59.5 with 512; 67.3 with 1024, 82.9 with 256)
+constexpr int QK_FWD_WGS = 1024, QK_WGS = 512;
 
 static bool vec_ok(int V, int es, const ifd_qk_args& a, bool bwd) {
   if ((a.rot / 2) % V || ((a.D - a.rot) / 2) % V) return false;

@@ -501,3 +501,12 @@ def test_backward_as_two_launches_and_as_one(case):
 def test_rows_whose_keys_are_shared_out(case):
     """Enough rows for the many-row kernel and enough keys to split them, with ragged lengths and rows without keys."""
     test_forward_and_backward(case)
+
+
+@pytest.mark.parametrize("case", [(2, 70, 90, 2, 1, 8, BF, True, None, None), (1, 200, 70, 2, 2, 4, F32, False, None, None),
+                                  (1, 150, 1100, 1, 1, 8, HF, False, None, None), (2, 5, 700, 4, 2, 4, F32, True, [700, 9], None),
+                                  (1, 90, 100, 2, 1, 104, BF, True, None, None), (1, 90, 100, 2, 1, 120, HF, False, None, None),
+                                  (1, 90, 100, 2, 1, 100, F32, True, None, None), (1, 3, 600, 2, 2, 88, BF, False, [599], None)],
+                         ids=lambda c: "-".join(str(x).replace("torch.", "") for x in c[:8]))
+def test_narrow_and_odd_heads(case):
+    test_forward_and_backward(case)
