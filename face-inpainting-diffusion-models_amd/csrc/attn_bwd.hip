@@ -4,7 +4,8 @@
 // Two passes, each owning its outputs, so that nothing is added atomically and the result does not depend on timing:
 // attn_bwd_q_kernel (a wave owns 32 query rows; three products per score tile) also leaves each row's lse2 and delta for
 // attn_bwd_kv_kernel (a wave owns 32 keys; four products). Seven products against the five of one pass with atomics on dq.
-// Short calls run both side by side in one launch (attn_bwd_both_kernel).
+// Short calls run both side by side in one launch (attn_bwd_both_kernel). Where there are few workgroups each pass deals its
+// walk out in shares (q_split, kv_split), whose fp32 sums attn_bwd_join_kernel adds in order.
 // Bound by the matrix units: 2 x 16|4 heads x 4096 x 128 bf16 causal 488 us (traced: row pass 215, key pass 280, join 23), 985
 // TFLOP/s over the seven products; 16 x 4 x 1024 x 64 fp32 484 us, 124 TFLOP/s, matrix units 78 % busy.
 #include "attn_dev.h"
@@ -13,11 +14,12 @@ namespace ifd {
 
 // (waves and tiles as in the forward kernel)
 template <typename T, int DP, int BK, int AHEAD, bool STATS>
-__device__ __forceinline__ void attn_bwd_q(const AttnK& p, lds_c* sm, int blk) {
+__device__ __forceinline__ void attn_bwd_q(const AttnK& p, lds_c* sm, int wg) {
   typedef AttnTile<T, DP> TL;
   typedef typename TL::frag frag;
   constexpr int NW = 4, KT = BK / 32, TB = BK * TL::ROWB;
   const int nblk = (p.Tq + NW * 32 - 1) / (NW * 32);
+  const int blk = wg / p.nsplit_q, sp = wg - blk * p.nsplit_q;
   const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, h = lane >> 5;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int BH = p.B * p.Hq;
@@ -60,7 +62,7 @@ __device__ __forceinline__ void attn_bwd_q(const AttnK& p, lds_c* sm, int blk) {
     const float l = p.lse[srow];
     if (l != -INFINITY) lse2 = l * 1.4426950408889634f;
     if (lim == 0) delta = 0.f;
-    if (STATS && h == 0) {
+    if (STATS && h == 0 && sp == 0) {
       p.ws[srow] = lse2;
       p.ws[(int64_t)p.B * p.Hq * p.Tq + srow] = delta;
     }
@@ -76,25 +78,26 @@ __device__ __forceinline__ void attn_bwd_q(const AttnK& p, lds_c* sm, int blk) {
   const int w_last = min(p.Tq, q0 + 32) - 1;
   const int w_end = __builtin_amdgcn_readfirstlane(w_last < q0 ? 0 : row_limit(p, qs, len, w_last));
   const int w_all = __builtin_amdgcn_readfirstlane(w_last < q0 ? 0 : row_limit(p, qs, len, q0));
-  const int nt = (wg_end + BK - 1) / BK;
+  const int tiles = (wg_end + BK - 1) / BK, per = (tiles + p.nsplit_q - 1) / p.nsplit_q;
+  const int tb = sp * per, nt = min(tiles, tb + per);  // this workgroup's tiles: [tb, nt)
   AttnStage<T, DP, BK, NW> sg;
   sg.init(w, lane, p.D);
   const char* kp = p.k + b * p.kb + hk * p.kh;
   const char* vp = p.v + b * p.vb + hk * p.vh;
   auto stage = [&](int t) {
     const int k0 = t * BK, n = min(BK, wg_end - k0);
-    lds_c* d = sm + (t & 1) * (2 * TB);
+    lds_c* d = sm + ((t - tb) & 1) * (2 * TB);
     sg.load(kp + (int64_t)k0 * p.kt, p.kt, n, d, w);
     sg.load(vp + (int64_t)k0 * p.vt, p.vt, n, d + TB, w);
   };
-  if (nt > 0) {
-    stage(0);
+  if (tb < nt) {
+    stage(tb);
     dma_wait();
     __syncthreads();
   }
-  for (int t = 0; t < nt; ++t) {
+  for (int t = tb; t < nt; ++t) {
     if (t + 1 < nt) stage(t + 1);
-    const lds_c* kb = sm + (t & 1) * (2 * TB);
+    const lds_c* kb = sm + ((t - tb) & 1) * (2 * TB);
     const lds_c* vb = kb + TB;
     const int k0 = t * BK;
     if (k0 < w_end) {
@@ -164,6 +167,19 @@ __device__ __forceinline__ void attn_bwd_q(const AttnK& p, lds_c* sm, int blk) {
     __syncthreads();
   }
   if (!ok) return;
+  if (p.nsplit_q > 1) {
+    float* po = p.ws_q + ((((int64_t)b * p.Hq + hq) * p.nsplit_q + sp) * p.Tq + i) * DP;
+#pragma unroll
+    for (int d = 0; d < TL::DT; ++d)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        f32x4 v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = lim ? acc[d][4 * j + e] : 0.f;
+        *reinterpret_cast<f32x4*>(po + d * 32 + 8 * j + 4 * h) = v;
+      }
+    return;
+  }
   T* op = reinterpret_cast<T*>(p.dq + b * p.dqb + hq * p.dqh + (int64_t)i * p.dqt);
 #pragma unroll
   for (int d = 0; d < TL::DT; ++d)
@@ -451,10 +467,24 @@ __global__ __launch_bounds__(256, OCC) void attn_bwd_both_kernel(AttnK p, int nq
     attn_bwd_kv<T, DP, 4, BQ, VL, true>(p, (lds_c*)smem, blockIdx.x - nq);
 }
 
-// dk, dv = the shares' sums in order; one thread per four channels of a (key, dk | dv) row.
+// dk, dv = the shares' sums in order; one thread per four channels of a (key, dk | dv) row. The workgroups from nkv on: dq.
 template <typename T, int DP>
-__global__ __launch_bounds__(256) void attn_bwd_join_kernel(AttnK p) {
+__global__ __launch_bounds__(256) void attn_bwd_join_kernel(AttnK p, int nkv) {
   typedef typename AttnT<T>::quad quad;
+  if ((int)blockIdx.x >= nkv) {
+    const int64_t g = (int64_t)(blockIdx.x - nkv) * 256 + threadIdx.x, row = g / (DP / 4);
+    const int ch = 4 * (int)(g - row * (DP / 4));
+    if (row >= (int64_t)p.B * p.Hq * p.Tq || ch >= p.D) return;
+    const int64_t bh = row / p.Tq;
+    const int i = (int)(row - bh * p.Tq), b = (int)(bh / p.Hq), hq = (int)(bh - (int64_t)b * p.Hq);
+    const float* w = p.ws_q + (bh * p.nsplit_q * p.Tq + i) * DP + ch;
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < p.nsplit_q; ++s) v += *reinterpret_cast<const f32x4*>(w + (int64_t)s * p.Tq * DP);
+    v *= p.scale;
+    *reinterpret_cast<quad*>(reinterpret_cast<T*>(p.dq + b * p.dqb + hq * p.dqh + (int64_t)i * p.dqt) + ch) =
+        __builtin_convertvector(v, quad);
+    return;
+  }
   constexpr int C4 = 2 * DP / 4;
   const int64_t g = (int64_t)blockIdx.x * 256 + threadIdx.x;
   const int64_t row = g / C4;
@@ -474,14 +504,26 @@ __global__ __launch_bounds__(256) void attn_bwd_join_kernel(AttnK p) {
   *reinterpret_cast<quad*>(o + ch) = __builtin_convertvector(v, quad);
 }
 
+// Shares of the row pass, whose workgroups else walk over all keys one after the other: where they are few, up to 128 of them
+// with two tiles of keys in fp32 and four in 16 bits, up to 192 with twice as many (us, in one share and so: 2 x 3 heads x
+// 1000 x 64 fp32 114, 79; 3 x 4 x 500 x 128 fp32 causal 126, 80; 1 x 4 x 2048 x 64 bf16 causal 48, 35; 1 x 8 x 1024 x 128 bf16
+// causal 46, 39, 45 with 256 workgroups; 8 x 4|2 x 300 x 40 fp32 causal 49, 65 with 192 of one or two tiles).
+static int q_split(const ifd_attention_args& a) {
+  const int64_t nq = (int64_t)a.B * a.Hq * cdiv(a.Tq, 128), tiles = cdiv(a.Tk, 64), few = a.dtype == IFD_F32 ? 2 : 4;
+  if (!nq || nq > 128) return 1;
+  const int64_t n = std::max(std::min(128 / nq, tiles / few), std::min(192 / nq, tiles / (2 * few)));
+  return (int)std::min<int64_t>(std::max<int64_t>(n, 1), 16);
+}
+
 // Shares of the key pass: workgroups of 128 keys (two per CU at a time) deal their walk out among each other. With a causal
 // mask, whose workgroups are unlike, until they fill the chip twice (2 x 4 heads x 4096 keys x 128: 518 us at 512
 // workgroups, 343 at 1024, 362 at 2048); without one only until they fill it once together with the row pass, more would
 // only add sums to join (8 x 8 x 512 x 64: 32 us in one share, 46 in two; 1 x 2 x 4096 x 64: 85 us in eight, 108 in four).
 // At least four row tiles each; fp32, whose products take eight times as long, two while every workgroup has a CU to
-// itself (2 x 4 x 130 x 64: 32 us against 47; past that, 2 x 3 x 1000 x 64, 142 against 121).
+// itself (2 x 4 x 130 x 64: 32 us against 47; past that, 2 x 3 x 1000 x 64, 142 against 121). (Row pass in one share.)
 static int kv_split(const ifd_attention_args& a) {
-  const int64_t base = std::max<int64_t>((int64_t)a.B * a.Hk * cdiv(a.Tk, 128), 1), nq = (int64_t)a.B * a.Hq * cdiv(a.Tq, 128);
+  const int64_t base = std::max<int64_t>((int64_t)a.B * a.Hk * cdiv(a.Tk, 128), 1);
+  const int64_t nq = (int64_t)a.B * a.Hq * cdiv(a.Tq, 128) * q_split(a);
   const int64_t tiles = (int64_t)(a.Hq / a.Hk) * cdiv(a.Tq, 64);
   int64_t n = std::min(a.causal ? cdiv(1024, base) : (640 - nq) / base, tiles / 4);
   if (a.dtype == IFD_F32) n = std::max(n, std::min((256 - nq) / base, tiles / 2));
@@ -495,7 +537,7 @@ static int kv_split(const ifd_attention_args& a) {
 constexpr int FUSE_ROWS = 512, FUSE_WGS = 1024;
 
 template <typename T, int DP>
-static int run_bwd(AttnK p, int nsplit, hipStream_t s) {
+static int run_bwd(const AttnK& p, hipStream_t s) {
   typedef AttnTile<T, DP> TL;
   constexpr int ROWB = TL::ROWB, BK = ROWB >= 512 ? 32 : 64, OCC = ROWB >= 512 ? 1 : 2;
   constexpr int AHEAD = sizeof(T) == 4 && DP == 64 ? 1 : TL::KS % 4 ? 3 : 4;  // (fp32 has no registers to read ahead into)
@@ -504,9 +546,8 @@ static int run_bwd(AttnK p, int nsplit, hipStream_t s) {
   constexpr bool VL = sizeof(T) == 2 ? DP == 128 : DP == 64;
   constexpr int BQ = VL ? 32 : BK;
   constexpr int lds_q = 4 * BK * ROWB, lds_kv = 4 * BQ * ROWB + (VL ? 128 * ROWB : 0);  // (without lse2 and delta)
-  const int64_t nq = cdiv(p.Tq, 128) * p.B * p.Hq, nkv = cdiv(p.Tk, 128) * p.B * p.Hk * nsplit;
-  p.nsplit = nsplit;
-  if (nq && nkv && nq + nkv <= FUSE_WGS && cdiv(cdiv(p.Tq, BQ) * p.G, nsplit) * BQ <= FUSE_ROWS) {
+  const int64_t nq = cdiv(p.Tq, 128) * p.B * p.Hq * p.nsplit_q, nkv = cdiv(p.Tk, 128) * p.B * p.Hk * p.nsplit;
+  if (nq && nkv && nq + nkv <= FUSE_WGS && cdiv(cdiv(p.Tq, BQ) * p.G, p.nsplit) * BQ <= FUSE_ROWS) {
     constexpr int lds = std::max(lds_q, lds_kv + FUSE_ROWS * 8);
     static bool attr[kMaxDevices] = {};
     auto kern = attn_bwd_both_kernel<T, DP, BK, AHEAD, BQ, VL, OCC>;
@@ -521,25 +562,26 @@ static int run_bwd(AttnK p, int nsplit, hipStream_t s) {
       hipLaunchKernelGGL(kern, dim3((unsigned)nq), dim3(256), lds_q, s, p);
       if (int e = IFD_LAUNCH_STATUS()) return e;
     }
-    if (!nkv) return 0;
-    constexpr int lds = lds_kv + 2048;
-    static bool attr[kMaxDevices] = {};
-    auto kern = attn_bwd_kv_kernel<T, DP, 4, BQ, VL, OCC>;
-    if (set_lds_attr_once(attr, reinterpret_cast<const void*>(kern), lds) != hipSuccess) return IFD_LAUNCH_STATUS();
-    hipLaunchKernelGGL(kern, dim3((unsigned)nkv), dim3(256), lds, s, p);
-    if (int e = IFD_LAUNCH_STATUS()) return e;
+    if (nkv) {
+      constexpr int lds = lds_kv + 2048;
+      static bool attr[kMaxDevices] = {};
+      auto kern = attn_bwd_kv_kernel<T, DP, 4, BQ, VL, OCC>;
+      if (set_lds_attr_once(attr, reinterpret_cast<const void*>(kern), lds) != hipSuccess) return IFD_LAUNCH_STATUS();
+      hipLaunchKernelGGL(kern, dim3((unsigned)nkv), dim3(256), lds, s, p);
+      if (int e = IFD_LAUNCH_STATUS()) return e;
+    }
   }
-  if (nsplit > 1) {
-    auto join = attn_bwd_join_kernel<T, DP>;
-    hipLaunchKernelGGL(join, dim3((unsigned)cdiv((int64_t)p.B * p.Hk * p.Tk * (DP / 2), 256)), dim3(256), 0, s, p);
-    return IFD_LAUNCH_STATUS();
-  }
-  return 0;
+  const int64_t jkv = p.nsplit > 1 ? cdiv((int64_t)p.B * p.Hk * p.Tk * (DP / 2), 256) : 0;
+  const int64_t jq = p.nsplit_q > 1 ? cdiv((int64_t)p.B * p.Hq * p.Tq * (DP / 4), 256) : 0;
+  if (jkv + jq == 0) return 0;
+  auto join = attn_bwd_join_kernel<T, DP>;
+  hipLaunchKernelGGL(join, dim3((unsigned)(jkv + jq)), dim3(256), 0, s, p, (int)jkv);
+  return IFD_LAUNCH_STATUS();
 }
 
 template <typename T>
-static int run_bwd_d(const AttnK& p, int nsplit, hipStream_t s) {
-  return p.D <= 64 ? run_bwd<T, 64>(p, nsplit, s) : p.D <= 96 ? run_bwd<T, 96>(p, nsplit, s) : run_bwd<T, 128>(p, nsplit, s);
+static int run_bwd_d(const AttnK& p, hipStream_t s) {
+  return p.D <= 64 ? run_bwd<T, 64>(p, s) : p.D <= 96 ? run_bwd<T, 96>(p, s) : run_bwd<T, 128>(p, s);
 }
 
 }  // namespace ifd
@@ -547,11 +589,18 @@ static int run_bwd_d(const AttnK& p, int nsplit, hipStream_t s) {
 using namespace ifd;
 extern "C" {
 
+// floats of workspace: lse2 and delta, the key pass' shares (both `head`), the row pass' shares
+static void bwd_ws(const ifd_attention_args& a, int64_t& head, int64_t& all) {
+  const int64_t dp = a.D <= 64 ? 64 : a.D <= 96 ? 96 : 128, n = kv_split(a), nq = q_split(a), rows = (int64_t)a.B * a.Hq * a.Tq;
+  head = 2 * rows + (n > 1 ? (int64_t)a.B * a.Hk * n * a.Tk * 2 * dp : 0);
+  all = head + (nq > 1 ? rows * nq * dp : 0);
+}
+
 int64_t ifd_op_attention_bwd_ws_bytes(const ifd_attention_args* a) {
   if (!a || attention_check(*a) || !a->B) return 0;
-  const int dp = a->D <= 64 ? 64 : a->D <= 96 ? 96 : 128, n = kv_split(*a);
-  const int64_t part = n > 1 ? (int64_t)a->B * a->Hk * n * a->Tk * 2 * dp : 0;
-  return (2 * (int64_t)a->B * a->Hq * a->Tq + part) * 4;
+  int64_t head, all;
+  bwd_ws(*a, head, all);
+  return all * 4;
 }
 
 int ifd_op_attention_bwd(const ifd_attention_args* a, void* ws, int64_t ws_bytes, void* stream) {
@@ -570,15 +619,20 @@ int ifd_op_attention_bwd(const ifd_attention_args* a, void* ws, int64_t ws_bytes
   IFD_OP_REQUIRE(a->lse != nullptr || !a->Tq, "a null lse");
   const int64_t need = ifd_op_attention_bwd_ws_bytes(a);
   IFD_OP_REQUIRE(ws_bytes >= need && (ws || !need) && !((uintptr_t)ws & 15), "workspace too small or not aligned to 16 bytes");
-  const int n = kv_split(*a);
-  IFD_OP_REQUIRE(cdiv(a->Tk, 128) * a->B * a->Hk * n < 0x7fffffff && cdiv(a->Tq, 128) * a->B * a->Hq < 0x7fffffff &&
+  const int n = kv_split(*a), nq = q_split(*a);
+  IFD_OP_REQUIRE(cdiv(a->Tk, 128) * a->B * a->Hk * n < 0x7fffffff && cdiv(a->Tq, 128) * a->B * a->Hq * nq < 0x7fffffff &&
                      (int64_t)a->B * a->Hk * a->Tk < (int64_t)1 << 31,
                  "sizes beyond one launch");
   AttnK p = attention_kernel_args(*a);
+  int64_t head, all;
+  bwd_ws(*a, head, all);
   p.ws = (float*)ws;
+  p.ws_q = p.ws + head;
+  p.nsplit = n;
+  p.nsplit_q = nq;
   hipStream_t s = (hipStream_t)stream;
-  return a->dtype == IFD_F32 ? run_bwd_d<float>(p, n, s)
-                             : a->dtype == IFD_BF16 ? run_bwd_d<__bf16>(p, n, s) : run_bwd_d<_Float16>(p, n, s);
+  return a->dtype == IFD_F32 ? run_bwd_d<float>(p, s)
+                             : a->dtype == IFD_BF16 ? run_bwd_d<__bf16>(p, s) : run_bwd_d<_Float16>(p, s);
 }
 
 }  // extern "C"

@@ -199,9 +199,9 @@ struct AttnK {  // kernel arguments: strides in bytes
   const int *kv_len, *q_start;
   int64_t qb, qh, kb, kh, vb, vh, ob, oh, gb, gh, dqb, dqh, dkb, dkh, dvb, dvh;
   int qt, kt, vt, ot, gt, dqt, dkt, dvt;  // token strides
-  int B, Tq, Tk, Hq, Hk, D, G, causal, nblk, nsplit;
+  int B, Tq, Tk, Hq, Hk, D, G, causal, nblk, nsplit, nsplit_q;
   float c, scale;  // c = scale log2(e)
-  float* ws;
+  float *ws, *ws_q;
 };
 
 __device__ __forceinline__ int seq_len(const AttnK& p, int b) {

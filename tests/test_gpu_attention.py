@@ -510,3 +510,12 @@ def test_rows_whose_keys_are_shared_out(case):
                          ids=lambda c: "-".join(str(x).replace("torch.", "") for x in c[:8]))
 def test_narrow_and_odd_heads(case):
     test_forward_and_backward(case)
+
+
+@pytest.mark.parametrize("case", [(1, 300, 1000, 2, 1, 64, F32, True, [900], [600]), (2, 129, 700, 3, 1, 80, HF, False, [700, 0], None),
+                                  (1, 77, 3000, 2, 2, 128, BF, True, None, [-20]), (1, 1, 900, 1, 1, 96, F32, False, None, None),
+                                  (1, 2500, 640, 4, 1, 64, BF, False, [635], None), (3, 33, 513, 1, 1, 128, F32, True, [513, 40, 512], None)],
+                         ids=lambda c: "-".join(str(x).replace("torch.", "") for x in c[:8]))
+def test_backward_whose_rows_keys_are_shared_out(case):
+    """Few rows and many keys: the row pass in shares, joined beside the key pass'; in one launch and in two."""
+    test_forward_and_backward(case)
