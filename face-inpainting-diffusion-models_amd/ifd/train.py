@@ -158,7 +158,7 @@ class UNetTrainer:
     state_bits=8: both AdamW moments as one byte a value and a scale per 256 values (ifd.optim.AdamW, `self.opt`): 2 bytes of
     state a parameter instead of 8; `seed` seeds their rounding. The gradients then stay unclipped in the grad buffer, a
     step whose gradient norm is not finite is left out, and norm_coef is fp64. state_dict() holds the parameters alone, as
-    with 32 bits; `opt.state_dict()` the states.
+    with 32 bits; `opt.state_dict()` the states and the step number: a new trainer that loads both goes on bit for bit.
 
     gnb_act (with fuse_gnb, round 6, off by default): that epilogue also writes the GroupNorm's forward output
     silu(z) — the input of the conv whose weight gradient is next (ifd_tr_conv_x3_gnb_act) — so that weight
@@ -194,9 +194,8 @@ class UNetTrainer:
         self.numel = n
         z = lambda: torch.zeros(n, device=self.dev, dtype=torch.float32)  # noqa: E731
         self.flat, self.grad = z(), z()
-        self.step_count = 0
+        self.opt, self._steps = None, 0
         if state_bits == 32:
-            self.opt = None
             self.m, self.v = z(), z()
             self.norm_coef = torch.zeros(2, device=self.dev)
         else:
@@ -224,6 +223,18 @@ class UNetTrainer:
         # the `is` check guards against a reused address, and every in-place write to a tensor (the
         # accumulating add_ / copy_ch / gn_bwd / resample_bwd paths) drops its entry (_dirty).
         self._gstat = {}
+
+    @property
+    def step_count(self):
+        """Optimizer steps done. With state_bits=8 it is the optimizer's own count, which opt.state_dict() holds."""
+        return self._steps if self.opt is None else self.opt.step_count
+
+    @step_count.setter
+    def step_count(self, n):
+        if self.opt is None:
+            self._steps = n
+        else:
+            self.opt.step_count = n
 
     def _dirty(self, t):
         """`t` is about to be written in place: its recorded statistics no longer describe it."""
@@ -1114,13 +1125,13 @@ class UNetTrainer:
 
     def optimizer_step(self):
         """clip_grad_norm_(max_norm) + AdamW (code/train_inpainting.py:64-66); norm on device, no sync."""
-        self.step_count += 1
         if self.opt is not None:
             o = self.opt
-            o.groups[0]["lr"], o.groups[0]["weight_decay"], o.step_count = self.lr, self.wd, self.step_count - 1
+            o.groups[0]["lr"], o.groups[0]["weight_decay"] = self.lr, self.wd
             o.betas, o.eps, o.max_norm = tuple(self.betas), self.eps, self.max_norm
             o.step([self.g(k) for k, _ in self.spec])
             return
+        self.step_count += 1
         work = torch.empty(1024, device=self.dev, dtype=torch.float64)
         b1, b2 = self.betas
         chk(lib().ifd_tr_clip_adamw(P(self.flat), P(self.grad), P(self.m), P(self.v), self.numel, self.max_norm,
