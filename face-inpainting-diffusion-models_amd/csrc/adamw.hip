@@ -114,6 +114,12 @@ __device__ __forceinline__ double recip(double x) {
   r = fma(r, fma(-x, r, 1.0), r);
   return fma(r, fma(-x, r, 1.0), r);
 }
+// NaN if one of the four is, else x
+__device__ __forceinline__ float nan_or(float x, f32x4 v) {
+  const float t = __builtin_elementwise_maximum(__builtin_elementwise_maximum(v[0], v[1]),
+                                                __builtin_elementwise_maximum(v[2], v[3]));
+  return t != t ? t : x;
+}
 __device__ __forceinline__ double hi_double(unsigned hi) { return __hiloint2double((int)hi, 0); }
 __device__ __forceinline__ double m_value(unsigned c) {  // without the scale
   const unsigned k = c & 127u;
@@ -179,8 +185,10 @@ __global__ __launch_bounds__(256) void adamw_multi_kernel(const AwTab t, const A
         xm = fmax(xm, fabs(m[j]));
         xv = fmax(xv, v[j]);
       }
-      // the scale rounds max |x| / 1.875 to fp32: rounding keeps order, so the largest rounded value of the lanes is it
-      const float am = wave_max_nonneg((float)(xm * (1.0 / 1.875))), av = wave_max_nonneg((float)(xv * (1.0 / 1.875)));
+      // the scale rounds max |x| / 1.875 to fp32: rounding keeps order, so the largest rounded value of the lanes is it.
+      // fmax drops a NaN: it is found in the fp32 moments, where a maximum that keeps it is one instruction.
+      const float am = wave_max_nonneg(nan_or((float)(xm * (1.0 / 1.875)), mf));
+      const float av = wave_max_nonneg(nan_or((float)(xv * (1.0 / 1.875)), vf));
       const double im = am > 0.f ? recip(am) : 0.0, iv = av > 0.f ? recip(av) : 0.0;
       unsigned nm = 0, nv = 0;
 #pragma unroll

@@ -1,6 +1,9 @@
-"""The optimizer's states where a run is cut or a step is refused: a trainer with 8-bit states saved and resumed.
+"""The optimizer's states where a run is cut or goes wrong: a trainer with 8-bit states saved and resumed, and states after a
+gradient that is not finite.
 
-The resumed run does the same launches on the same bytes as the uncut one, so every bit has to be equal.
+The resumed run does the same launches on the same bytes as the uncut one, so every bit has to be equal. A block of 8-bit
+states has one scale, the largest magnitude over 1.875: where one of its values is NaN the scale is NaN, and so are the values
+that its 256 bytes stand for (NaN times any byte's value, 0 too).
 """
 import pytest
 import torch
@@ -54,3 +57,25 @@ def test_a_refused_step_is_not_counted():
     tr.step_count = 41  # a caller may set it, as with 32-bit states
     tr.optimizer_step()
     assert tr.step_count == tr.opt.step_count == 42
+
+
+@pytest.mark.parametrize("at", [0, 77, 255, 511, 599])
+def test_nan_gradient_spoils_its_8bit_block(at):
+    """Without the clip. Every lane of the block's maximum, both directions of a first and of a later step."""
+    from ifd.optim import AdamW
+    g = torch.Generator(device=DEV).manual_seed(at)
+    p = torch.randn(600, device=DEV, generator=g)
+    opt = AdamW([p], lr=1e-3, state_bits=8)
+    for k in range(3):
+        d = torch.randn(600, device=DEV, generator=g)
+        if k == 1:
+            d[at] = float("nan")
+        opt.step([d])
+        m, v = opt.moments()
+        b = at // 256
+        bad = torch.zeros(m.numel(), dtype=torch.bool, device=DEV)
+        if k:
+            bad[b * 256:(b + 1) * 256] = True
+        assert torch.equal(torch.isnan(m), bad) and torch.equal(torch.isnan(v), bad), k
+        spoilt = torch.isnan(p)
+        assert (spoilt.sum() == 1 and spoilt[at]) if k == 1 else torch.equal(spoilt, bad[:600] & (k == 2))
