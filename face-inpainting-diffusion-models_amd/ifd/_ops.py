@@ -106,12 +106,26 @@ def no_grad(*tensors):
                        "backward function yourself")
 
 
+def _apart(t):
+    """Whether t's strides nest: every dimension steps over all that the dimensions of smaller strides reach, so that no two
+    elements are one place. (Slices and permutations of a buffer nest; strides that interleave without meeting do not.)"""
+    if not t.numel():
+        return True
+    reach = 0
+    for s, n in sorted(zip(t.stride(), t.shape)):
+        if n > 1:
+            if s <= reach:
+                return False
+            reach += (n - 1) * s
+    return True
+
+
 def output(t, like, name):
     """Checks a caller's output tensor: like its input, every element a place of its own; marks it as written."""
     if not (t.shape == like.shape and t.dtype == like.dtype and t.device == like.device):
         refuse(f"{name} must be like its input")
-    if any(s == 0 and n > 1 for s, n in zip(t.stride(), t.shape)):
-        refuse(f"{name} has elements that share their place")
+    if not _apart(t):
+        refuse(f"{name} has elements that share their place, or strides {t.stride()} that do not nest")
     torch.autograd.graph.increment_version(t)
     return t
 

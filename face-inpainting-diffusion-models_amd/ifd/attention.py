@@ -13,7 +13,7 @@ Tk - Tq: the rows are the last ones). kv_len, q_start: int32 [B] on the GPU, rea
 Keys that no row of their sequence sees (at and past kv_len, or behind the last row's) change nothing, whatever they hold.
 A key that some rows see and others not must be finite in v (for the backward pass in k too), or it may spoil those others.
 A row that sees no key gets out = 0, lse = -inf and zero gradients, whatever q and dout hold there. Output tensors of the
-caller (out, dq, dk, dv) must not overlap the inputs nor each other.
+caller (out, dq, dk, dv) must not overlap the inputs, each other or themselves (strides must nest).
 
 The backward pass keeps no score matrix: it recomputes the probabilities from lse. Both directions are deterministic.
 Calls run on the current stream of the tensors' device and can be captured into a graph. They record nothing for autograd:

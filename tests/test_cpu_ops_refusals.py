@@ -1,0 +1,67 @@
+"""Calls of the attention-layer operators that must be refused before anything is written, on the host (no GPU): the device
+check is replaced, so that every other check runs on CPU tensors."""
+import pytest
+import torch
+
+
+@pytest.fixture
+def anywhere(monkeypatch):
+    """CPU tensors pass the device check; a call that reaches the library fails the test."""
+    from ifd import _ops, attention, optim, rotary
+
+    def reached(*a):
+        raise AssertionError("the call was not refused")
+    for m in (_ops, attention, optim, rotary):
+        if hasattr(m, "same_device"):
+            monkeypatch.setattr(m, "same_device", lambda *t: t[0].device)
+        if hasattr(m, "call"):
+            monkeypatch.setattr(m, "call", reached)
+
+
+def _qkv():
+    return torch.zeros(2, 6, 4, 16), torch.zeros(2, 6, 2, 16), torch.zeros(2, 6, 2, 16)
+
+
+# strides of a [2, 6, 4, 16] tensor some of whose elements are one place
+SHARED = [(384, 64, 0, 1), (0, 64, 16, 1), (384, 16, 16, 1), (64, 64, 16, 1), (384, 64, 12, 1), (320, 64, 16, 1), (16, 64, 16, 1)]
+# and of one whose elements are all apart: padded, transposed, every other head, batch innermost
+APART = [(384, 64, 16, 1), (500, 80, 20, 1), (384, 16, 96, 1), (1024, 128, 32, 1), (64, 128, 16, 1)]
+
+
+@pytest.mark.parametrize("st", SHARED)
+def test_outputs_whose_elements_share_a_place(anywhere, st):
+    from ifd.attention import attention, attention_bwd
+    from ifd.rotary import qk_norm_rope, qk_norm_rope_bwd
+    q, k, v = _qkv()
+    o = torch.zeros(4096).as_strided((2, 6, 4, 16), st)
+    calls = [lambda: attention(q, k, v, out=o), lambda: qk_norm_rope(q, k, q_out=o),
+             lambda: attention_bwd(q, q, k, v, q, torch.zeros(2, 4, 6), dq=o),
+             lambda: qk_norm_rope_bwd(q, k, q, k, dq=o), lambda: qk_norm_rope(o, k, q_out=o)]
+    for f in calls:
+        with pytest.raises(ValueError, match="share their place"):
+            f()
+
+
+@pytest.mark.parametrize("st", APART)
+def test_outputs_whose_elements_are_apart(anywhere, st):
+    from ifd import _ops
+    x = torch.zeros(8192).as_strided((2, 6, 4, 16), st)
+    assert _ops.output(x, torch.zeros(2, 6, 4, 16), "out") is x
+    one = torch.zeros(8192).as_strided((2, 1, 4, 16), (384, 0, 16, 1))  # a size of one: its stride says nothing
+    assert _ops.output(one, torch.zeros(2, 1, 4, 16), "out") is one
+    none = torch.zeros(8192).as_strided((2, 0, 4, 16), (0, 0, 0, 1))
+    assert _ops.output(none, torch.zeros(2, 0, 4, 16), "out") is none
+
+
+def test_places_agree_with_an_enumeration():
+    """Every stride triple of a small set against the set of addresses: no shared place is let through, and what is refused
+    either shares one or has strides that do not nest."""
+    import itertools
+    from ifd._ops import _apart
+    n = (2, 3, 4)
+    for st in itertools.product((1, 2, 3, 4, 6, 8, 9, 12), repeat=3):
+        seen = [sum(i * s for i, s in zip(ix, st)) for ix in itertools.product(*map(range, n))]
+        order = sorted(zip(st, n))
+        nest = all(b[0] > sum((m - 1) * s for s, m in order[:i + 1]) for i, b in enumerate(order[1:]))
+        assert _apart(torch.zeros(256).as_strided(n, st)) == nest
+        assert not nest or len(set(seen)) == len(seen)
