@@ -4,6 +4,7 @@ from __future__ import annotations
 import ctypes
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -98,12 +99,18 @@ def same_device(*tensors):
 
 
 def no_grad(*tensors):
-    """These operators record nothing for autograd: a call that autograd would have to follow is refused, not cut off."""
+    """These operators record nothing for autograd: a call that autograd would have to follow, in either direction, is refused,
+    not cut off."""
     if torch.is_grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:
                 refuse("the operator records no gradients: call it under torch.no_grad() (or with detached tensors) and its "
                        "backward function yourself")
+    # (the level spares the usual call 6 us a tensor; a torch that does not tell it is asked tensor by tensor)
+    if getattr(forward_ad, "_current_level", 0) >= 0:
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                refuse("the operator has no forward-mode derivative: a tensor carries a tangent")
 
 
 def _apart(t):

@@ -17,7 +17,7 @@ caller (out, dq, dk, dv) must not overlap the inputs, each other or themselves (
 
 The backward pass keeps no score matrix: it recomputes the probabilities from lse. Both directions are deterministic.
 Calls run on the current stream of the tensors' device and can be captured into a graph. They record nothing for autograd:
-tensors that require gradients are refused unless under torch.no_grad().
+tensors that require gradients are refused unless under torch.no_grad(), tensors with a forward-mode tangent always.
 """
 from __future__ import annotations
 
@@ -121,7 +121,7 @@ def attention_bwd(dout, q, k, v, out, lse, scale=None, causal=False, kv_len=None
     if lse.shape != (shape[0], shape[2], shape[1]) or lse.dtype is not torch.float32:
         refuse("lse must be the forward's, fp32 [B, Hq, Tq]")
     same_device(q, dout, out, lse)
-    no_grad(dout, out)
+    no_grad(dout, out, lse)
     e = 4 if dt is torch.float32 else 2
     dout, out, lse = _lay(dout, e), _lay(out, e), lse.contiguous()
     ins = (q, k, v, dout, out)

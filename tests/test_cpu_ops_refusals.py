@@ -65,3 +65,27 @@ def test_places_agree_with_an_enumeration():
         nest = all(b[0] > sum((m - 1) * s for s, m in order[:i + 1]) for i, b in enumerate(order[1:]))
         assert _apart(torch.zeros(256).as_strided(n, st)) == nest
         assert not nest or len(set(seen)) == len(seen)
+
+
+def test_forward_mode_tangents_are_refused(anywhere):
+    """An operator that records nothing must not drop a tangent, under torch.no_grad() no more than without it."""
+    import torch.autograd.forward_ad as fw
+    from ifd.attention import attention, attention_bwd
+    from ifd.rotary import qk_norm_rope, qk_norm_rope_bwd
+    q, k, v = _qkv()
+    w, lse = torch.ones(16), torch.zeros(2, 4, 6)
+    with fw.dual_level():
+        d = lambda t: fw.make_dual(t, torch.ones_like(t))  # noqa: E731
+        calls = [lambda: attention(d(q), k, v), lambda: attention(q, d(k), v), lambda: attention(q, k, d(v)),
+                 lambda: attention_bwd(d(q), q, k, v, q, lse), lambda: attention_bwd(q, q, k, v, d(q), lse),
+                 lambda: attention_bwd(q, q, k, v, q, d(lse)), lambda: attention_bwd(q, q, k, d(v), q, lse),
+                 lambda: qk_norm_rope(q, d(k)), lambda: qk_norm_rope(q, k, d(w)), lambda: qk_norm_rope_bwd(q, d(k), q, k)]
+        for f in calls:
+            with pytest.raises(ValueError, match="tangent"):
+                f()
+            with torch.no_grad(), pytest.raises(ValueError, match="tangent"):
+                f()
+        with pytest.raises(AssertionError, match="not refused"):  # no tangent: the call goes on
+            attention(q, k, v)
+    with pytest.raises(ValueError, match="tangent"):
+        torch.func.jvp(lambda x: attention(x, k, v)[0], (q,), (q,))
