@@ -133,6 +133,7 @@ def output(t, like, name):
         refuse(f"{name} must be like its input")
     if not _apart(t):
         refuse(f"{name} has elements that share their place, or strides {t.stride()} that do not nest")
+    no_grad(t)
     torch.autograd.graph.increment_version(t)
     return t
 

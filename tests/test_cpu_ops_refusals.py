@@ -89,3 +89,28 @@ def test_forward_mode_tangents_are_refused(anywhere):
             attention(q, k, v)
     with pytest.raises(ValueError, match="tangent"):
         torch.func.jvp(lambda x: attention(x, k, v)[0], (q,), (q,))
+
+
+def test_outputs_that_autograd_follows_are_refused(anywhere):
+    """A caller's output that requires gradients or carries a tangent would be written behind autograd's back."""
+    import torch.autograd.forward_ad as fw
+    from ifd.attention import attention, attention_bwd
+    from ifd.rotary import qk_norm_rope, qk_norm_rope_bwd
+    q, k, v = _qkv()
+    lse = torch.zeros(2, 4, 6)
+    calls = lambda o: [lambda: attention(q, k, v, out=o), lambda: qk_norm_rope(q, k, q_out=o),  # noqa: E731
+                       lambda: attention_bwd(q, q, k, v, q, lse, dq=o), lambda: qk_norm_rope_bwd(q, k, q, k, dq=o)]
+    leaf = torch.zeros(2, 6, 4, 16, requires_grad=True)
+    for o in (leaf, leaf * 2, leaf[:]):
+        was = o._version
+        for f in calls(o):
+            with pytest.raises(ValueError, match="records no gradients"):
+                f()
+            assert o._version == was
+            with torch.no_grad(), pytest.raises(AssertionError, match="not refused"):
+                f()
+            was = o._version
+    with fw.dual_level():
+        for f in calls(fw.make_dual(torch.zeros(2, 6, 4, 16), torch.ones(2, 6, 4, 16))):
+            with torch.no_grad(), pytest.raises(ValueError, match="tangent"):
+                f()
