@@ -3,9 +3,10 @@
     opt = AdamW(params, lr=5e-5, weight_decay=0.01, max_norm=1.0, state_bits=8)
     opt.step(grads)                     # or opt.step() with the parameters' .grad
 
-params: a list of tensors, or of groups {"params": [...], "lr": ..., "weight_decay": ...}; fp32, bf16 or fp16, contiguous, on
-one GPU; gradients likewise, of any of these types. The arithmetic is torch.optim.AdamW's (decoupled decay, bias correction),
-with clip_grad_norm_(max_norm) over all tensors folded in (the gradients themselves are not changed).
+params: a list of tensors, or of groups {"params": [...], "lr": ..., "weight_decay": ...} ("params" may be one tensor); fp32,
+bf16 or fp16, contiguous, on one GPU; gradients likewise, of any of these types. The arithmetic is torch.optim.AdamW's
+(decoupled decay, bias correction), with clip_grad_norm_(max_norm) over all tensors folded in (the gradients themselves are
+not changed).
 
 State memory: 8 bytes a value with state_bits=32, 2 with state_bits=8 (a byte per moment and one scale per 256 values; the
 format and its rounding are described in include/ifd_ops.h). The step uses the moments before they are rounded.
@@ -37,11 +38,13 @@ class AdamW:
         need(0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0, f"betas must be in [0, 1), got {betas}")
         need(eps > 0.0 and lr >= 0.0 and weight_decay >= 0.0, "eps must be positive, lr and weight_decay not negative")
         need(max_norm is None or max_norm > 0.0, f"max_norm must be positive or None, got {max_norm}")
+        need(not isinstance(params, (torch.Tensor, dict)), "params: a list of tensors or of groups")
         params = list(params)
         if params and not isinstance(params[0], dict):
             params = [{"params": params}]
         need(all(isinstance(g, dict) for g in params), "params: a list of tensors or of groups")
-        self.groups = [{"lr": lr, "weight_decay": weight_decay, **g, "params": list(g["params"])} for g in params]
+        one = lambda p: [p] if isinstance(p, torch.Tensor) else list(p)  # noqa: E731
+        self.groups = [{"lr": lr, "weight_decay": weight_decay, **g, "params": one(g["params"])} for g in params]
         self.params = [p for g in self.groups for p in g["params"]]
         need(self.params, "no parameters")
         self.betas, self.eps, self.max_norm, self.state_bits = tuple(betas), float(eps), max_norm, state_bits

@@ -114,3 +114,14 @@ def test_outputs_that_autograd_follows_are_refused(anywhere):
         for f in calls(fw.make_dual(torch.zeros(2, 6, 4, 16), torch.ones(2, 6, 4, 16))):
             with torch.no_grad(), pytest.raises(ValueError, match="tangent"):
                 f()
+
+
+def test_optimizer_takes_no_tensor_for_a_list(anywhere):
+    """A tensor walks over its rows: views of their own that never have a .grad. One tensor as a group's "params" is that
+    tensor, as in torch.optim; in the list's place it is refused."""
+    from ifd.optim import AdamW
+    w = torch.nn.Parameter(torch.zeros(3, 4))
+    assert AdamW([{"params": w}, {"params": [torch.zeros(5)]}]).params[0] is w
+    with pytest.raises(ValueError, match="a list of tensors or of groups"):
+        AdamW(w)
+    assert len(AdamW(iter([w, torch.zeros(2)])).params) == 2
