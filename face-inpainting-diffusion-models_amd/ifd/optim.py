@@ -43,6 +43,11 @@ class AdamW:
         if params and not isinstance(params[0], dict):
             params = [{"params": params}]
         need(all(isinstance(g, dict) for g in params), "params: a list of tensors or of groups")
+        for g in params:
+            need("params" in g, "a group without params")
+            other = sorted(set(g) - {"params", "lr", "weight_decay"})
+            need(not other, f"a group sets its lr and weight_decay alone, not {', '.join(map(str, other))}")
+            need(g.get("lr", lr) >= 0.0 and g.get("weight_decay", weight_decay) >= 0.0, "a group's lr and weight_decay: not negative")
         one = lambda p: [p] if isinstance(p, torch.Tensor) else list(p)  # noqa: E731
         self.groups = [{"lr": lr, "weight_decay": weight_decay, **g, "params": one(g["params"])} for g in params]
         self.params = [p for g in self.groups for p in g["params"]]

@@ -125,3 +125,17 @@ def test_optimizer_takes_no_tensor_for_a_list(anywhere):
     with pytest.raises(ValueError, match="a list of tensors or of groups"):
         AdamW(w)
     assert len(AdamW(iter([w, torch.zeros(2)])).params) == 2
+
+
+def test_group_options_are_not_ignored(anywhere):
+    """betas, eps, max_norm and the rest belong to the optimizer: a group that sets one is refused, as are rates below 0 in a
+    group and a group without parameters."""
+    from ifd.optim import AdamW
+    p = torch.zeros(5)
+    for g, msg in (({"params": [p], "betas": (0.5, 0.9)}, "betas"), ({"params": [p], "eps": 1e-3}, "eps"),
+                   ({"params": [p], "amsgrad": True}, "amsgrad"), ({"params": [p], "lr": -1.0}, "not negative"),
+                   ({"params": [p], "weight_decay": float("nan")}, "not negative"), ({"lr": 1.0}, "params")):
+        with pytest.raises(ValueError, match=msg):
+            AdamW([g])
+    o = AdamW([{"params": [p], "lr": 0.5, "weight_decay": 0.0}], lr=1.0, weight_decay=1.0)
+    assert o.groups[0]["lr"] == 0.5 and o.groups[0]["weight_decay"] == 0.0
