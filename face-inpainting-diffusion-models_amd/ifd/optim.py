@@ -148,12 +148,15 @@ class AdamW:
 
     def load_moments(self, m, v, m_scale=None, v_scale=None):
         """Copies states in, in the layout of m, v (and m_scale, v_scale) of this optimizer."""
-        for n, t in (("m", m), ("v", v), ("m_scale", m_scale), ("v_scale", v_scale)):
+        given = {"m": m, "v": v, "m_scale": m_scale, "v_scale": v_scale}
+        for n, t in given.items():
             own = getattr(self, n)
             need((own is None) == (t is None), f"{n}: {'not used with' if own is None else 'needed with'} {self.state_bits}-bit states")
             if own is not None:
                 need(t.dtype == own.dtype and t.shape == own.shape, f"{n} must be {own.dtype} {tuple(own.shape)}")
-                own.copy_(t)
+        for n, t in given.items():
+            if t is not None:
+                getattr(self, n).copy_(t)
 
     def state_dict(self):
         """Everything a resumed run needs, bit for bit (copies)."""
@@ -163,5 +166,7 @@ class AdamW:
 
     def load_state_dict(self, d):
         need(d["state_bits"] == self.state_bits, f"states of {d['state_bits']} bits for an optimizer of {self.state_bits}")
+        step, seed = int(d["step"]), int(d["seed"]) & 0xFFFFFFFF
+        need(step >= 0, f"a step number of {step}")
         self.load_moments(d["m"], d["v"], d.get("m_scale"), d.get("v_scale"))
-        self.step_count, self.seed = int(d["step"]), int(d["seed"])
+        self.step_count, self.seed = step, seed

@@ -139,3 +139,26 @@ def test_group_options_are_not_ignored(anywhere):
             AdamW([g])
     o = AdamW([{"params": [p], "lr": 0.5, "weight_decay": 0.0}], lr=1.0, weight_decay=1.0)
     assert o.groups[0]["lr"] == 0.5 and o.groups[0]["weight_decay"] == 0.0
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_refused_states_change_nothing(anywhere, bits):
+    """load_moments and load_state_dict look at every part before they copy one."""
+    from ifd.optim import AdamW
+    src, dst = AdamW([torch.zeros(300)], state_bits=bits, seed=3), AdamW([torch.zeros(300)], state_bits=bits)
+    for t in (src.m, src.v, src.m_scale, src.v_scale):
+        if t is not None:
+            t.fill_(7)
+    src.step_count = 9
+    good = src.state_dict()
+    bad = [{**good, "v": good["v"][:-1]}, {**good, "v": None}, {k: v for k, v in good.items() if k != "step"},
+           {k: v for k, v in good.items() if k != "seed"}, {**good, "state_bits": 40 - bits}, {**good, "step": -1}]
+    if bits == 8:
+        bad += [{**good, "v_scale": None}, {**good, "v_scale": good["v_scale"].double()}]
+    for d in bad:
+        with pytest.raises((ValueError, KeyError)):
+            dst.load_state_dict(d)
+        assert dst.step_count == 0 and dst.seed == 0
+        assert all((t == 0).all() for t in (dst.m, dst.v, dst.m_scale, dst.v_scale) if t is not None)
+    dst.load_state_dict(good)
+    assert dst.step_count == 9 and dst.seed == 3 and (dst.m == 7).all() and (dst.v == 7).all()
