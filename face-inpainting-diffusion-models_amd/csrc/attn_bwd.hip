@@ -411,7 +411,7 @@ __device__ __forceinline__ void attn_bwd_kv(const AttnK& p, lds_c* sm, int blk) 
   if (key >= p.Tk) return;
   if (p.nsplit > 1) {
     if (!ok) return;
-    float* po = p.ws + 2 * (int64_t)p.B * p.Hq * p.Tq + ((((int64_t)b * p.Hk + hk) * p.nsplit + sp) * p.Tk + key) * (2 * DP);
+    float* po = p.ws_kv + ((((int64_t)b * p.Hk + hk) * p.nsplit + sp) * p.Tk + key) * (2 * DP);
 #pragma unroll
     for (int d = 0; d < TL::DT; ++d)
 #pragma unroll
@@ -495,7 +495,7 @@ __global__ __launch_bounds__(256) void attn_bwd_join_kernel(AttnK p, int nkv) {
   const int key = (int)(row - bh * p.Tk), b = (int)(bh / p.Hk), hk = (int)(bh - (int64_t)b * p.Hk);
   f32x4 v = {0.f, 0.f, 0.f, 0.f};
   if (key < row_limit(p, q_first(p, b), seq_len(p, b), p.Tq - 1)) {
-    const float* w = p.ws + 2 * (int64_t)p.B * p.Hq * p.Tq + (bh * p.nsplit * p.Tk + key) * (2 * DP) + isv * DP + ch;
+    const float* w = p.ws_kv + (bh * p.nsplit * p.Tk + key) * (2 * DP) + isv * DP + ch;
     for (int s = 0; s < p.nsplit; ++s) v += *reinterpret_cast<const f32x4*>(w + (int64_t)s * p.Tk * (2 * DP));
     if (!isv) v *= p.scale;
   }
@@ -589,17 +589,18 @@ static int run_bwd_d(const AttnK& p, hipStream_t s) {
 using namespace ifd;
 extern "C" {
 
-// floats of workspace: lse2 and delta, the key pass' shares (both `head`), the row pass' shares
-static void bwd_ws(const ifd_attention_args& a, int64_t& head, int64_t& all) {
+// floats of workspace up to where the key pass' shares begin (behind lse2 and delta, on 16 bytes), the row pass', and the end
+static void bwd_ws(const ifd_attention_args& a, int64_t& kv, int64_t& q, int64_t& all) {
   const int64_t dp = a.D <= 64 ? 64 : a.D <= 96 ? 96 : 128, n = kv_split(a), nq = q_split(a), rows = (int64_t)a.B * a.Hq * a.Tq;
-  head = 2 * rows + (n > 1 ? (int64_t)a.B * a.Hk * n * a.Tk * 2 * dp : 0);
-  all = head + (nq > 1 ? rows * nq * dp : 0);
+  kv = (2 * rows + 3) & ~(int64_t)3;
+  q = kv + (n > 1 ? (int64_t)a.B * a.Hk * n * a.Tk * 2 * dp : 0);
+  all = q + (nq > 1 ? rows * nq * dp : 0);
 }
 
 int64_t ifd_op_attention_bwd_ws_bytes(const ifd_attention_args* a) {
   if (!a || attention_check(*a) || !a->B) return 0;
-  int64_t head, all;
-  bwd_ws(*a, head, all);
+  int64_t kv, q, all;
+  bwd_ws(*a, kv, q, all);
   return all * 4;
 }
 
@@ -624,10 +625,11 @@ int ifd_op_attention_bwd(const ifd_attention_args* a, void* ws, int64_t ws_bytes
                      (int64_t)a->B * a->Hk * a->Tk < (int64_t)1 << 31,
                  "sizes beyond one launch");
   AttnK p = attention_kernel_args(*a);
-  int64_t head, all;
-  bwd_ws(*a, head, all);
+  int64_t kv, q, all;
+  bwd_ws(*a, kv, q, all);
   p.ws = (float*)ws;
-  p.ws_q = p.ws + head;
+  p.ws_kv = p.ws + kv;
+  p.ws_q = p.ws + q;
   p.nsplit = n;
   p.nsplit_q = nq;
   hipStream_t s = (hipStream_t)stream;

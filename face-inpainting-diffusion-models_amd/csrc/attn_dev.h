@@ -201,7 +201,7 @@ struct AttnK {  // kernel arguments: strides in bytes
   int qt, kt, vt, ot, gt, dqt, dkt, dvt;  // token strides
   int B, Tq, Tk, Hq, Hk, D, G, causal, nblk, nsplit, nsplit_q;
   float c, scale;  // c = scale log2(e)
-  float *ws, *ws_q;
+  float *ws, *ws_kv, *ws_q;  // backward: lse2 and delta, the key pass' shares, the row pass' shares
 };
 
 __device__ __forceinline__ int seq_len(const AttnK& p, int b) {

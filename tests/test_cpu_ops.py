@@ -253,3 +253,14 @@ def test_overlap_of_parameters_and_of_two_outputs(monkeypatch):
     lse = torch.zeros(1, 2, 3)
     with pytest.raises(ValueError, match="dv overlaps"):
         attention.attention_bwd(q.clone(), q, k, k.clone(), q.clone(), lse, dk=o[:, :, :2], dv=o[:, :, :2])
+
+
+@pytest.mark.parametrize("kw", [dict(B=1, Tq=129, Tk=2100, Hq=1, Hk=1, D=128), dict(B=3, Tq=33, Tk=1000, Hq=1, Hk=1, D=64, dtype=0),
+                                dict(B=1, Tq=1, Tk=700, Hq=1, Hk=1, D=96), dict(B=1, Tq=777, Tk=777, Hq=3, Hk=3, D=80, causal=1)])
+def test_backward_workspace_parts_are_aligned(kw):
+    """The partial sums behind lse2 and delta (2 B Hq Tq floats, here an odd number of pairs) are written in 16-byte pieces:
+    their start has to be a multiple of 16 bytes, as all that follows it is."""
+    from ifd import _ops
+    assert kw["B"] * kw["Hq"] * kw["Tq"] % 2
+    n = _ops.lib().ifd_op_attention_bwd_ws_bytes(ctypes.byref(_attention_args(**kw)))
+    assert n > 8 * kw["B"] * kw["Hq"] * kw["Tq"] and n % 16 == 0
