@@ -363,6 +363,7 @@ int ifd_op_grad_norm(int nt, const void* const* g, const int64_t* n, const uint8
   IFD_OP_REQUIRE(max_norm >= 0.0, "max_norm must not be negative");
   const int64_t need = ifd_op_grad_norm_ws_bytes(nt, n);
   IFD_OP_REQUIRE(ws_bytes >= need && (ws || !need), "workspace too small");
+  IFD_OP_REQUIRE(on(ws, 8) && on(norm_coef, 8), "norm_coef or the workspace: an address off its elements");
   hipStream_t s = (hipStream_t)stream;
   double* part = (double*)ws;
   int64_t total = 0;
@@ -387,6 +388,7 @@ int ifd_op_adamw(const ifd_adamw_args* a, void* stream) {
   if (!a->nt) return 0;
   IFD_OP_REQUIRE(a->p && a->ptype && a->m && a->v && (a->bits == 32 || (a->m_scale && a->v_scale)), "a null tensor");
   IFD_OP_REQUIRE(!((uintptr_t)a->m & 15) && !((uintptr_t)a->v & 15), "states must be aligned to 16 bytes");
+  IFD_OP_REQUIRE(on(a->m_scale, 4) && on(a->v_scale, 4) && on(a->norm_coef, 8), "scales or norm_coef: an address off its elements");
   for (int i = 0; i < a->nt; ++i) {
     IFD_OP_REQUIRE(a->ptype[i] <= IFD_F16, "parameter type");
     IFD_OP_REQUIRE(a->p[i] || !a->g[i] || !a->n[i], "a gradient without its parameter");
@@ -418,6 +420,7 @@ int ifd_op_state_values(const void* m, const float* m_scale, const void* v, cons
   IFD_OP_REQUIRE(m && v && m_scale && v_scale && m_out && v_out, "a null tensor");
   IFD_OP_REQUIRE(!(((uintptr_t)m | (uintptr_t)v) & 3) && !(((uintptr_t)m_out | (uintptr_t)v_out) & 15),
                  "states must be aligned to 4 bytes, outputs to 16");
+  IFD_OP_REQUIRE(on(m_scale, 4) && on(v_scale, 4), "a scale's address is off its elements");
   hipLaunchKernelGGL(state_values_kernel, dim3((unsigned)std::min<int64_t>(cdiv(nblocks, 4), 16384)), dim3(256), 0,
                      (hipStream_t)stream, (const unsigned*)m, m_scale, (const unsigned*)v, v_scale, nblocks * 64,
                      (f32x4*)m_out, (f32x4*)v_out);

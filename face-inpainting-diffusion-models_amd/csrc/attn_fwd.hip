@@ -475,6 +475,7 @@ const char* attention_check(const ifd_attention_args& a) {
   if (!(a.scale > 0.f) || !(a.scale < 3e38f)) return "scale must be positive and finite";
   if (a.Tk > 0x3fffffff || (int64_t)a.Tq * (a.Hq / a.Hk) > 0x3fffffff || (int64_t)a.B * a.Hq > 0x3fffffff)
     return "sizes beyond 2^30 rows";
+  if (!on(a.lse, 4) || !on(a.kv_len, 4) || !on(a.q_start, 4)) return "lse, kv_len or q_start: an address off its elements";
   return nullptr;
 }
 

@@ -18,6 +18,9 @@ inline int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
     }                                                                                    \
   } while (0)
 
+// p is null or starts on a multiple of n bytes
+inline bool on(const void* p, int64_t n) { return ((uintptr_t)p & (uintptr_t)(n - 1)) == 0; }
+
 // The checks that both directions of attention share; nullptr, or what is wrong.
 const char* attention_check(const ifd_attention_args& a);
 

@@ -233,6 +233,11 @@ static const char* qk_check(const ifd_qk_args& a) {
     if (s > lim || s < -lim) return "a token's heads reach over more than 2 GiB";
   if ((int64_t)a.Hq + a.Hk > 1 << 20 || (int64_t)a.B * a.T * (a.Hq + a.Hk) >= (int64_t)1 << 31)
     return "sizes: 2^31 head rows and more";
+  const int64_t es = dtype_bytes(a.dtype);
+  for (const void* t : {a.q, a.k, a.gq, a.gk, (const void*)a.q_out, (const void*)a.k_out, (const void*)a.dq, (const void*)a.dk})
+    if (!on(t, es)) return "a tensor's address off its elements";
+  if (!on(a.wq, 4) || !on(a.wk, 4) || !on(a.dwq, 4) || !on(a.dwk, 4) || !on(a.pos, 8) || !on(a.turns, 8))
+    return "weights, positions or frequencies: an address off its elements";
   return nullptr;
 }
 
@@ -338,6 +343,7 @@ int ifd_op_qk_norm_rope_bwd(const ifd_qk_args* a, void* ws, int64_t ws_bytes, vo
   IFD_OP_REQUIRE(none || !a->rot || (a->pos && a->turns), "a rotation without positions or frequencies");
   const int64_t need = ifd_op_qk_norm_rope_bwd_ws_bytes(a);
   IFD_OP_REQUIRE(ws_bytes >= need && (ws || !need), "workspace too small");
+  IFD_OP_REQUIRE(on(ws, 4), "the workspace's address is off its elements");
   hipStream_t s = (hipStream_t)stream;
   int nwg = 0;
   if (!none) {

@@ -57,8 +57,8 @@ int ifd_op_attention_bwd(const ifd_attention_args* a, void* ws, int64_t ws_bytes
  *   the first `rot` channels in pairs (i, i + rot / 2), or (2i, 2i + 1) with interleaved != 0, turned by the angle
  *   2 pi pos turns[i] and scaled by mscale; the other channels are n.
  * q, k, their outputs and gradients: [B][T][Hq | Hk][D] of one type, strides {batch, token, head} in elements, channels
- * adjacent (any alignment; 16 bytes is fastest). Hq or Hk may be 0. An output may be its input (in place). pos int64 with
- * strides {batch, token} (0: shared); turns fp64 [rot / 2]: frequency / 2 pi. D <= 128, even. */
+ * adjacent (on a multiple of an element; 16 bytes is fastest). Hq or Hk may be 0. An output may be its input (in place).
+ * pos int64 with strides {batch, token} (0: shared); turns fp64 [rot / 2]: frequency / 2 pi. D <= 128, even. */
 typedef struct ifd_qk_args {
   int dtype, B, T, Hq, Hk, D, rot, interleaved, norm;
   float eps, mscale;

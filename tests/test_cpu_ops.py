@@ -264,3 +264,42 @@ def test_backward_workspace_parts_are_aligned(kw):
     assert kw["B"] * kw["Hq"] * kw["Tq"] % 2
     n = _ops.lib().ifd_op_attention_bwd_ws_bytes(ctypes.byref(_attention_args(**kw)))
     assert n > 8 * kw["B"] * kw["Hq"] * kw["Tq"] and n % 16 == 0
+
+
+def test_addresses_off_their_elements_are_refused():
+    """Every array that a kernel reads or writes element by element starts on a multiple of its element."""
+    from ifd import _lib, _ops
+    L, keep = _ops.lib(), []
+    for n in ("lse", "kv_len", "q_start"):
+        a = _attention_args()
+        setattr(a, n, 0x10002)
+        for name in ("ifd_op_attention", "ifd_op_attention_bwd"):
+            with pytest.raises(RuntimeError, match=name + ": .*address"):
+                _lib.check(getattr(L, name)(ctypes.byref(a), 0x10000, 1 << 40, None))
+    good = dict(dtype=1, B=1, T=2, Hq=2, Hk=1, D=64, rot=64, norm=1, eps=1e-6, mscale=1.0)
+    ptrs = ("q", "k", "q_out", "k_out", "gq", "gk", "dq", "dk", "wq", "wk", "pos", "turns", "dwq", "dwk")
+    for n in ptrs:
+        a = _ops.QkArgs(**good)
+        for m in ptrs:
+            setattr(a, m, 0x10000)
+        setattr(a, n, 0x10001 if n[0] in "qkgd" and n[:2] != "dw" else 0x10002 if n[0] in "wd" else 0x10004)
+        if n not in ("gq", "gk", "dq", "dk", "dwq", "dwk"):
+            with pytest.raises(RuntimeError, match="ifd_op_qk_norm_rope: .*address"):
+                _lib.check(L.ifd_op_qk_norm_rope(ctypes.byref(a), None))
+        if n not in ("q_out", "k_out"):
+            with pytest.raises(RuntimeError, match="ifd_op_qk_norm_rope_bwd: .*address"):
+                _lib.check(L.ifd_op_qk_norm_rope_bwd(ctypes.byref(a), 0x10000, 1 << 30, None))
+    with pytest.raises(RuntimeError, match="ifd_op_qk_norm_rope_bwd: .*address"):
+        for m in ptrs:
+            setattr(a, m, 0x10000)
+        _lib.check(L.ifd_op_qk_norm_rope_bwd(ctypes.byref(a), 0x10002, 1 << 30, None))
+    n, g, t = (ctypes.c_int64 * 1)(5000), (ctypes.c_void_p * 1)(0x20000), (ctypes.c_uint8 * 1)(0)
+    for coef, ws in ((0x30004, 0x30000), (0x30000, 0x30004)):
+        with pytest.raises(RuntimeError, match="ifd_op_grad_norm: .*address"):
+            _lib.check(L.ifd_op_grad_norm(1, g, n, t, 1.0, coef, ws, 1 << 20, None))
+    for kw in (dict(m_scale=0x30002), dict(v_scale=0x30001), dict(norm_coef=0x30004)):
+        with pytest.raises(RuntimeError, match="ifd_op_adamw: .*address"):
+            _lib.check(L.ifd_op_adamw(ctypes.byref(_adamw_args(keep, **kw)), None))
+    for args in ((0x10, 0x2, 0x10, 0x10), (0x10, 0x10, 0x10, 0x2)):
+        with pytest.raises(RuntimeError, match="ifd_op_state_values: .*address"):
+            _lib.check(L.ifd_op_state_values(*args, 4, 0x10, 0x10, None))
