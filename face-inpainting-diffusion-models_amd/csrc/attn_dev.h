@@ -67,12 +67,14 @@ struct AttnT<float> {
   }
 };
 
+// Bytes of a head's row in LDS: the head width that the products cover (dp: 64, 96 or 128), rounded to a power of two
+constexpr int attn_row_bytes(int dp, int es) { return (dp == 96 ? 128 : dp) * es; }
+
 template <typename T, int DP>
 struct AttnTile {
   typedef AttnT<T> A;
   typedef typename A::frag frag;
-  // DP: the head width the products cover (64, 96 or 128); a row in LDS takes the next power of two
-  static constexpr int ES = sizeof(T), CE = 16 / ES, NCH = (DP == 96 ? 128 : DP) / CE, ROWB = NCH * 16;
+  static constexpr int ES = sizeof(T), CE = 16 / ES, ROWB = attn_row_bytes(DP, ES), NCH = ROWB / 16;
   static constexpr int KS = DP / CE / 2, DT = DP / 32, PS = A::PS;
 
   static __device__ __forceinline__ int swz(int r) {

@@ -495,6 +495,9 @@ struct FwdPlan {
   int64_t wgs;
 };
 
+// Keys of a tile of attn_fwd_kernel
+constexpr int rows_tile(int dp, int es) { return attn_row_bytes(dp, es) >= 512 ? 32 : 64; }
+
 // Which kernel, and into how many shares of the keys. attn_split_kernel reads every key once for all heads of a group, but
 // its waves share no tiles: it is taken for up to 32 rows a head, or 128 rows a group of narrow heads (us, it against
 // attn_fwd_kernel: 2 x 8|4 heads x 24 x 3000 x 96 bf16 13, 18; 8 x 8|4 x 64 x 700 x 64 fp32 19, 36; the other way round
@@ -503,7 +506,9 @@ struct FwdPlan {
 // bf16 103, 36; 3 x 6|3 x 500 x 3000 x 80 fp32 348, 131; 2 x 8 x 1024 x 4096 x 64 fp16 58, 38; with 256 workgroups in one
 // share already, 4 x 8 x 1024 x 1024 x 64, two take 29 instead of 21), of eight tiles at least, four in fp32, whose tiles
 // take longer to multiply (4 x 8|2 x 100 x 4096 x 128 bf16 27 in shares of eight tiles, 30 of four; 2 x 4 x 700 x 128 fp32
-// causal 62 and 37).
+// causal 62 and 37). fp32 heads of 65 to 96 channels, whose tiles multiply faster for as much to join, take four only up to
+// one workgroup a CU (2 x 4 x 700 x 80 causal 51 in shares of eight tiles, 32 of four; 1 x 2 x 2000 x 80 47 as 256 workgroups,
+// 52 as 480; but 3 x 3 x 500 x 3000 x 80 77 and 64).
 static FwdPlan fwd_plan(const ifd_attention_args& a) {
   const int G = a.Hq / a.Hk, es = (int)dtype_bytes(a.dtype);
   FwdPlan r;
@@ -512,8 +517,10 @@ static FwdPlan fwd_plan(const ifd_attention_args& a) {
   if (!r.few) {
     r.dp = a.D <= 64 ? 64 : a.D <= 96 ? 96 : 128;
     r.wgs = cdiv(a.Tq, 128) * a.B * a.Hq;
-    const int64_t tiles = cdiv(a.Tk, r.dp * es >= 512 ? 32 : 64);
-    r.nsplit = r.wgs > 128 ? 1 : (int)std::max<int64_t>(1, std::min<int64_t>({512 / r.wgs, tiles / (es == 4 ? 4 : 8), 64}));
+    const int64_t tiles = cdiv(a.Tk, rows_tile(r.dp, es));
+    int64_t n = es == 4 ? tiles / 4 : tiles / 8;
+    if (es == 4 && r.dp == 96 && r.wgs <= 128) n = std::max(tiles / 8, std::min(n, 256 / r.wgs));
+    r.nsplit = r.wgs > 128 ? 1 : (int)std::max<int64_t>(1, std::min<int64_t>({512 / r.wgs, n, 64}));
   } else {
     r.dp = a.D <= 64 ? 64 : 128;
     r.wgs = cdiv(rows, 32) * a.B * a.Hk;
@@ -547,7 +554,7 @@ AttnK attention_kernel_args(const ifd_attention_args& a) {
 
 template <typename T, int DP, bool SPLIT>
 static int run_rows(const AttnK& p, int64_t wgs, hipStream_t s) {
-  constexpr int ROWB = AttnTile<T, DP>::ROWB, BK = ROWB >= 512 ? 32 : 64, OCC = ROWB == 128 ? 4 : ROWB == 256 ? 2 : 1;
+  constexpr int ROWB = AttnTile<T, DP>::ROWB, BK = rows_tile(DP, sizeof(T)), OCC = ROWB == 128 ? 4 : ROWB == 256 ? 2 : 1;
   constexpr int lds = 4 * BK * ROWB;
   static bool attr[kMaxDevices] = {};
   auto kern = attn_fwd_kernel<T, DP, BK, OCC, SPLIT>;

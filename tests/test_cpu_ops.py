@@ -303,3 +303,18 @@ def test_addresses_off_their_elements_are_refused():
     for args in ((0x10, 0x2, 0x10, 0x10), (0x10, 0x10, 0x10, 0x2)):
         with pytest.raises(RuntimeError, match="ifd_op_state_values: .*address"):
             _lib.check(L.ifd_op_state_values(*args, 4, 0x10, 0x10, None))
+
+
+def test_shares_of_wide_fp32_heads_count_the_kernels_tiles():
+    """Shares of the keys in the many-row forward kernel: four tiles at least in fp32, and a tile of heads of 65 to 128
+    channels is 32 keys (64 of narrower ones). 700 keys of 80 channels are 22 tiles, five shares, and not half as many. Heads
+    of 65 to 96 channels take eight tiles where four would make more than 256 workgroups."""
+    from ifd import _ops
+    for D, dp, keys in ((64, 64, 64), (80, 96, 32), (96, 96, 32), (128, 128, 32)):
+        for Tq, Tk in ((700, 700), (200, 3000), (129, 257), (2000, 2000), (500, 1100)):
+            kw = dict(dtype=0, B=1, Tq=Tq, Tk=Tk, Hq=4, Hk=4, D=D)
+            n = _ops.lib().ifd_op_attention_ws_bytes(ctypes.byref(_attention_args(**kw)))
+            wgs, tiles = -(-Tq // 128) * 4, -(-Tk // keys)
+            shares = max(tiles // 8, min(tiles // 4, 256 // wgs)) if dp == 96 else tiles // 4
+            want = min(512 // wgs, shares, 64)
+            assert n == (4 * Tq * want * (dp + 4) * 4 if want > 1 else 0), (D, Tq, Tk)
