@@ -89,11 +89,7 @@ __global__ __launch_bounds__(256) void skinny_kernel(const float* __restrict__ i
 #pragma unroll
     for (int q = 0; q < SK_NB; ++q) acc[q] = 0.f;
     if (j < J) {
-      // (16 weight loads in flight per wave: the loop is latency-bound at ~1 wave per SIMD; the
-      // accumulation order per slot is unchanged)
-#pragma unroll 16
-      for (int kk = k0; kk < k0 + kc; ++kk) {
-        const float w = wt[(size_t)kk * J + j];
+      auto add = [&](int kk, float w) {
         const f32x4* s4 = reinterpret_cast<const f32x4*>(sk + (size_t)kk * SK_NB);
 #pragma unroll
         for (int g = 0; g < SK_NB / 4; ++g) {
@@ -101,7 +97,19 @@ __global__ __launch_bounds__(256) void skinny_kernel(const float* __restrict__ i
 #pragma unroll
           for (int c = 0; c < 4; ++c) acc[4 * g + c] = fmaf(w, s[c], acc[4 * g + c]);  // one rounding in every slot
         }
+      };
+      // The loop is latency-bound at ~1 wave per SIMD: 16 weights are read ahead of the products that take them (left to the
+      // scheduler, they are read one at a time). The accumulation order per slot is that of the plain loop.
+      int kk = k0;
+      for (; kk + 16 <= k0 + kc; kk += 16) {
+        float w[16];
+#pragma unroll
+        for (int u = 0; u < 16; ++u) w[u] = wt[(size_t)(kk + u) * J + j];
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int u = 0; u < 16; ++u) add(kk + u, w[u]);
       }
+      for (; kk < k0 + kc; ++kk) add(kk, wt[(size_t)kk * J + j]);
     }
 #pragma unroll
     for (int q = 0; q < SK_NB; ++q) red[(kq * SK_NB + q) * SK_JB + jj] = acc[q];
