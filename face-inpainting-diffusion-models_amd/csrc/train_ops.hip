@@ -1986,11 +1986,18 @@ __global__ __launch_bounds__(256) void attn_bwd_cols_kernel(const float* __restr
   for (int t = 0; t < T; ++t) {
     const float qv = base[(int64_t)t * row + qo + lane];
     const float dov = dob[(int64_t)t * C + head * 64 + lane];
+    float ds[AB_R / 4], p[AB_R / 4];
 #pragma unroll
     for (int i = 0; i < AB_R / 4; ++i) {
       const int s = min(s0 + wave + 4 * i, T - 1);
-      dk[i] += dSm[mo + (int64_t)t * T + s] * qv;
-      dv[i] += Pm[mo + (int64_t)t * T + s] * dov;
+      ds[i] = dSm[mo + (int64_t)t * T + s];
+      p[i] = Pm[mo + (int64_t)t * T + s];
+    }
+    __builtin_amdgcn_sched_barrier(0);  // all loads ahead of the sums (left to the scheduler, they are read one at a time)
+#pragma unroll
+    for (int i = 0; i < AB_R / 4; ++i) {
+      dk[i] += ds[i] * qv;
+      dv[i] += p[i] * dov;
     }
   }
 #pragma unroll

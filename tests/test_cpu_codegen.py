@@ -58,3 +58,13 @@ def misc(tmp_path_factory):
 
 def test_embedding_layers_keep_16_weight_loads_in_flight(misc):
     assert _in_flight(_kernel(misc, "skinny_kernel")) >= 16
+
+
+@pytest.fixture(scope="module")
+def train_ops(tmp_path_factory):
+    return _assembly("train_ops", tmp_path_factory.mktemp("asm"))
+
+
+def test_attention_backward_of_odd_maps_reads_a_row_at_once(train_ops):
+    """Per query row: q, dout and the probabilities and their gradients of eight keys, 18 loads."""
+    assert _in_flight(_kernel(train_ops, "attn_bwd_cols_kernel")) >= 18
