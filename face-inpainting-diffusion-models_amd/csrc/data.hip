@@ -133,7 +133,19 @@ __global__ void resample_v_kernel(const unsigned char* __restrict__ in, int Hsrc
   const int ymin = bounds[2 * yy] - yshift, ymax = bounds[2 * yy + 1];
   const unsigned char* col = in + (n * Hsrc) * WC + xc;
   int ss = 1 << (PB - 1);
-  for (int y = 0; y < ymax; ++y) ss += (int)col[(int64_t)(ymin + y) * WC] * kk[yy * ksize + y];
+  int y = 0;
+  for (; y + 4 <= ymax; y += 4) {  // four taps' loads ahead of their sums (integers: the order changes nothing)
+    int v[4], k[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      v[u] = col[(int64_t)(ymin + y + u) * WC];
+      k[u] = kk[yy * ksize + y + u];
+    }
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) ss += v[u] * k[u];
+  }
+  for (; y < ymax; ++y) ss += (int)col[(int64_t)(ymin + y) * WC] * kk[yy * ksize + y];
   out[i] = clip8(ss);
 }
 

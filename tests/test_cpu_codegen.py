@@ -68,3 +68,8 @@ def train_ops(tmp_path_factory):
 def test_attention_backward_of_odd_maps_reads_a_row_at_once(train_ops):
     """Per query row: q, dout and the probabilities and their gradients of eight keys, 18 loads."""
     assert _in_flight(_kernel(train_ops, "attn_bwd_cols_kernel")) >= 18
+
+
+def test_vertical_resampling_reads_rows_ahead(tmp_path):
+    """Four taps: four pixels, and their coefficients in one load."""
+    assert _in_flight(_kernel(_assembly("data", tmp_path), "resample_v_kernel")) >= 5
