@@ -6,8 +6,9 @@
 // attn_bwd_kv_kernel (a wave owns 32 keys; four products). Seven products against the five of one pass with atomics on dq.
 // Short calls run both side by side in one launch (attn_bwd_both_kernel). Where there are few workgroups each pass deals its
 // walk out in shares (q_split, kv_split), whose fp32 sums attn_bwd_join_kernel adds in order.
-// Bound by the matrix units: 2 x 16|4 heads x 4096 x 128 bf16 causal 488 us (traced: row pass 215, key pass 280, join 23), 985
-// TFLOP/s over the seven products; 16 x 4 x 1024 x 64 fp32 484 us, 124 TFLOP/s, matrix units 78 % busy.
+// Bound by the matrix units: 2 x 16|4 heads x 4096 x 128 bf16 causal 491 us, 980 TFLOP/s over the seven products (traced, at
+// lower clocks: row pass 223, key pass 292, join 23), matrix units busy in 57 and 55 % of the cycles; 16 x 4 x 1024 x 64 fp32
+// 487 us, 123 TFLOP/s (traced: 228, 307), busy in 83 and 81 %.
 #include "attn_dev.h"
 
 namespace ifd {
@@ -505,7 +506,7 @@ __global__ __launch_bounds__(256) void attn_bwd_join_kernel(AttnK p, int nkv) {
 }
 
 // Shares of the row pass, whose workgroups else walk over all keys one after the other: where they are few, up to 128 of them
-// with two tiles of keys in fp32 and four in 16 bits, up to 192 with twice as many (us, in one share and so: 2 x 3 heads x
+// with 128 keys in fp32 and 256 in 16 bits, up to 192 with twice as many (us, in one share and so: 2 x 3 heads x
 // 1000 x 64 fp32 114, 79; 3 x 4 x 500 x 128 fp32 causal 126, 80; 1 x 4 x 2048 x 64 bf16 causal 48, 35; 1 x 8 x 1024 x 128 bf16
 // causal 46, 39, 45 with 256 workgroups; 8 x 4|2 x 300 x 40 fp32 causal 49, 65 with 192 of one or two tiles).
 static int q_split(const ifd_attention_args& a) {
@@ -541,8 +542,8 @@ static int run_bwd(const AttnK& p, hipStream_t s) {
   typedef AttnTile<T, DP> TL;
   constexpr int ROWB = TL::ROWB, BK = ROWB >= 512 ? 32 : 64, OCC = ROWB >= 512 ? 1 : 2;
   constexpr int AHEAD = sizeof(T) == 4 && DP == 64 ? 1 : TL::KS % 4 ? 3 : 4;  // (fp32 has no registers to read ahead into)
-  // V in LDS where K, V and both results together pass the registers (16-bit 2 x 16|4 heads x 4096 x 128 causal 583 -> 553 us
-  // traced, fp32 16 x 4 x 1024 x 64 502 -> 485)
+  // V in LDS where K, V and both results together pass the registers (the whole backward, in registers and so: 16-bit 2 x
+  // 16|4 heads x 4096 x 128 causal 583, 553 us traced; fp32 16 x 4 x 1024 x 64 502, 485 untraced)
   constexpr bool VL = sizeof(T) == 2 ? DP == 128 : DP == 64;
   constexpr int BQ = VL ? 32 : BK;
   constexpr int lds_q = 4 * BK * ROWB, lds_kv = 4 * BQ * ROWB + (VL ? 128 * ROWB : 0);  // (without lse2 and delta)

@@ -116,7 +116,10 @@ struct AttnTile {
       return f;
     }
   }
-  // a result tile's registers of contraction step t, rounded to T (16-bit: nearest, once)
+  // a result tile's registers of contraction step t as an operand. In the 16-bit types P and dS are rounded to T here, to
+  // nearest, once: the matrix units take no wider operand at their rate (fp32 products run at an eighth of it). The results'
+  // error grows from 1.7e-3 of their norm, their own rounding, to 2.3e-3 (bf16; fp16 2.1e-4 to 3.0e-4). fp16 holds dS down to
+  // 2^-24: gradients much smaller than 1 need a loss scale, as any fp16 gradient does.
   static __device__ __forceinline__ frag pack(const f32x16& s, int t) {
     frag f;
     if constexpr (ES == 2) {

@@ -129,8 +129,9 @@ __device__ __forceinline__ float* part_row(const AttnK& p, int b, int hk, int r,
 // SPLIT: the keys are dealt to nsplit workgroups, whose results attn_join_kernel joins.
 // Bound by the matrix units, in the 16-bit types with the exponentials beside them (a wave's tile of 64 keys at 64 channels:
 // 16 products of 32 cycles, 576 cycles of exponentials, scaling, sums and conversions): 4 x 8 heads x 4096 x 4096 x 64 bf16
-// 158 us, 870 TFLOP/s (four waves a SIMD, OCC; traced 179, against 189 with three and 202 with two); fp32 32 x 8 x 256 x 256 x
-// 64 43 us, 101 TFLOP/s.
+// 154 us, 890 TFLOP/s, matrix units busy in 45 % of the cycles (four waves a SIMD, OCC, for four registers spilled: in one
+// traced run 179, 189 with three, 202 with two; traced runs of it vary from 162 to 187). fp32 32 x 8 x 256 x 256 x 64 43 us, 101
+// TFLOP/s, busy in 70 %: a workgroup has four tiles, and nothing covers its first loads and its last stores.
 template <typename T, int DP, int BK, int OCC, bool SPLIT>
 __global__ __launch_bounds__(256, OCC) void attn_fwd_kernel(AttnK p) {
   typedef AttnTile<T, DP> TL;
@@ -272,7 +273,7 @@ __global__ __launch_bounds__(256, OCC) void attn_fwd_kernel(AttnK p) {
 // one 32-row tile, every key is read once, and the keys are split over the NW waves of a workgroup (each streams its own
 // tiles through its own LDS, no barriers) and over `nsplit` workgroups. The waves' results are joined in LDS, the
 // workgroups' by attn_join_kernel: O = sum_s 2^(m_s - m) O_s, l likewise.
-// Bound by reading the keys: one token against 8 x 4 heads x up to 16384 x 128 bf16, 144 MB, 34 us, 4.3 TB/s, and 4 to join.
+// Bound by reading the keys: one token against 8 x 4 heads x up to 16384 x 128 bf16, 144 MB, 34 us, 4.3 TB/s, and 5 to join.
 template <typename T, int DP, int NW, int BK>
 __global__ __launch_bounds__(NW * 64) void attn_split_kernel(AttnK p) {
   typedef AttnTile<T, DP> TL;
@@ -509,6 +510,8 @@ constexpr int rows_tile(int dp, int es) { return attn_row_bytes(dp, es) >= 512 ?
 // causal 62 and 37). fp32 heads of 65 to 96 channels, whose tiles multiply faster for as much to join, take four only up to
 // one workgroup a CU (2 x 4 x 700 x 80 causal 51 in shares of eight tiles, 32 of four; 1 x 2 x 2000 x 80 47 as 256 workgroups,
 // 52 as 480; but 3 x 3 x 500 x 3000 x 80 77 and 64).
+// attn_split_kernel's shares: 256 workgroups or the next multiple above (a workgroup's LDS lets one into a CU at a time, so
+// that group counts which do not divide 256 run a second, partly filled round; not measured), eight tiles each at least.
 static FwdPlan fwd_plan(const ifd_attention_args& a) {
   const int G = a.Hq / a.Hk, es = (int)dtype_bytes(a.dtype);
   FwdPlan r;
@@ -597,7 +600,8 @@ static int run_fwd(const FwdPlan& pl, AttnK p, hipStream_t s) {
 }
 
 // The UNet's QKVAttention (code/nn.py:222-235) on qkv [N][T][3C]: heads of 64 channels at offsets 0, C, 2C; queries and keys
-// carry `scale` each.
+// carry `scale` each. In one share however few the workgroups: an image's result then does not depend on the batch it is in,
+// and the call needs no workspace (what shares would gain at batch 1 is not measured).
 int launch_attention_rows(const float* qkv, int N, int T, int C, float scale, float* out, hipStream_t s) {
   AttnK p = {};
   p.q = (const char*)qkv; p.k = (const char*)(qkv + C); p.v = (const char*)(qkv + 2 * C);

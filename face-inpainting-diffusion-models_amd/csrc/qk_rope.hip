@@ -4,9 +4,13 @@
 //   backward: dn = the transposed rotation of dy, dw = sum dn x rstd, u = dn w, dx = rstd (u - x rstd mean(u x rstd))
 // Bound by memory: every value is read once and written once. A head's D / 2 channel pairs are spread over a group of
 // lanes, V pairs each, both members of a pair in one lane (two vector loads), so only the norm's sum crosses lanes. The
-// angle (fp64 product, whole turns dropped, fp32 sine and cosine: exact for any int64 position that fp64 holds) depends on
-// the token and the lane alone: it is computed once per token and reused for every head, and the lane groups that hold
-// different heads of a token compute a share of its V angles each and exchange them (one each for eight groups and V = 8).
+// angle depends on the token and the lane alone: it is computed once per token and reused for every head, and the lane groups
+// that hold different heads of a token compute a share of its V angles each and exchange them (one each for eight groups and
+// V = 8). It is an fp64 product whose whole and quarter turns are dropped before it is rounded to fp32 (2^-27 of a turn off
+// at most); the product's own rounding passes that beyond positions of 2^27 (2^-15 of a turn at 2^40).
+// fp32 throughout but for that: sums of D values, the hardware's reciprocal square root (1 ulp), sine and cosine. A workgroup's
+// part of dw is an fp32 sum over its tokens and heads, the workgroups' parts are added in fp64: fp32 outputs of the backward
+// are 1.1e-7 of their norm off (elementary fp32 operations with fp64 angles and sums: 6.6e-8).
 #include <type_traits>
 #include "lanes.h"
 #include "ops.h"

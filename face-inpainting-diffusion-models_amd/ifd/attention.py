@@ -11,11 +11,13 @@ three slices of a packed projection or a slice of a longer key-value cache; tens
 Row i of sequence b sees key j when j < kv_len[b] (default Tk) and, with causal=True, j <= q_start[b] + i (default
 Tk - Tq: the rows are the last ones). kv_len, q_start: int32 [B] on the GPU, read by the kernels (no synchronisation).
 Keys that no row of their sequence sees (at and past kv_len, or behind the last row's) change nothing, whatever they hold.
-A key that some rows see and others not must be finite in v (for the backward pass in k too), or it may spoil those others.
+A key that some rows see and others not must be finite in v (for the backward pass in k too), or it may spoil those others;
+so may, in the backward pass, a row that sees some keys and is not finite in q, out or dout the gradients of the others.
 A row that sees no key gets out = 0, lse = -inf and zero gradients, whatever q and dout hold there. Output tensors of the
 caller (out, dq, dk, dv) must not overlap the inputs, each other or themselves (strides must nest).
 
-The backward pass keeps no score matrix: it recomputes the probabilities from lse. Both directions are deterministic.
+The backward pass keeps no score matrix: it recomputes the probabilities from lse. Both directions are deterministic. Scores
+(scale q.k) may reach 1e8 in magnitude; from 4e8 on results are not finite. In fp16 small gradients need a loss scale.
 Calls run on the current stream of the tensors' device and can be captured into a graph. They record nothing for autograd:
 tensors that require gradients are refused unless under torch.no_grad(), tensors with a forward-mode tangent always.
 """

@@ -157,7 +157,7 @@ class UNetTrainer:
 
     state_bits=8: both AdamW moments as one byte a value and a scale per 256 values (ifd.optim.AdamW, `self.opt`): 2 bytes of
     state a parameter instead of 8; `seed` seeds their rounding. The gradients then stay unclipped in the grad buffer, a
-    step whose gradient norm is not finite is left out, and norm_coef is fp64. state_dict() holds the parameters alone, as
+    step whose gradient norm is not finite is left out (but counted), and norm_coef is fp64. state_dict() holds the parameters alone, as
     with 32 bits; `opt.state_dict()` the states and the step number: a new trainer that loads both goes on bit for bit.
 
     gnb_act (with fuse_gnb, round 6, off by default): that epilogue also writes the GroupNorm's forward output
@@ -826,7 +826,8 @@ class UNetTrainer:
         return out, ro
 
     # Tokens up to which attention keeps its probabilities (ifd_tr_attention / _bwd, 2 N heads T^2 floats of scratch in the
-    # backward); longer maps (attention at a higher resolution) run ifd.attention, whose backward recomputes them.
+    # backward); longer maps (attention at a higher resolution) run ifd.attention, whose backward recomputes them. The limit is
+    # what those kernels hold, a row of 256 scores; which side is faster below it has not been measured in the training step.
     ATTN_ROWS = 256
 
     @staticmethod

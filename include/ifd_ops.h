@@ -26,10 +26,14 @@ extern "C" {
  * Row i of sequence b sees key j when j < kv_len[b] (NULL: Tk; values are clamped to [0, Tk]) and, with causal != 0,
  * j <= q_start[b] + i (NULL: q_start = Tk - Tq). A row that sees no key gets out 0, lse -inf and no gradient, whatever q
  * and dout hold there. Keys that no row of their sequence sees (at and past kv_len, or behind the last row's) are not
- * read; their dk, dv are written as zeros. A key that some rows see must be finite in v (backward: in k too).
+ * read; their dk, dv are written as zeros. A key that some rows see must be finite in v (backward: in k too), and in the
+ * backward a row that sees some keys in q, out and dout: what is not finite there may spoil pairs that the mask leaves out
+ * (0 times it is added), besides those that it is in.
  * D <= 128 and a multiple of 8 (16-bit types) or 4 (fp32); pointers and strides in multiples of 16 bytes; scale > 0.
  * Scores, softmax statistics and every sum are fp32. The 16-bit types round P (and dS) once to the tensors' type as
- * operands of the second matrix products. */
+ * operands of the second matrix products (fp16: gradients much smaller than 1 need a loss scale, dS ends at 2^-24).
+ * |scale q.k| up to 1e8: beyond 4e8 the exponent's fp32 reference point is too coarse and results are not finite. The
+ * backward's probabilities are relatively off by up to |lse| 2^-22, the rounding of lse among it. */
 typedef struct ifd_attention_args {
   int dtype, B, Tq, Tk, Hq, Hk, D, causal;
   float scale;
@@ -94,7 +98,8 @@ int ifd_op_grad_norm(int nt, const void* const* g, const int64_t* n, const uint8
  *   at random, from seed and step).
  * norm_coef (device, from ifd_op_grad_norm) or NULL: the gradients are scaled by norm_coef[1]; a norm that is not finite
  * leaves everything as it was. Without it a gradient that is not finite spoils its parameter and state, with 8-bit states
- * the 256 values that share its scale. */
+ * the states of the 256 values that share its scale (which is NaN or infinite from then on), and with the next step their
+ * parameters. */
 typedef struct ifd_adamw_args {
   int nt, bits, step;
   uint32_t seed;
