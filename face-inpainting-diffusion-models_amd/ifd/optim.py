@@ -108,9 +108,9 @@ class AdamW:
             at += k
         if self.max_norm is not None:
             self._norm(L, arrays)
-        self.step_count += 1
+        k = self.step_count + 1
         for grp, (p, g, cnt, pt, gt) in zip(self.groups, arrays):
-            a = AdamwArgs(len(cnt), self.state_bits, self.step_count, self.seed)
+            a = AdamwArgs(len(cnt), self.state_bits, k, self.seed)
             keep = ctypes.create_string_buffer(pt, len(pt)), ctypes.create_string_buffer(gt, len(gt))
             a.p, a.g, a.n, a.ptype, a.gtype = (ctypes.addressof(x) for x in (p, g, cnt, *keep))
             a.m, a.v = self.m.data_ptr(), self.v.data_ptr()
@@ -120,6 +120,7 @@ class AdamW:
             a.eps, a.wd = self.eps, grp["weight_decay"]
             a.norm_coef = None if self.max_norm is None else self.norm_coef.data_ptr()
             call(L.ifd_op_adamw, dev, ctypes.byref(a))
+        self.step_count = k
         if any([p.requires_grad for p in self.params]):  # (autograd learns that saved parameters have changed)
             torch.autograd.graph.increment_version(self.params)
 

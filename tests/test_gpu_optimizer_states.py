@@ -79,3 +79,18 @@ def test_nan_gradient_spoils_its_8bit_block(at):
         assert torch.equal(torch.isnan(m), bad) and torch.equal(torch.isnan(v), bad), k
         spoilt = torch.isnan(p)
         assert (spoilt.sum() == 1 and spoilt[at]) if k == 1 else torch.equal(spoilt, bad[:600] & (k == 2))
+
+
+def test_a_step_that_the_library_refuses_is_not_counted():
+    """Hyperparameters are the caller's to change between steps; the library checks them at the call."""
+    from ifd.optim import AdamW
+    for bits in (8, 32):
+        p = torch.ones(300, device=DEV)
+        opt = AdamW([p], lr=1e-3, state_bits=bits)
+        opt.betas = (1.5, 0.999)
+        with pytest.raises(RuntimeError, match="b1, b2 or eps"):
+            opt.step([torch.ones_like(p)])
+        assert opt.step_count == 0 and (p == 1).all()
+        opt.betas = (0.9, 0.999)
+        opt.step([torch.ones_like(p)])
+        assert opt.step_count == 1 and (p < 1).all()
