@@ -13,8 +13,8 @@ format and its rounding are described in include/ifd_ops.h). The step uses the m
 
 With max_norm a step whose gradient norm is not finite leaves parameters and states as they were; it counts as a step all the
 same (step_count, and with it the bias corrections: the host does not learn of the norm). Without max_norm such a gradient
-spoils what ifd_op_adamw in include/ifd_ops.h says. opt.norm_coef (fp64, on the GPU) holds the norm and the clip coefficient. Nothing synchronises; a step can be captured into a graph only with its step
-number fixed, so the optimizer refuses capture.
+spoils what ifd_op_adamw in include/ifd_ops.h says. opt.norm_coef (fp64, on the GPU) holds the norm and the clip coefficient.
+Nothing synchronises; a step can be captured into a graph only with its step number fixed, so the optimizer refuses capture.
 """
 from __future__ import annotations
 

@@ -9,9 +9,9 @@ slices of a packed projection). n = x / sqrt(mean x^2 + eps) * w over each head'
 are then turned in pairs by the angle pos * inv_freq (fp64, so that far positions keep their angle) and scaled by
 rope.mscale. norm=False leaves out the norm, rope=None the rotation, wq / wk=None the weights; k=None takes queries alone.
 pos: int64 [B, T] or [T]. Statistics and products are fp32, each output is rounded once. Deterministic. An output may be the
-tensor of its own input (of its own gradient, backward) and must else overlap no input, no other output and not itself. Nothing is
-recorded for autograd: tensors that require gradients are refused unless under torch.no_grad(), those with a forward-mode
-tangent always.
+tensor of its own input (of its own gradient, backward) and must else overlap no input, no other output and not itself.
+Nothing is recorded for autograd: tensors that require gradients are refused unless under torch.no_grad(), those with a
+forward-mode tangent always.
 """
 from __future__ import annotations
 

@@ -157,8 +157,8 @@ class UNetTrainer:
 
     state_bits=8: both AdamW moments as one byte a value and a scale per 256 values (ifd.optim.AdamW, `self.opt`): 2 bytes of
     state a parameter instead of 8; `seed` seeds their rounding. The gradients then stay unclipped in the grad buffer, a
-    step whose gradient norm is not finite is left out (but counted), and norm_coef is fp64. state_dict() holds the parameters alone, as
-    with 32 bits; `opt.state_dict()` the states and the step number: a new trainer that loads both goes on bit for bit.
+    step whose gradient norm is not finite is left out (but counted), and norm_coef is fp64. state_dict() holds the parameters
+    alone, as with 32 bits; `opt.state_dict()` the states and the step number: a new trainer that loads both goes on bit for bit.
 
     gnb_act (with fuse_gnb, round 6, off by default): that epilogue also writes the GroupNorm's forward output
     silu(z) — the input of the conv whose weight gradient is next (ifd_tr_conv_x3_gnb_act) — so that weight
